@@ -289,6 +289,127 @@ int innerq_lse_merge_ranks(const float* parts, int n_ranks, int64_t rank_stride,
 int innerq_decode_attn_noalloc(const innerq_attn_args* args, void* out, int64_t o_sb,
                                int64_t o_sh, float* lse, void* stream);
 
+/*
+ * Paged 4-bit cache for continuous batching: every sequence has its own
+ * length, its own slot (16-bit sink and recent window) and its own list of
+ * pages.  Symmetric 4-bit codes in groups of 32, keys grouped over channels
+ * and values over tokens (src/innerq/quant.py:95-119 with the default axes of
+ * cache.py:87-88).  Of a sequence of L tokens the first w_sink and the last
+ * w_recent .. w_recent + 31 stay in the dtype; the
+ * n_packed = max(0, L - w_sink - w_recent) / 32 * 32 between them are in the
+ * pages.  A group that holds a value that is not finite has a NaN scale.
+ *   pages   [n_pages][Hkv][page_tiles][4608] bytes (innerq_b200/csrc/paged.cuh)
+ *   dense_k, dense_v  [n_slots][Hkv][w_sink + w_recent + 32][D] dtype
+ *   table   [B] rows (table_stride apart) of max_pages page numbers
+ *   slots, seq_lens   [B]
+ * The lengths, slots and page numbers are read on the device, so a launch can
+ * be recorded in a CUDA graph and replayed.  What they name wrongly is never
+ * read or written: a page or slot out of range drops the write, reads as NaN
+ * and makes that sequence's attention NaN.  A negative length is no tokens.
+ */
+typedef struct {
+  int32_t struct_size; /* sizeof(innerq_paged) */
+  int32_t dtype, D, Hkv;
+  int32_t page_tiles;  /* tiles of 32 tokens in a page, 1 to 64 */
+  int32_t n_pages, n_slots;
+  int32_t w_sink, w_recent; /* multiples of 32 */
+  int32_t B, max_pages;
+  void* pages;
+  void* dense_k;
+  void* dense_v;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* slots;
+  const int32_t* seq_lens;
+} innerq_paged;
+
+/* New tokens of the sequences: q [T][Hq][D], k and v [T][Hkv][D] with strides
+ * (token, head), rows contiguous and 16-byte aligned. */
+typedef struct {
+  int32_t struct_size; /* sizeof(innerq_paged_new) */
+  int32_t Hq, T;
+  int32_t rot_dim;     /* channels that are rotated: 0, or a multiple of 16 up to D */
+  int32_t interleaved; /* pairs (2i, 2i + 1) instead of (i, i + rot_dim / 2) */
+  int32_t max_pos;     /* rows of cos and sin; a position beyond them rotates to NaN */
+  const void* q;       /* NULL with Hq == 0 */
+  int64_t q_st, q_sh;
+  const void* k;
+  int64_t k_st, k_sh;
+  const void* v;
+  int64_t v_st, v_sh;
+  const int32_t* cu_seqlens; /* [B + 1] first token of each sequence, ascending from 0; NULL:
+                              * one token per sequence (T == B) */
+  const float* cos;          /* [max_pos][rot_dim / 2] fp32, rows cs_stride apart */
+  const float* sin;
+  int64_t cs_stride;
+  void* q_out;         /* rotated queries */
+  int64_t qo_st, qo_sh;
+  void* k_out;         /* rotated keys in the dtype (for attention over the prompt), or NULL */
+  int64_t ko_st, ko_sh;
+} innerq_paged_new;
+
+/*
+ * Append new tokens: rotate q and k by their positions (seq_lens[b] is the
+ * length BEFORE the call, the position of sequence b's first new token), write
+ * k and v to the sink / window, and quantize and pack the tiles that leave the
+ * window.  The pages a sequence needs for its new length must be in its row of
+ * the table.  One launch for one token per sequence, else two.
+ */
+int innerq_paged_append(const innerq_paged* cache, const innerq_paged_new* tokens, void* stream);
+
+/*
+ * What the cache holds for tokens starts[b] .. of each sequence, dequantized
+ * and rounded to the dtype: token cu_seqlens[b] + i of k_out / v_out
+ * [n_tokens][Hkv][D] is token starts[b] + i of sequence b (seq_lens: the
+ * lengths now).  Positions outside a sequence read as NaN.
+ */
+int innerq_paged_read(const innerq_paged* cache, const int32_t* starts, const int32_t* cu_seqlens,
+                      int n_tokens, void* k_out, void* v_out, void* stream);
+
+/*
+ * Decode attention over the paged cache, one query token per sequence:
+ *   out[b][hq] = softmax(q[b][hq] . K[b][hq / (Hq / Hkv)]^T * scale) V
+ * over all seq_lens[b] tokens; zeros (and lse -inf) for a sequence without
+ * tokens.  Hq / Hkv from 1 to 8.  lse (nullable, [B][Hq] fp32): log2-sum-exp2
+ * of the scaled logits.  workspace: innerq_paged_attn_workspace bytes, 16-byte
+ * aligned, contents irrelevant.
+ */
+int64_t innerq_paged_attn_workspace(const innerq_paged* cache, int Hq);
+int innerq_paged_attn(const innerq_paged* cache, int Hq, const void* q, int64_t q_sb, int64_t q_sh,
+                      float scale, void* workspace, int64_t workspace_bytes, void* out, int64_t o_sb,
+                      int64_t o_sh, float* lse, void* stream);
+
+/*
+ * Attention of whole prompts packed one behind the other: queries
+ * q [Tq][Hq][D], keys and values [Tk][Hkv][D], sequence b's at tokens
+ * cu_q[b] .. cu_q[b + 1] and cu_k[b] .. cu_k[b + 1].  Causal: query i of a
+ * sequence of nq queries and nk keys sees keys j <= i + nk - nq, so a chunk of
+ * a prompt sees the tokens before it.  A query that sees no key gets zeros and
+ * lse -inf.  What is masked (later tokens, other sequences) never reaches a
+ * result, whatever bits it holds.  Hq any multiple of Hkv.  The lengths are
+ * read on the device.
+ */
+typedef struct {
+  int32_t struct_size; /* sizeof(innerq_prompt_args) */
+  int32_t dtype, D, B, Hq, Hkv;
+  int32_t Tq, Tk;      /* rows of q and of k, v */
+  int32_t causal;
+  float scale;
+  const void* q;       /* strides (token, head) in elements; rows contiguous, 16-byte aligned */
+  int64_t q_st, q_sh;
+  const void* k;
+  int64_t k_st, k_sh;
+  const void* v;
+  int64_t v_st, v_sh;
+  const int32_t* cu_q; /* [B + 1] */
+  const int32_t* cu_k; /* [B + 1] */
+  void* out;           /* [Tq][Hq][D] */
+  int64_t o_st, o_sh;
+  float* lse;          /* nullable, [Tq][Hq] log2-sum-exp2 of the scaled logits */
+} innerq_prompt_args;
+
+int innerq_prompt_attn(const innerq_prompt_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,7 +12,7 @@ Compute runs in ``libinnerq_b200.so`` (hand-written CUDA for sm_100a, C ABI in
 """
 from . import _lib  # noqa: F401
 
-__all__ = ["quant", "cache", "models", "attention", "store"]
+__all__ = ["quant", "cache", "models", "attention", "store", "paged", "prompt"]
 
 
 def __getattr__(name):

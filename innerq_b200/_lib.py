@@ -22,7 +22,8 @@ EXPORTS = (
     "innerq_quant_pack", "innerq_unpack_ref", "innerq_dequant", "innerq_attn_plan",
     "innerq_decode_attn_workspace", "innerq_decode_attn", "innerq_decode_attn_partials",
     "innerq_lse_merge", "innerq_dequant_ref", "innerq_decode_attn_noalloc", "innerq_append_step",
-    "innerq_partials_rank_floats", "innerq_lse_merge_ranks",
+    "innerq_partials_rank_floats", "innerq_lse_merge_ranks", "innerq_paged_append",
+    "innerq_paged_read", "innerq_paged_attn_workspace", "innerq_paged_attn", "innerq_prompt_attn",
 )
 
 
@@ -77,6 +78,43 @@ class AttnArgs(C.Structure):
     ]
 
 
+class Paged(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32), ("dtype", C.c_int32), ("D", C.c_int32), ("Hkv", C.c_int32),
+        ("page_tiles", C.c_int32), ("n_pages", C.c_int32), ("n_slots", C.c_int32),
+        ("w_sink", C.c_int32), ("w_recent", C.c_int32), ("B", C.c_int32), ("max_pages", C.c_int32),
+        ("pages", C.c_void_p), ("dense_k", C.c_void_p), ("dense_v", C.c_void_p),
+        ("table", C.c_void_p), ("table_stride", C.c_int64),
+        ("slots", C.c_void_p), ("seq_lens", C.c_void_p),
+    ]
+
+
+class PagedNew(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32), ("Hq", C.c_int32), ("T", C.c_int32), ("rot_dim", C.c_int32),
+        ("interleaved", C.c_int32), ("max_pos", C.c_int32),
+        ("q", C.c_void_p), ("q_st", C.c_int64), ("q_sh", C.c_int64),
+        ("k", C.c_void_p), ("k_st", C.c_int64), ("k_sh", C.c_int64),
+        ("v", C.c_void_p), ("v_st", C.c_int64), ("v_sh", C.c_int64),
+        ("cu_seqlens", C.c_void_p), ("cos", C.c_void_p), ("sin", C.c_void_p), ("cs_stride", C.c_int64),
+        ("q_out", C.c_void_p), ("qo_st", C.c_int64), ("qo_sh", C.c_int64),
+        ("k_out", C.c_void_p), ("ko_st", C.c_int64), ("ko_sh", C.c_int64),
+    ]
+
+
+class PromptArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_int32), ("dtype", C.c_int32), ("D", C.c_int32), ("B", C.c_int32),
+        ("Hq", C.c_int32), ("Hkv", C.c_int32), ("Tq", C.c_int32), ("Tk", C.c_int32),
+        ("causal", C.c_int32), ("scale", C.c_float),
+        ("q", C.c_void_p), ("q_st", C.c_int64), ("q_sh", C.c_int64),
+        ("k", C.c_void_p), ("k_st", C.c_int64), ("k_sh", C.c_int64),
+        ("v", C.c_void_p), ("v_st", C.c_int64), ("v_sh", C.c_int64),
+        ("cu_q", C.c_void_p), ("cu_k", C.c_void_p),
+        ("out", C.c_void_p), ("o_st", C.c_int64), ("o_sh", C.c_int64), ("lse", C.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -112,6 +150,12 @@ def load() -> C.CDLL:
         "innerq_lse_merge": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, i64, vp, vp]),
         "innerq_partials_rank_floats": (i64, [i32, i32, i32, i32]),
         "innerq_lse_merge_ranks": (i32, [vp, i32, i64, i32, i32, i32, i32, i32, vp, i64, i64, vp, vp]),
+        "innerq_paged_append": (i32, [C.POINTER(Paged), C.POINTER(PagedNew), vp]),
+        "innerq_paged_read": (i32, [C.POINTER(Paged), vp, vp, i32, vp, vp, vp]),
+        "innerq_paged_attn_workspace": (i64, [C.POINTER(Paged), i32]),
+        "innerq_paged_attn": (i32, [C.POINTER(Paged), i32, vp, i64, i64, C.c_float, vp, i64, vp, i64, i64,
+                                    vp, vp]),
+        "innerq_prompt_attn": (i32, [C.POINTER(PromptArgs), vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(lib, name)
@@ -128,7 +172,8 @@ KERNELS_PER_CALL = {
     "innerq_norm_factor": 1, "innerq_quant_pack": 1, "innerq_unpack_ref": 1, "innerq_dequant": 1,
     "innerq_dequant_ref": 1, "innerq_decode_attn": 3, "innerq_decode_attn_partials": 2,
     "innerq_lse_merge": 1, "innerq_decode_attn_noalloc": 3, "innerq_append_step": 1,
-    "innerq_lse_merge_ranks": 1,
+    "innerq_lse_merge_ranks": 1, "innerq_paged_append": 1, "innerq_paged_read": 1,
+    "innerq_paged_attn": 1, "innerq_prompt_attn": 1,
 }
 launch_count = [0]
 

@@ -1,0 +1,368 @@
+"""The paged 4-bit cache (append with rotation, read-back, ragged decode
+attention) against a plain implementation in 64 bits that decodes the page
+format token by token."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
+ULP = {"fp16": 2.0 ** -11, "bf16": 2.0 ** -8}  # half a step of the type, relative
+
+
+class Oracle:
+    """Keys and values of sequences in numpy: what each token is held as."""
+
+    def __init__(self, sink, recent, dt):
+        self.sink, self.recent, self.dt = sink, recent, dt
+        self.k, self.v = {}, {}  # sequence -> [n, H, D] in the type, rotated
+        self.ck, self.cv = {}, {}  # what the cache holds, float64
+
+    def rnd(self, x):
+        return torch.from_numpy(np.asarray(x, np.float32)).to(self.dt).float().numpy()
+
+    def packed(self, n):
+        return max(0, n - self.sink - self.recent) // 32 * 32
+
+    def group(self, x, axis):
+        """A tile quantized in groups of 32 along axis (whole axis in groups), as float64."""
+        x = np.moveaxis(x.astype(np.float32), axis, -1)
+        g = x.reshape(x.shape[:-1] + (-1, 32))
+        with np.errstate(all="ignore"):
+            top = np.abs(g).max(-1, keepdims=True)
+            scale = self.rnd(top / np.float32(7))
+            q = self.rnd(np.abs(g) / scale)
+            c = np.rint(np.clip(np.nan_to_num(q, nan=0.0, posinf=7.0), 0, 7)) * np.sign(np.nan_to_num(g))
+            good = np.isfinite(top)
+            val = np.where(good, c, 0) * np.where(good, scale, np.nan).astype(np.float64)
+        return np.moveaxis(val.reshape(x.shape), -1, axis)
+
+    def append(self, b, k, v):
+        """k (rotated) and v [n, H, D] in the type, as float32."""
+        old = self.k[b].shape[0] if b in self.k else 0
+        cat = lambda d, x: np.concatenate([d[b], x]) if b in d else x  # noqa: E731
+        self.k[b], self.v[b] = cat(self.k, k), cat(self.v, v)
+        self.ck[b], self.cv[b] = cat(self.ck, k.astype(np.float64)), cat(self.cv, v.astype(np.float64))
+        lo, hi = self.packed(old), self.packed(self.k[b].shape[0])
+        for t in range(self.sink + lo, self.sink + hi, 32):
+            self.ck[b][t:t + 32] = self.group(self.k[b][t:t + 32], 2)
+            self.cv[b][t:t + 32] = self.group(self.v[b][t:t + 32], 0)
+
+    def attend(self, b, q, scale):
+        """q [Hq, D] float -> out [Hq, D], lse (base 2)."""
+        k, v = self.ck[b], self.cv[b]
+        R = q.shape[0] // k.shape[1]
+        out = np.zeros(q.shape)
+        lse = np.full(q.shape[0], -np.inf)
+        for h in range(q.shape[0]):
+            s = k[:, h // R] @ q[h].astype(np.float64) * scale
+            if len(s):
+                m = s.max()
+                p = np.exp(s - m)
+                out[h] = p @ v[:, h // R] / p.sum()
+                lse[h] = (m + np.log(p.sum())) / math.log(2)
+        return out, lse
+
+
+def rotate64(x, cos, sin, interleaved):
+    """x [n, H, D] float32, cos / sin [n, rot / 2]: fp32 products and sums."""
+    x = x.astype(np.float32)
+    r = 2 * cos.shape[1]
+    c, s = cos[:, None].astype(np.float32), sin[:, None].astype(np.float32)
+    y = x.copy()
+    a, b = (x[..., 0:r:2], x[..., 1:r:2]) if interleaved else (x[..., :r // 2], x[..., r // 2:r])
+    p, q = a * c - b * s, b * c + a * s
+    if interleaved:
+        y[..., 0:r:2], y[..., 1:r:2] = p, q
+    else:
+        y[..., :r // 2], y[..., r // 2:r] = p, q
+    return y
+
+
+def table(n, rot):
+    ang = np.arange(n)[:, None] * 10000.0 ** -(np.arange(0, rot, 2) / rot)
+    return np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
+
+
+class Server:
+    """A PagedCache driven like a scheduler does, next to its oracle."""
+
+    def __init__(self, n_seq, hkv, dt, sink, recent, page, max_len, seed=0, rot=128, interleaved=False):
+        from innerq_b200.paged import PagedCache
+        self.r = np.random.RandomState(seed)
+        self.g = torch.Generator(device="cuda").manual_seed(seed)
+        self.dt, self.hkv = DT[dt], hkv
+        cols = max(1, -(-max_len // page))
+        self.cache = PagedCache.allocate(n_seq * cols + 2, hkv, n_seq + 2, page, sink, recent, self.dt)
+        self.cache.pages.fill_(0x5A)
+        for d in (self.cache.dense_k, self.cache.dense_v):
+            d.fill_(float("nan"))  # what was never written must never be seen
+        self.table = torch.from_numpy(self.r.permutation(n_seq * cols + 2)[:n_seq * cols].reshape(n_seq, cols)
+                                      .astype(np.int32)).cuda()
+        self.slots = torch.from_numpy(self.r.permutation(n_seq + 2)[:n_seq].astype(np.int32)).cuda()
+        self.lens = np.zeros(n_seq, np.int32)
+        self.oracle = Oracle(sink, recent, self.dt)
+        self.rot, self.interleaved = rot, interleaved
+        self.cos, self.sin = table(max_len + 1, rot) if rot else (None, None)
+        self.size = torch.exp(torch.randn((hkv, D), device="cuda", generator=self.g))
+
+    def dev(self, x):
+        return torch.from_numpy(np.asarray(x, np.int32)).cuda()
+
+    def step(self, new, hq=0, seqs=None, one=False, kv=None):
+        """Append new[i] tokens to sequence seqs[i]; returns (got q, expected q)."""
+        seqs = np.arange(len(new)) if seqs is None else np.asarray(seqs)
+        T = int(np.sum(new))
+        x = torch.randn((T, hq + 2 * self.hkv, D), device="cuda", generator=self.g)
+        x[:, hq:hq + self.hkv] *= self.size
+        x = x.to(self.dt)
+        if kv is not None:
+            kv(x[:, hq:hq + self.hkv], x[:, hq + self.hkv:])
+        at = torch.from_numpy(seqs).cuda()
+        cs = dict(cos=torch.from_numpy(self.cos).cuda(), sin=torch.from_numpy(self.sin).cuda(),
+                  interleaved=self.interleaved) if self.rot else {}
+        q, k = self.cache.append(x[:, :hq] if hq else None, x[:, hq:hq + self.hkv], x[:, hq + self.hkv:], self.table[at],
+                                 self.slots[at], self.dev(self.lens[seqs]),
+                                 None if one else self.dev(np.concatenate([[0], np.cumsum(new)])), return_k=True, **cs)
+        n = x.float().cpu().numpy()
+        pos = np.concatenate([self.lens[b] + np.arange(c) for b, c in zip(seqs, new)] + [np.zeros(0, np.int64)]).astype(int)
+        turn = lambda y: self.oracle.rnd(rotate64(y, self.cos[pos], self.sin[pos], self.interleaved)) if self.rot else y  # noqa: E731
+        wq, wk = turn(n[:, :hq]), turn(n[:, hq:hq + self.hkv])
+        o = 0
+        for b, c in zip(seqs, new):
+            self.oracle.append(b, wk[o:o + c], n[o:o + c, hq + self.hkv:])
+            self.lens[b] += c
+            o += c
+        np.testing.assert_array_equal(k.float().cpu().numpy(), wk)
+        if hq:
+            np.testing.assert_array_equal(q.float().cpu().numpy(), wq)
+
+    def check_read(self, seqs=None):
+        """Every token of the sequences reads back as the oracle holds it, bit for bit."""
+        seqs = np.arange(len(self.lens)) if seqs is None else np.asarray(seqs)
+        n = self.lens[seqs]
+        at = torch.from_numpy(seqs).cuda()
+        k, v = self.cache.read(self.table[at], self.slots[at], self.dev(n), self.dev(np.zeros_like(n)),
+                               self.dev(np.concatenate([[0], np.cumsum(n)])), int(n.sum()))
+        o = 0
+        for b, c in zip(seqs, n):
+            if c:
+                np.testing.assert_array_equal(k[o:o + c].float().cpu().numpy(), self.oracle.rnd(self.oracle.ck[b]))
+                np.testing.assert_array_equal(v[o:o + c].float().cpu().numpy(), self.oracle.rnd(self.oracle.cv[b]))
+            o += c
+
+    def check_attend(self, hq, seqs=None, scale=None, dtype="fp16"):
+        seqs = np.arange(len(self.lens)) if seqs is None else np.asarray(seqs)
+        at = torch.from_numpy(seqs).cuda()
+        q = torch.randn((len(seqs), hq, D), device="cuda", generator=self.g).to(self.dt)
+        lse = torch.full((len(seqs), hq), 7.0, device="cuda")
+        out = self.cache.attend(q, self.table[at], self.slots[at], self.dev(self.lens[seqs]), scale=scale, lse=lse)
+        for i, b in enumerate(seqs):
+            if b not in self.oracle.k:
+                self.oracle.k[b] = self.oracle.v[b] = np.zeros((0, self.hkv, D), np.float32)
+                self.oracle.ck[b] = self.oracle.cv[b] = np.zeros((0, self.hkv, D))
+            want, wl = self.oracle.attend(b, q[i].float().cpu().numpy(), scale if scale is not None else D ** -0.5)
+            close(out[i].double().cpu().numpy(), want, dtype, np.abs(np.nan_to_num(self.oracle.cv[b], nan=0, posinf=0, neginf=0)).max() if self.lens[b] else 1.0)
+            np.testing.assert_allclose(lse[i].cpu().numpy(), wl, rtol=1e-5, atol=2e-3)
+
+
+def close(got, want, dtype, vmax):
+    """Each probability is rounded to 11 bits or more before it meets the
+    values: an error of at most 2^-11 sum p |v| <= 2^-11 max |v|, and the
+    output is rounded to its type."""
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    err = np.nan_to_num(np.abs(got - want))
+    bound = ULP[dtype] * np.abs(np.nan_to_num(want)) + 2.0 ** -11 * vmax
+    assert (err <= bound).all(), (err.max(), bound.flat[err.argmax()])
+
+
+@pytest.mark.parametrize("dtype,hkv,hq,sink,recent,page,rot,inter", [
+    ("fp16", 2, 8, 32, 96, 64, 128, False),
+    ("bf16", 1, 5, 0, 0, 32, 64, False),
+    ("fp16", 3, 3, 64, 32, 128, 128, True),
+    ("bf16", 2, 14, 32, 0, 256, 32, True),
+    ("fp16", 1, 8, 0, 32, 32, 0, False),
+])
+def test_prompts_then_decode(dtype, hkv, hq, sink, recent, page, rot, inter):
+    """Ragged prompts (one of no tokens, one of one), chunks of them, then
+    single tokens across several flushes; everything read back bit for bit and
+    attended to."""
+    s = Server(5, hkv, dtype, sink, recent, page, 700, seed=hq, rot=rot, interleaved=inter)
+    s.step([1, 0, 33, 257, 128], hq)
+    s.check_read()
+    s.step([70, 5, 64, 130, 31], hq)  # chunks that begin anywhere
+    s.check_read()
+    s.check_attend(hq, dtype=dtype)
+    for i in range(70):
+        s.step([1] * 5, hq, one=True)
+        if i % 23 == 0:
+            s.check_read()
+    s.check_read()
+    s.check_attend(hq, dtype=dtype)
+
+
+@pytest.mark.parametrize("length", [0, 1, 2, 31, 32, 33, 63, 64, 65, 95, 96, 97, 127, 128, 129, 160, 161, 191, 192, 193, 1000])
+def test_every_length_near_the_seams(length):
+    s = Server(2, 1, "fp16", 32, 32, 64, 1100, seed=length)
+    s.step([length, 5], 4)
+    s.check_read()
+    s.check_attend(4)
+
+
+@pytest.mark.parametrize("ratio", [1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_head_ratios(ratio, dtype):
+    s = Server(3, 2, dtype, 32, 32, 32, 900, seed=ratio)
+    s.step([300, 801, 40], 2 * ratio)
+    s.check_attend(2 * ratio, dtype=dtype)
+
+
+def test_subset_order_and_scale():
+    """Rows of a batch are any sequences in any order, one of them unused."""
+    s = Server(6, 2, "fp16", 32, 96, 64, 3000, seed=3)
+    s.step([2500, 10, 600, 0, 77, 1203], 8)
+    s.check_attend(8, seqs=[5, 0, 3, 2])
+    s.check_attend(8, seqs=[4], scale=0.3)
+    s.check_attend(8, seqs=[0, 1], scale=0.0)
+    s.check_attend(8, seqs=[0, 1], scale=-0.1)
+
+
+def test_long_and_many():
+    """Work split over many blocks, and many short sequences."""
+    s = Server(1, 1, "fp16", 32, 96, 128, 40000, seed=4)
+    s.step([39001], 4)
+    s.check_attend(4)
+    n = np.random.RandomState(5).randint(0, 150, 300)
+    s = Server(300, 1, "bf16", 0, 32, 32, 160, seed=5)
+    s.step(n, 2)
+    s.check_attend(2, dtype="bf16")
+
+
+def test_values_that_are_not_finite_stay_in_their_groups():
+    """A NaN or an infinity in a quantized group makes that group NaN (key:
+    32 channels of a token; value: one channel of 32 tokens) and nothing else;
+    the attention is NaN exactly where the formula says."""
+    s = Server(2, 1, "fp16", 0, 0, 32, 400, seed=6, rot=0)
+
+    def poison(k, v):
+        v[40, 0, 7] = float("inf")
+        v[100, 0, 9] = float("nan")
+    s.step([200, 90], 2, kv=poison)
+    s.check_read()
+    s.check_attend(2)
+
+    def poison_key(k, v):
+        k[5, 0, 70] = float("-inf")
+    s.step([64, 64], 2, kv=poison_key)
+    s.check_read()
+    s.check_attend(2, seqs=[1])
+
+
+def test_zero_groups_and_extremes():
+    """Groups of zeros, of the type's smallest and largest values."""
+    s = Server(1, 1, "fp16", 0, 0, 32, 200, seed=7, rot=0)
+
+    def edge(k, v):
+        k[:32] = 0
+        v[32:64] = 0
+        k[64:96] *= 2.0 ** -24 / k[64:96].abs().clamp(min=2.0 ** -24)
+        v[96:128, 0, :5] = 65504.0
+    s.step([160], 2, kv=edge)
+    s.check_read()
+
+
+def test_strided_inputs_and_streams():
+    """Slices of a fused projection with an odd width, work on a stream of its
+    own, outputs into a strided view."""
+    from innerq_b200.paged import PagedCache
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn((3, 4 + 2 + 2 + 1, 136), device="cuda", generator=g).half()
+    args = dict(page_table=torch.zeros((3, 1), dtype=torch.int32, device="cuda"),
+                slots=torch.arange(3, dtype=torch.int32, device="cuda"))
+    zero = torch.zeros(3, dtype=torch.int32, device="cuda")
+    outs = []
+    for contiguous in (False, True):
+        c = PagedCache.allocate(1, 2, 3, 32, 0, 32)
+        y = x[..., 3:131]  # rows that begin inside a 16-byte word
+        q, k, v = y[:, :4], y[:, 4:6], y[:, 6:8]
+        if contiguous:
+            q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            qr = c.append(q, k, v, seq_lens=zero, **args)
+            wide = torch.zeros((3, 4, 256), dtype=torch.float16, device="cuda")
+            out = c.attend(qr, seq_lens=zero + 1, out=wide[..., 64:192], **args)
+        torch.cuda.current_stream().wait_stream(st)
+        assert torch.equal(qr, q) and (wide[..., :64] == 0).all() and (wide[..., 192:] == 0).all()
+        outs.append(out.clone())
+        want = v.repeat_interleave(2, 1)  # one token: its value
+        assert torch.equal(out, want)
+    assert torch.equal(*outs)
+
+
+def test_names_out_of_range_are_nan_and_write_nothing():
+    """A page, slot or position that does not exist: NaN, nothing written."""
+    from innerq_b200.paged import PagedCache
+    c = PagedCache.allocate(2, 1, 1, 32, 0, 0)
+    c.pages.zero_(), c.dense_k.zero_(), c.dense_v.zero_()
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn((70, 4, 128), device="cuda", generator=g).half()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    for tab, slot in ((i32(0, 1), 3), (i32(7, -1), 0)):
+        c.append(x[:, :2], x[:, 2:3], x[:, 3:], tab[None], i32(slot), i32(0), i32(0, 70))
+        if slot:
+            assert int(c.pages.count_nonzero()) == 0 and int(c.dense_k.count_nonzero()) == 0
+        assert torch.isnan(c.attend(x[:1, :2], tab[None], i32(slot), i32(70))).all()
+    # more tokens than the table has pages for
+    assert torch.isnan(c.attend(x[:1, :2], i32(0)[None], i32(0), i32(100))).all()
+    assert torch.equal(c.attend(x[:1, :2], i32(0)[None], i32(0), i32(-5)), torch.zeros_like(x[:1, :2]))
+    cs = torch.ones((10, 64), device="cuda")
+    q = c.append(x[:12, :2], x[:12, 2:3], x[:12, 3:], i32(0, 1)[None], i32(0), i32(0), i32(0, 12), cos=cs, sin=cs)
+    assert torch.isnan(q[10:]).all() and not torch.isnan(q[:10]).any()
+    k, v = c.read(i32(0, 1)[None], i32(0), i32(12), i32(-1), i32(0, 14), 14)
+    bad = torch.isnan(k).all(-1)[:, 0]
+    assert bad.tolist() == [True] + [False] * 10 + [True] * 3  # 10, 11: keys without an angle
+    assert torch.isnan(v).all(-1)[:, 0].tolist() == [True] + [False] * 12 + [True]
+
+
+def test_decode_step_in_a_graph():
+    """Append and attend recorded once, replayed while the lengths move on the device."""
+    s = Server(3, 2, "fp16", 32, 32, 64, 500, seed=10)
+    s.step([100, 37, 250], 8)
+    lens = s.dev(s.lens)
+    x = torch.empty((3, 12, D), dtype=torch.float16, device="cuda")
+    out = torch.empty((3, 8, D), dtype=torch.float16, device="cuda")
+    cos, sin = torch.from_numpy(s.cos).cuda(), torch.from_numpy(s.sin).cuda()
+
+    def one():
+        q = s.cache.append(x[:, :8], x[:, 8:10], x[:, 10:], s.table, s.slots, lens, cos=cos, sin=sin)
+        lens.add_(1)
+        s.cache.attend(q, s.table, s.slots, lens, out=out)
+    x.normal_()
+    keep = [t.clone() for t in (s.cache.pages, s.cache.dense_k, s.cache.dense_v, lens)]
+    one()  # warm-up, undone
+    for a, b in zip((s.cache.pages, s.cache.dense_k, s.cache.dense_v, lens), keep):
+        a.copy_(b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one()
+    for i in range(40):
+        x.normal_()
+        graph.replay()
+        n = x.float().cpu().numpy()
+        pos = s.lens.astype(int)
+        rot = lambda y: s.oracle.rnd(rotate64(y, s.cos[pos], s.sin[pos], False))  # noqa: E731
+        q, k = rot(n[:, :8]), rot(n[:, 8:10])
+        for b in range(3):
+            s.oracle.append(b, k[b:b + 1], n[b:b + 1, 10:])
+            s.lens[b] += 1
+        if i % 13 == 0 or i == 39:
+            for b in range(3):
+                want, _ = s.oracle.attend(b, q[b], D ** -0.5)
+                close(out[b].double().cpu().numpy(), want, "fp16", np.abs(s.oracle.cv[b]).max())
+    s.check_read()

@@ -1,0 +1,179 @@
+"""Attention over packed prompts against the formula in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
+ULP = {"fp16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+def cu(n):
+    return torch.from_numpy(np.concatenate([[0], np.cumsum(n)]).astype(np.int32)).cuda()
+
+
+def reference(q, k, v, nq, nk, causal, scale):
+    """out [Tq, Hq, D], lse [Tq, Hq] (base 2), the largest |v| a row can see [Tq, Hq], in float64."""
+    q, k, v = q.double(), k.double(), v.double()
+    R = q.shape[1] // k.shape[1]
+    out, lse = torch.zeros_like(q), torch.full(q.shape[:2], float("-inf"), dtype=torch.float64, device=q.device)
+    vmax = torch.zeros_like(lse)
+    o = p = 0
+    for a, b in zip(nq, nk):
+        if a and b:
+            kk, vv = (x[p:p + b].repeat_interleave(R, 1).transpose(0, 1) for x in (k, v))
+            i, j = torch.arange(a, device=q.device)[:, None], torch.arange(b, device=q.device)
+            seen = (j <= i + b - a) if causal else torch.ones((a, b), dtype=torch.bool, device=q.device)
+            s = (q[o:o + a].transpose(0, 1) @ kk.transpose(1, 2)) * scale
+            s = torch.where(seen, s, float("-inf"))  # whatever is there
+            m = s.amax(-1, keepdim=True)
+            e = torch.where(seen & (m > float("-inf")), torch.exp(s - m), torch.where(torch.isnan(m) & seen, m, 0.0))
+            l = e.sum(-1, keepdim=True)
+            w = torch.where(l == 0, 0.0, e / torch.where(l == 0, 1.0, l))
+            for r0 in range(0, a, 256):  # a masked value does not count, a seen one does even with weight 0
+                ww, ss = w[:, r0:r0 + 256], seen[r0:r0 + 256]
+                bad = ~torch.isfinite(vv)
+                res = ww @ torch.where(bad, 0.0, vv)
+                if bad.any():
+                    hit = ss.double() @ bad.double()
+                    for h in range(q.shape[1]):
+                        for r, d in zip(*torch.nonzero(hit[h], as_tuple=True)):
+                            res[h, r, d] = (ww[h, r, ss[r]] * vv[h, ss[r], d]).sum()
+                out[o + r0:o + min(a, r0 + 256)] = res.transpose(0, 1)
+            lse[o:o + a] = ((m + torch.log(l)) / np.log(2.0))[..., 0].T
+            vmax[o:o + a] = torch.nan_to_num(vv, 0, 0, 0).abs().amax((1, 2))[None].expand(a, -1)
+        o, p = o + a, p + b
+    return out, lse, vmax
+
+
+def check(q, k, v, nq, nk, causal, dtype, scale=None, **kw):
+    from innerq_b200.prompt import prompt_attention
+    lse = torch.full(q.shape[:2], 3.0, device="cuda")
+    out = prompt_attention(q, k, v, cu(nq), None if nk is nq else cu(nk), scale=scale, causal=causal, lse=lse, **kw)
+    want, wl, vmax = reference(q, k, v, nq, nk, causal, D ** -0.5 if scale is None else scale)
+    n = int(sum(nq))
+    got, want, wl, vmax = out[:n].double(), want[:n], wl[:n], vmax[:n]
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    # probabilities are rounded to the type before they meet the values, the
+    # output is rounded to its type
+    err = torch.nan_to_num(got - want).abs()
+    bound = ULP[dtype] * (torch.nan_to_num(want).abs() + vmax[..., None])
+    assert bool((err <= bound).all()), float((err - bound).max())
+    fine = torch.isfinite(wl)
+    assert torch.equal(torch.isneginf(lse[:n]), torch.isneginf(wl))
+    assert bool(((lse[:n].double() - wl)[fine].abs() <= 2e-3 + 1e-5 * wl[fine].abs()).all())
+    return out
+
+
+def data(nq, nk, hq, hkv, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda n, h: torch.randn((int(sum(n)), h, D), device="cuda", generator=g).to(DT[dtype])  # noqa: E731
+    return r(nq, hq), r(nk, hkv), r(nk, hkv)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n", [[1], [2, 1, 3], [127], [128], [129], [255, 1, 257], [0, 300, 0, 64, 1, 0], [513, 40], [1030]])
+def test_lengths(n, causal, dtype):
+    q, k, v = data(n, n, 4, 2, dtype, seed=sum(n))
+    check(q, k, v, n, n, causal, dtype)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 3), (6, 2), (5, 1), (8, 8), (16, 2), (40, 8), (7, 1), (20, 1)])
+def test_heads(hq, hkv):
+    n = [200, 77]
+    q, k, v = data(n, n, hq, hkv, "fp16", seed=hq)
+    check(q, k, v, n, n, True, "fp16")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("nq,nk", [([1], [1000]), ([1, 1, 1], [5, 300, 129]), ([64, 200], [1000, 200]), ([130, 5], [131, 900]),
+                                   ([10, 300, 8], [4, 100, 0]), ([300], [1]), ([257, 0, 3], [130, 50, 3])])
+def test_keys_longer_or_shorter_than_queries(nq, nk, causal):
+    """A chunk sees what came before it; more queries than keys leave rows
+    that see nothing: zeros."""
+    q, k, v = data(nq, nk, 4, 2, "bf16", seed=sum(nq) + sum(nk))
+    check(q, k, v, nq, nk, causal, "bf16")
+
+
+def test_long():
+    n = [5000, 1, 3001]
+    q, k, v = data(n, n, 2, 1, "fp16", seed=1)
+    check(q, k, v, n, n, True, "fp16")
+
+
+@pytest.mark.parametrize("scale", [0.0, 1.0, -0.05, 3e-3])
+def test_scales(scale):
+    """Peaked and flat distributions; logits far beyond the exponent's range."""
+    n = [300, 170]
+    q, k, v = data(n, n, 2, 2, "fp16", seed=2)
+    check(q * 4, k, v, n, n, True, "fp16", scale=scale)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_masked_places_may_hold_anything(bad, dtype):
+    """Values and keys that are not finite reach exactly the queries that see
+    them: not earlier tokens, not the neighbouring sequences."""
+    n = [200, 140, 300]
+    q, k, v = data(n, n, 2, 1, dtype, seed=3)
+    v[200 + 139] = bad  # the last token of the second sequence
+    v[50, 0, 3] = bad
+    check(q, k, v, n, n, True, dtype)
+    q, k, v = data(n, n, 2, 1, dtype, seed=4)
+    k[150] = float("nan")
+    check(q, k, v, n, n, True, dtype)
+    q, k, v = data(n, n, 2, 1, dtype, seed=5)
+    k[199, 0] = float("nan")
+    v[199, 0] = bad
+    check(q, k, v, n, n, True, dtype)
+
+
+def test_rising_logits():
+    """A running maximum that grows from key to key by more than any
+    deferred rescaling allows."""
+    n = [700]
+    q, k, v = data(n, n, 2, 1, "bf16", seed=6)
+    q[:] = 1.0
+    k[:] = (torch.arange(700, device="cuda") / 8.0)[:, None, None].to(torch.bfloat16)
+    check(q, k, v, n, n, True, "bf16", scale=0.25)
+    check(q, k, v, n, n, True, "bf16", scale=-0.25)
+
+
+def test_rows_past_the_last_sequence_are_left_alone():
+    n = [100, 60]
+    q, k, v = data([200], [200], 2, 1, "fp16", seed=7)
+    k[160:], v[160:] = float("nan"), float("nan")
+    out = torch.full((200, 2, D), 5.0, dtype=torch.float16, device="cuda")
+    check(q, k, v, n, n, True, "fp16", out=out)
+    assert (out[160:] == 5).all()
+
+
+def test_strides_and_streams():
+    """q, k, v as slices of one projection; a stream of its own; out strided."""
+    from innerq_b200.prompt import prompt_attention
+    n = [130, 31]
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn((161, 8, 144), device="cuda", generator=g).half()
+    for view in (x[..., :128], x[..., 8:136], x[..., 5:133]):
+        q, k, v = view[:, :4], view[:, 4:6], view[:, 6:]
+        wide = torch.zeros((161, 4, 256), dtype=torch.float16, device="cuda")
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            prompt_attention(q, k, v, cu(n), out=wide[..., 64:192])
+        torch.cuda.current_stream().wait_stream(st)
+        want = prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu(n))
+        assert torch.equal(wide[..., 64:192], want)
+        assert (wide[..., :64] == 0).all() and (wide[..., 192:] == 0).all()
+    check(q.contiguous(), k.contiguous(), v.contiguous(), n, n, True, "fp16")
+
+
+def test_same_inputs_same_bits():
+    from innerq_b200.prompt import prompt_attention
+    n = [1000, 333]
+    q, k, v = data(n, n, 4, 2, "bf16", seed=9)
+    a = prompt_attention(q, k, v, cu(n))
+    assert torch.equal(a, prompt_attention(q, k, v, cu(n)))
