@@ -39,6 +39,7 @@
 // largest weight.
 // Dense (fp16 / bf16) rows use m16n8k16 with hi/lo-split B operands.
 #pragma once
+#include "async_ptx.cuh"
 #include "common.cuh"
 
 namespace innerq {
@@ -107,9 +108,6 @@ struct DevArgs {
 constexpr int kWarps = 4;
 // staging ring depth (stages of kWarps tiles); 2 keeps 4 CTAs per SM
 __host__ __device__ constexpr int stages_for(int rp) { return 2; }
-// bounded mbarrier wait: each try suspends the warp for up to ~100 us (hint,
-// in ns) instead of spinning; 1 << 16 tries bound the wait to seconds
-constexpr uint32_t kWaitLimit = 1u << 16;
 
 // bytes of one staged tile (K codes, K scales [, K zeros], V codes, V scales
 // [, V zeros] [, hybrid: asymmetric V codes, their scales and zeros, the mask])
@@ -119,50 +117,6 @@ __host__ __device__ inline int stage_bytes(int bk, int bv, int ng, int kasym, in
 }
 __host__ __device__ inline int attn_dyn_smem(int bk, int bv, int ng, int kasym, int vasym, int rp, int hyb = 0) {
   return kWarps * stages_for(rp) * stage_bytes(bk, bv, ng, kasym, vasym, hyb);
-}
-
-// ------------------------------------------------------------ PTX helpers ---
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_fence_init() {
-  asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-}
-__device__ __forceinline__ void mbar_arrive_tx(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 100000;\n"
-      " selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, uint32_t limit) {
-  for (uint32_t it = 0; it < limit; ++it)
-    if (mbar_try_wait(bar, parity)) return true;
-  return false;
-}
-__device__ __forceinline__ void fence_proxy_async() {
-  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-}
-// plain (non-multicast) bulk copy global -> this CTA's shared memory
-__device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
-          smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
 }
 
 // 2^x with the MUFU approximation (ex2.approx.ftz.f32: ~2 ulp; 2^-inf = 0)

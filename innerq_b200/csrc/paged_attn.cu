@@ -1,10 +1,41 @@
-// Decode attention over the paged 4-bit cache: one query token per sequence,
-// a length per sequence.
+// Decode attention over the paged 4-bit cache: one query token per sequence, a
+// length per sequence, flash-decoding over 32-token tiles.
+//
+// Mathematics.  A 4-bit code u (0..15, offset 8) placed in the mantissa of a
+// 16-bit word IS the fp16 subnormal u 2^-24 (16 u 2^-24 four bits higher), so
+// one AND expands two codes into an fp16 tensor-core operand, exactly:
+//   q.k_t = sum_g s_tg (sum_{d in g} q_d u_td - 8 sum_{d in g} q_d)
+//   out_d = sum_tiles s_gd (sum_t p_t u_td - 8 sum_t p_t) / sum_t p_t
+// The inner sums are mma.m16n8k16 (codes as A: 16 tokens, or 16 channels, by
+// 8 query heads) with fp32 accumulators that start at the offset term; group
+// scales are applied in fp32.  The query is scaled per head by a power of two
+// into [2^14, 2^15), exact in fp16 for both dtypes; the slots whose codes sit
+// four bits higher take q / 16 and p / 16.  A probability is 2^15 p rounded to
+// fp16 (11 bits down to 2^-29 of the tile's largest), the one rounding of the
+// 4-bit path, and the sum that divides the result is taken over the rounded
+// values by an MMA against ones.  16-bit tokens (sink, window) use the same
+// MMAs on their own type; bf16 probabilities are split into two parts there.
+//
+// Work.  The tiles of all (sequence, head) units form one list that is cut
+// into equal ranges, one per resident CTA, so ragged lengths balance without
+// the host knowing them; the four warps of a CTA take every fourth tile of its
+// range, each with a ring of bulk copies of its own (one 4608-byte copy per
+// tile) and no synchronisation until a unit ends.  A unit inside one range is
+// written at once, the others leave fp32 partials that merge_kernel joins.
+#include <algorithm>
+
+#include "async_ptx.cuh"
 #include "innerq_internal.h"
 #include "paged.cuh"
 
 namespace innerq {
 namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStages = 2;
+constexpr int kCtasPerSm = 4;
+constexpr int kHeadPitch = 148;  // floats per head of the combine buffer: conflict-free
+constexpr float kPScale = 15.f;  // probabilities carry 2^15
 
 struct AttnDev {
   const uint16_t* q;
@@ -12,79 +43,627 @@ struct AttnDev {
   uint16_t* out;
   int64_t o_sb, o_sh;
   float* lse;
+  float* po;        // [2 grid][R][kD]
+  float* pm;        // [2 grid][R]
+  float* pl;
+  int32_t* starts;  // [B + 1] first tile of each sequence in the list
   float scale_log2;
-  int Hq, R;
+  int Hq, R, cap;   // cap: most tiles a sequence can have
 };
 
-// One block per (sequence, KV head): a tile of 32 tokens at a time is expanded
-// to fp32 in shared memory; online softmax over the tiles.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  return r;
+}
+// d = a b + (c0, c1, c0, c1)
 template <int DT>
-__global__ void __launch_bounds__(128) attn_simple_kernel(PagedDev c, AttnDev a) {
-  griddep_wait();
-  griddep_launch_dependents();
-  __shared__ float kt[32][kD + 1], vt[32][kD], p[8][32], qs[8][kD], corr[8], ms[8], ls[8];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int len = max(0, c.lens[b]), np = c.n_packed(len);
-  for (int r = 0; r < a.R; ++r) qs[r][tid] = to_f<DT>(a.q[b * a.q_sb + (h * a.R + r) * a.q_sh + tid]);
-  if (tid < 8) ms[tid] = -INFINITY, ls[tid] = 0.f;
-  float acc[8];
+__device__ __forceinline__ void mma_c(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+  if constexpr (DT == F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+template <int DT>
+__device__ __forceinline__ void mma_acc(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  const uint32_t b[2] = {b0, b1};
+  mma_dt<DT>(d, a, b);
+}
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int DT> __device__ __forceinline__ float lo_f(uint32_t w) { return to_f<DT>((uint16_t)(w & 0xffff)); }
+template <int DT> __device__ __forceinline__ float hi_f(uint32_t w) { return to_f<DT>((uint16_t)(w >> 16)); }
+
+// two code words (rows gid and gid + 8 of an A operand) -> the operands of two
+// k-steps: slots 0-7 hold nibbles 0, 4 (2, 6), slots 8-15 nibbles 1, 5 (3, 7)
+__device__ __forceinline__ void code_frags(uint32_t w0, uint32_t w1, uint32_t a[4], uint32_t b[4]) {
+  a[0] = w0 & 0x000f000fu;
+  a[1] = w1 & 0x000f000fu;
+  a[2] = w0 & 0x00f000f0u;
+  a[3] = w1 & 0x00f000f0u;
+  w0 >>= 8;
+  w1 >>= 8;
+  b[0] = w0 & 0x000f000fu;
+  b[1] = w1 & 0x000f000fu;
+  b[2] = w0 & 0x00f000f0u;
+  b[3] = w1 & 0x00f000f0u;
+}
+
+// What one warp has accumulated of a unit.  A lane holds the query heads
+// 2 tq + {0, 1} and, of each, the channels 16 gid + 2 mt + {0, 1}:
+// acc[mt][2 i + c] is channel 16 gid + 2 mt + i of head 2 tq + c, in units of
+// 2^-9 (codes carry 2^-24, probabilities 2^15); l carries 2^15.
+struct State {
+  float acc[8][4], m[2], l[2];
+  __device__ __forceinline__ void reset() {
 #pragma unroll
-  for (int r = 0; r < 8; ++r) acc[r] = 0.f;
-  const int64_t base = c.dense_base(b, h);
-  for (int t0 = 0; t0 < len; t0 += 32) {
-    __syncthreads();
-    const bool packed = t0 >= c.w_sink && t0 - c.w_sink < np;
-    const uint8_t* blk = packed ? c.tile(b, h, (t0 - c.w_sink) >> 5) : nullptr;
-    const int d = tid;
-    for (int r = 0; r < 32; ++r) {
-      float kv = NAN, vv = NAN;
-      if (packed && blk != nullptr) {
-        const uint32_t wk = reinterpret_cast<const uint32_t*>(blk)[(r * 4 + ((d >> 3) & 3)) * 4 + (d >> 5)];
-        const float sk = to_f<DT>(reinterpret_cast<const uint16_t*>(blk + kKScale)[(r & 7) * 16 + (r >> 3) * 4 + (d >> 5)]);
-        kv = (float)((int)((wk >> (4 * (d & 7))) & 15u) - 8) * sk;
-        const int wi = ((((d >> 2) & 3) * 8 + (d >> 4)) * 4 + ((r >> 1) & 3)) * 4 + (d & 3);
-        const uint32_t wv = reinterpret_cast<const uint32_t*>(blk + kVCodes)[wi];
-        vv = (float)((int)((wv >> (4 * ((r >> 3) + 4 * (r & 1)))) & 15u) - 8) *
-             to_f<DT>(reinterpret_cast<const uint16_t*>(blk + kVScale)[d]);
-      } else if (!packed && base >= 0) {
-        const int64_t at = base + (int64_t)c.row_of(t0 + r) * kD + d;
-        kv = to_f<DT>(c.dk[at]);
-        vv = to_f<DT>(c.dv[at]);
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+  }
+  __device__ __forceinline__ void poison() {
+    l[0] = l[1] = NAN;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = NAN;
+  }
+  // raise the running maxima to those of the tile x[row pair][..] and rescale
+  __device__ __forceinline__ void raise(const float x[2][4], float mb[2]) {
+    float t0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2]));
+    float t1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]));
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, o));
+      t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, o));
+    }
+    if (__any_sync(~0u, t0 > m[0] || t1 > m[1])) {
+      const float n0 = fmaxf(m[0], t0), n1 = fmaxf(m[1], t1);
+      const float c0 = ex2(m[0] - (n0 == -INFINITY ? 0.f : n0)), c1 = ex2(m[1] - (n1 == -INFINITY ? 0.f : n1));
+      m[0] = n0;
+      m[1] = n1;
+      l[0] *= c0;
+      l[1] *= c1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        acc[i][0] *= c0;
+        acc[i][1] *= c1;
+        acc[i][2] *= c0;
+        acc[i][3] *= c1;
       }
-      kt[r][d] = kv;
-      vt[r][d] = t0 + r < len ? vv : 0.f;
     }
-    __syncthreads();
-    for (int i = tid; i < a.R * 32; i += 128) {
-      const int r = i >> 5, t = i & 31;
-      float s = 0.f;
-      for (int x = 0; x < kD; ++x) s += qs[r][x] * kt[t][x];
-      p[r][t] = t0 + t < len ? s * a.scale_log2 : -INFINITY;
+    mb[0] = m[0] == -INFINITY ? 0.f : m[0];
+    mb[1] = m[1] == -INFINITY ? 0.f : m[1];
+  }
+};
+
+// The query of a unit as MMA operands: lane (gid, tq) holds head gid's
+// channels 32 g + 8 tq + 0..7 as B operands, and for its columns (heads
+// 2 tq + {0, 1}) the offset terms and the factor of the logits.
+struct Query {
+  uint32_t b[16];
+  float off[4][2], f[2];
+};
+
+template <int DT>
+__device__ __forceinline__ void load_query(const AttnDev& a, int b, int h, int lane, Query& o) {
+  const int gid = lane >> 2, tq = lane & 3;
+  uint4 w[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) w[g] = make_uint4(0, 0, 0, 0);
+  if (gid < a.R) {
+    const uint4* src = reinterpret_cast<const uint4*>(a.q + b * a.q_sb + (int64_t)(h * a.R + gid) * a.q_sh) + tq;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) w[g] = __ldg(src + 4 * g);
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const uint32_t* x = reinterpret_cast<const uint32_t*>(&w[g]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(lo_f<DT>(x[i])), fabsf(hi_f<DT>(x[i]))));
+  }
+  top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+  int e = 0;
+  if (top > 0.f && top < INFINITY) e = min(100, max(-100, 14 - ilogbf(top)));
+  const float up = exp2f((float)e);
+  float sum[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const uint32_t* x = reinterpret_cast<const uint32_t*>(&w[g]);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = lo_f<DT>(x[i]) * up;
+      v[2 * i + 1] = hi_f<DT>(x[i]) * up;
     }
-    __syncthreads();
-    if (tid < a.R) {
-      float m = ms[tid];
-      for (int t = 0; t < 32; ++t) m = fmaxf(m, p[tid][t]);
-      const float base_m = m == -INFINITY ? 0.f : m;
-      corr[tid] = exp2f(ms[tid] - base_m);
-      float l = ls[tid] * corr[tid];
-      for (int t = 0; t < 32; ++t) l += p[tid][t] = exp2f(p[tid][t] - base_m);
-      ms[tid] = m;
-      ls[tid] = l;
+    sum[g] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    sum[g] += __shfl_xor_sync(~0u, sum[g], 1);
+    sum[g] += __shfl_xor_sync(~0u, sum[g], 2);
+    o.b[4 * g] = half2_of(v[0], v[4]);
+    o.b[4 * g + 1] = half2_of(v[1] * 0.0625f, v[5] * 0.0625f);
+    o.b[4 * g + 2] = half2_of(v[2], v[6]);
+    o.b[4 * g + 3] = half2_of(v[3] * 0.0625f, v[7] * 0.0625f);
+  }
+  const float f = a.scale_log2 * exp2f((float)(24 - e));
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int src = (2 * tq + c) * 4;
+    o.f[c] = __shfl_sync(~0u, f, src);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) o.off[g][c] = __shfl_sync(~0u, sum[g], src) * (-8.f / 16777216.f);
+  }
+}
+
+// one packed tile in shared memory
+template <int DT>
+__device__ __forceinline__ void packed_tile(const uint8_t* blk, int lane, const Query& q, State& s) {
+  const int gid = lane >> 2;
+  float x[2][4];
+#pragma unroll
+  for (int mm = 0; mm < 2; ++mm) {
+    const uint4 w0 = reinterpret_cast<const uint4*>(blk)[64 * mm + lane];
+    const uint4 w1 = reinterpret_cast<const uint4*>(blk)[64 * mm + 32 + lane];
+    // scales of rows 8 (2 mm) + gid and 8 (2 mm + 1) + gid, four groups each
+    const uint4 sc = reinterpret_cast<const uint4*>(blk + kKScale)[2 * gid + mm];
+    const uint32_t* p0 = reinterpret_cast<const uint32_t*>(&w0);
+    const uint32_t* p1 = reinterpret_cast<const uint32_t*>(&w1);
+    const uint32_t* ps = reinterpret_cast<const uint32_t*>(&sc);
+    x[mm][0] = x[mm][1] = x[mm][2] = x[mm][3] = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uint32_t a[4], b[4];
+      code_frags(p0[g], p1[g], a, b);
+      float d[4];
+      mma_c<F16>(d, a, q.b[4 * g], q.b[4 * g + 1], q.off[g][0], q.off[g][1]);
+      mma_acc<F16>(d, b, q.b[4 * g + 2], q.b[4 * g + 3]);
+      const float s0 = g & 1 ? hi_f<DT>(ps[g >> 1]) : lo_f<DT>(ps[g >> 1]);
+      const float s1 = g & 1 ? hi_f<DT>(ps[2 + (g >> 1)]) : lo_f<DT>(ps[2 + (g >> 1)]);
+      x[mm][0] = fmaf(s0, d[0], x[mm][0]);
+      x[mm][1] = fmaf(s0, d[1], x[mm][1]);
+      x[mm][2] = fmaf(s1, d[2], x[mm][2]);
+      x[mm][3] = fmaf(s1, d[3], x[mm][3]);
     }
-    __syncthreads();
-    for (int r = 0; r < a.R; ++r) {
-      float s = acc[r] * corr[r];
-      for (int t = 0; t < 32; ++t) s += p[r][t] * vt[t][tid];
-      acc[r] = s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[mm][i] *= q.f[i & 1];
+  }
+  float mb[2];
+  s.raise(x, mb);
+  const float b0 = kPScale - mb[0], b1 = kPScale - mb[1];
+  uint32_t pb[4];
+#pragma unroll
+  for (int mm = 0; mm < 2; ++mm) {
+    pb[2 * mm] = transpose8x8(half2_of(ex2(x[mm][0] + b0), ex2(x[mm][1] + b1)));
+    pb[2 * mm + 1] = transpose8x8(half2_of(ex2(x[mm][2] + (b0 - 4.f)), ex2(x[mm][3] + (b1 - 4.f))));
+  }
+  float ps[4];
+  {
+    const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u};  // 1 and 16
+    mma_c<F16>(ps, ones, pb[0], pb[1], 0.f, 0.f);
+    mma_acc<F16>(ps, ones, pb[2], pb[3]);
+  }
+  s.l[0] += ps[0];
+  s.l[1] += ps[1];
+  const float o0 = ps[0] * (-8.f / 16777216.f), o1 = ps[1] * (-8.f / 16777216.f);
+  const uint4 v0 = reinterpret_cast<const uint4*>(blk + kVScale)[2 * gid];
+  const uint4 v1 = reinterpret_cast<const uint4*>(blk + kVScale)[2 * gid + 1];
+#pragma unroll
+  for (int pc = 0; pc < 4; ++pc) {
+    const uint4 w = reinterpret_cast<const uint4*>(blk + kVCodes)[32 * pc + lane];
+    const uint32_t* pw = reinterpret_cast<const uint32_t*>(&w);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int mt = 2 * pc + m;
+      uint32_t a[4], b[4];
+      code_frags(pw[2 * m], pw[2 * m + 1], a, b);
+      float d[4];
+      mma_c<F16>(d, a, pb[0], pb[1], o0, o1);
+      mma_acc<F16>(d, b, pb[2], pb[3]);
+      const uint32_t sc = reinterpret_cast<const uint32_t*>(mt < 4 ? &v0 : &v1)[mt & 3];
+      const float s0 = lo_f<DT>(sc), s1 = hi_f<DT>(sc);
+      s.acc[mt][0] = fmaf(s0, d[0], s.acc[mt][0]);
+      s.acc[mt][1] = fmaf(s0, d[1], s.acc[mt][1]);
+      s.acc[mt][2] = fmaf(s1, d[2], s.acc[mt][2]);
+      s.acc[mt][3] = fmaf(s1, d[3], s.acc[mt][3]);
     }
+  }
+}
+
+// one 16-bit tile (sink or window) straight from global memory: kr / vr point
+// at its first row, `valid` of its 32 rows hold tokens
+template <int DT>
+__device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* vr, int valid, const AttnDev& a, int b, int h,
+                                        int lane, State& s) {
+  const int gid = lane >> 2, tq = lane & 3;
+  uint4 qw[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) qw[g] = make_uint4(0, 0, 0, 0);
+  if (gid < a.R) {
+    const uint4* src = reinterpret_cast<const uint4*>(a.q + b * a.q_sb + (int64_t)(h * a.R + gid) * a.q_sh) + tq;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) qw[g] = __ldg(src + 4 * g);
+  }
+  float x[2][4];
+#pragma unroll
+  for (int mm = 0; mm < 2; ++mm) {
+    const uint4* r0 = reinterpret_cast<const uint4*>(kr + (16 * mm + gid) * kD) + tq;
+    const uint4* r1 = r0 + 8 * kD / 8;
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const uint4 y0 = r0[4 * g], y1 = r1[4 * g];
+      const uint32_t a0[4] = {y0.x, y1.x, y0.y, y1.y}, a1[4] = {y0.z, y1.z, y0.w, y1.w};
+      mma_acc<DT>(d, a0, qw[g].x, qw[g].y);
+      mma_acc<DT>(d, a1, qw[g].z, qw[g].w);
+    }
+    const bool in0 = 16 * mm + gid < valid, in1 = 16 * mm + 8 + gid < valid;
+    x[mm][0] = in0 ? d[0] * a.scale_log2 : -INFINITY;
+    x[mm][1] = in0 ? d[1] * a.scale_log2 : -INFINITY;
+    x[mm][2] = in1 ? d[2] * a.scale_log2 : -INFINITY;
+    x[mm][3] = in1 ? d[3] * a.scale_log2 : -INFINITY;
+  }
+  float mb[2];
+  s.raise(x, mb);
+  uint32_t pb[4], pe[4];  // bf16: the rounded probabilities and what the rounding left
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float p0 = ex2(x[i >> 1][2 * (i & 1)] - mb[0] + kPScale), p1 = ex2(x[i >> 1][2 * (i & 1) + 1] - mb[1] + kPScale);
+    const uint16_t h0 = from_f<DT>(p0), h1 = from_f<DT>(p1);
+    pb[i] = transpose8x8(pack2(h0, h1));
+    if constexpr (DT == BF16) pe[i] = transpose8x8(pack2(from_f<DT>(p0 - to_f<DT>(h0)), from_f<DT>(p1 - to_f<DT>(h1))));
+  }
+  float ps[4];
+  const uint32_t one = DT == F16 ? 0x3c003c00u : 0x3f803f80u;
+  const uint32_t ones[4] = {one, one, one, one};
+  mma_c<DT>(ps, ones, pb[0], pb[1], 0.f, 0.f);
+  mma_acc<DT>(ps, ones, pb[2], pb[3]);
+  if constexpr (DT == BF16) {
+    mma_acc<DT>(ps, ones, pe[0], pe[1]);
+    mma_acc<DT>(ps, ones, pe[2], pe[3]);
+  }
+  s.l[0] += ps[0];
+  s.l[1] += ps[1];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {  // channels 16 gid + 8 half ..: m-tiles 4 half ..
+    uint4 v[8];                           // tokens 2 tq + {0, 1, 8, 9, 16, 17, 24, 25}
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int t = 8 * (i >> 1) + 2 * tq + (i & 1);
+      v[i] = reinterpret_cast<const uint4*>(vr + t * kD)[2 * gid + half];
+      if (t >= valid) v[i] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const uint32_t*>(&v[i])[m];
+      uint32_t f[2][4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        f[k][0] = __byte_perm(w[4 * k], w[4 * k + 1], 0x5410);
+        f[k][1] = __byte_perm(w[4 * k], w[4 * k + 1], 0x7632);
+        f[k][2] = __byte_perm(w[4 * k + 2], w[4 * k + 3], 0x5410);
+        f[k][3] = __byte_perm(w[4 * k + 2], w[4 * k + 3], 0x7632);
+      }
+      float d[4];
+      mma_c<DT>(d, f[0], pb[0], pb[1], 0.f, 0.f);
+      mma_acc<DT>(d, f[1], pb[2], pb[3]);
+      if constexpr (DT == BF16) {
+        mma_acc<DT>(d, f[0], pe[0], pe[1]);
+        mma_acc<DT>(d, f[1], pe[2], pe[3]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.acc[4 * half + m][i] = fmaf(d[i], 1.f / 16777216.f, s.acc[4 * half + m][i]);
+    }
+  }
+}
+
+__device__ __forceinline__ int tiles_of(const PagedDev& c, int b, int cap) {
+  const int len = c.lens[b];
+  return len <= 0 ? 0 : min((int)(((int64_t)len + 31) >> 5), cap);
+}
+
+// inclusive scan over the block
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(~0u, v, o);
+    if (lane >= o) v += x;
+  }
+  if (lane == 31) warp_sums[w] = v;
+  __syncthreads();
+  int add = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < w) add += warp_sums[i];
+    total += warp_sums[i];
   }
   __syncthreads();
-  for (int r = 0; r < a.R; ++r) {
-    const int hq = h * a.R + r;
-    a.out[b * a.o_sb + hq * a.o_sh + tid] = from_f<DT>(len > 0 ? acc[r] / ls[r] : 0.f);
-    if (a.lse && tid == 0) a.lse[(int64_t)b * a.Hq + hq] = ms[r] + log2f(ls[r]);
+  return v + add;
+}
+
+template <int RH>
+struct alignas(128) Smem {
+  uint8_t ring[kWarps][kStages][kBlockBytes];
+  float buf[kWarps][RH][kHeadPitch];
+  float m[kWarps][8], l[kWarps][8];
+  uint64_t bars[kWarps][kStages];
+  int bad[kWarps][kStages];
+  int sums[kWarps];
+  int unit_b, unit_start, unit_tiles;
+};
+
+// tiles per CTA: equal ranges, whole rounds of the four warps
+__device__ __forceinline__ int range_of(int total, int grid) {
+  return max(kWarps, ((total + grid - 1) / grid + kWarps - 1) / kWarps * kWarps);
+}
+
+template <int DT, int RH>
+__global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnDev a) {
+  extern __shared__ __align__(128) uint8_t raw[];
+  Smem<RH>& sm = *reinterpret_cast<Smem<RH>*>(raw);
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) mbar_init(&sm.bars[w][i], 1);
+    mbar_fence_init();
   }
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // the list of tiles: where this CTA's range begins
+  int total = 0;
+  for (int b0 = 0; b0 < c.B; b0 += 128) {
+    int sum;
+    block_scan(b0 + tid < c.B ? tiles_of(c, b0 + tid, a.cap) * c.Hkv : 0, sm.sums, sum);
+    total += sum;
+  }
+  const int per = range_of(total, gridDim.x);
+  const int lo = blockIdx.x * per, hi = min(total, lo + per);
+  if (blockIdx.x == 0 || lo < total) {
+    for (int b0 = 0, at = 0; b0 < c.B; b0 += 128) {
+      int sum;
+      const int n = b0 + tid < c.B ? tiles_of(c, b0 + tid, a.cap) : 0;
+      const int end = at + block_scan(n * c.Hkv, sm.sums, sum), start = end - n * c.Hkv;
+      if (n > 0 && start <= lo && lo < end) {
+        sm.unit_b = b0 + tid;
+        sm.unit_start = start;
+        sm.unit_tiles = n;
+      }
+      if (blockIdx.x == 0 && b0 + tid < c.B) a.starts[b0 + tid] = start;
+      at += sum;
+    }
+    if (blockIdx.x == 0 && tid == 0) a.starts[c.B] = total;
+  }
+  if (lo >= total) return;
+  __syncthreads();
+  int b = sm.unit_b, nt = sm.unit_tiles;
+  int h = (lo - sm.unit_start) / nt;
+  int u0 = sm.unit_start + h * nt;
+  const int sink_tiles = c.w_sink >> 5;
+
+  // the copies of this warp's packed tiles, in order (lane 0)
+  int pb = b, ph = h, pu0 = u0, pnt = nt, pidx = lo + w, ptiles = c.n_packed(c.lens[b]) >> 5;
+  int issued = 0;
+  const uint8_t* next = nullptr;
+  bool have = false;
+  auto find_next = [&]() {
+    have = false;
+    while (pidx < hi) {
+      while (pidx >= pu0 + pnt) {
+        pu0 += pnt;
+        if (++ph == c.Hkv) {
+          ph = 0;
+          do {
+            ++pb;
+            pnt = tiles_of(c, pb, a.cap);
+          } while (pnt == 0);
+          ptiles = c.n_packed(c.lens[pb]) >> 5;
+        }
+      }
+      const int t = pidx - pu0 - sink_tiles;
+      pidx += kWarps;
+      if (t >= 0 && t < ptiles) {
+        next = c.tile(pb, ph, t);
+        have = true;
+        return;
+      }
+    }
+  };
+  auto issue = [&]() {
+    if (!have) return;
+    const int st = issued % kStages;
+    sm.bad[w][st] = next == nullptr;
+    if (next != nullptr) {
+      mbar_arrive_tx(&sm.bars[w][st], kBlockBytes);
+      bulk_g2s(sm.ring[w][st], next, kBlockBytes, &sm.bars[w][st]);
+    } else {
+      mbar_arrive(&sm.bars[w][st]);
+    }
+    ++issued;
+    find_next();
+  };
+  if (lane == 0) {
+    find_next();
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) issue();
+  }
+
+  int used = 0, idx = lo + w;
+  bool failed = false;
+  State s;
+  Query q;
+  while (true) {
+    const int len = c.lens[b], packed = c.n_packed(len) >> 5, end = min(hi, u0 + nt);
+    load_query<DT>(a, b, h, lane, q);
+    s.reset();
+#pragma unroll 1
+    for (; idx < end; idx += kWarps) {
+      const int t = idx - u0, tp = t - sink_tiles;
+      if (tp >= 0 && tp < packed) {
+        const int st = used % kStages;
+        if (!failed && !mbar_wait_bounded(&sm.bars[w][st], (used / kStages) & 1, kWaitLimit)) failed = true;
+        if (failed) {
+          s.poison();
+          continue;
+        }
+        if (sm.bad[w][st])
+          s.poison();
+        else
+          packed_tile<DT>(sm.ring[w][st], lane, q, s);
+        ++used;
+        __syncwarp();
+        if (lane == 0) issue();
+      } else {
+        const int64_t base = c.dense_base(b, h) + (int64_t)c.row_of(32 * t) * kD;
+        if (c.dense_base(b, h) < 0)
+          s.poison();
+        else
+          dense_tile<DT>(c.dk + base, c.dv + base, len - 32 * t, a, b, h, lane, s);
+      }
+    }
+    // join the four warps
+    const int gid = lane >> 2, tq = lane & 3;
+    if (gid == 0) {
+      sm.m[w][2 * tq] = s.m[0];
+      sm.m[w][2 * tq + 1] = s.m[1];
+    }
+    __syncthreads();
+    float top[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(fmaxf(sm.m[0][2 * tq + i], sm.m[1][2 * tq + i]), fmaxf(sm.m[2][2 * tq + i], sm.m[3][2 * tq + i]));
+      const float f = ex2(s.m[i] - (top[i] == -INFINITY ? 0.f : top[i]));
+      if (2 * tq + i < RH) {
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt)
+          *reinterpret_cast<float2*>(&sm.buf[w][2 * tq + i][18 * gid + 2 * mt]) =
+              make_float2(s.acc[mt][i] * f, s.acc[mt][i + 2] * f);
+        if (gid == 0) sm.l[w][2 * tq + i] = s.l[i] * f;
+      }
+    }
+    __syncthreads();
+    const bool whole = lo <= u0 && u0 + nt <= hi;
+    const int slot = 2 * blockIdx.x + (lo > u0 ? 0 : 1);
+    for (int r = 0; r < a.R; ++r) {
+      const int at = 18 * (tid >> 4) + (tid & 15);
+      const float o = (sm.buf[0][r][at] + sm.buf[1][r][at]) + (sm.buf[2][r][at] + sm.buf[3][r][at]);
+      const float l = (sm.l[0][r] + sm.l[1][r]) + (sm.l[2][r] + sm.l[3][r]);
+      const float m = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
+      if (whole) {
+        const int hq = h * a.R + r;
+        a.out[b * a.o_sb + hq * a.o_sh + tid] = from_f<DT>(o * 16777216.f / l);
+        if (a.lse && tid == 0) a.lse[(int64_t)b * a.Hq + hq] = m + log2f(l) - kPScale;
+      } else {
+        a.po[((int64_t)slot * a.R + r) * kD + tid] = o;
+        if (tid == 0) {
+          a.pm[slot * a.R + r] = m;
+          a.pl[slot * a.R + r] = l;
+        }
+      }
+    }
+    u0 += nt;
+    if (u0 >= hi) break;
+    if (++h == c.Hkv) {
+      h = 0;
+      do {
+        ++b;
+        nt = tiles_of(c, b, a.cap);
+      } while (nt == 0);
+    }
+    __syncthreads();
+  }
+  if (failed && lane == 0) {  // copies still in flight must land before the CTA's memory is given away
+    for (int i = used; i < issued; ++i)
+      mbar_wait_bounded(&sm.bars[w][i % kStages], (i / kStages) & 1, kWaitLimit / 16);
+  }
+}
+
+// Joins the partials of the units that were cut; zeros for units without tokens.
+template <int DT>
+__global__ void __launch_bounds__(128) merge_kernel(AttnDev a, int Hkv, int grid, int B) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int b = blockIdx.y, hq = blockIdx.x, tid = threadIdx.x;
+  const int s0 = a.starts[b], nt = (a.starts[b + 1] - s0) / Hkv;
+  uint16_t* out = a.out + b * a.o_sb + hq * a.o_sh + tid;
+  if (nt == 0) {
+    *out = 0;
+    if (a.lse && tid == 0) a.lse[(int64_t)b * a.Hq + hq] = -INFINITY;
+    return;
+  }
+  const int per = range_of(a.starts[B], grid);
+  const int u0 = s0 + hq / a.R * nt, r = hq % a.R;
+  const int c0 = u0 / per, c1 = (u0 + nt - 1) / per;
+  if (c0 == c1) return;
+  auto slot = [&](int i) { return (2 * i + (i * per > u0 ? 0 : 1)) * a.R + r; };
+  float m = -INFINITY;
+  for (int i = c0; i <= c1; ++i) m = fmaxf(m, a.pm[slot(i)]);
+  const float mb = m == -INFINITY ? 0.f : m;
+  float o = 0.f, l = 0.f;
+#pragma unroll 4
+  for (int i = c0; i <= c1; ++i) {
+    const int s = slot(i);
+    const float f = ex2(a.pm[s] - mb);
+    l = fmaf(f, a.pl[s], l);
+    o = fmaf(f, a.po[(int64_t)s * kD + tid], o);
+  }
+  *out = from_f<DT>(o * 16777216.f / l);
+  if (a.lse && tid == 0) a.lse[(int64_t)b * a.Hq + hq] = m + log2f(l) - kPScale;
+}
+
+int grid_size() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148 * kCtasPerSm;
+  if (!cached[dev]) {
+    int n = 0;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    cached[dev] = (n > 0 ? n : 148) * kCtasPerSm;
+  }
+  return cached[dev];
+}
+
+template <int DT, int RH>
+cudaError_t launch_attn(const PagedDev& c, const AttnDev& a, int grid, cudaStream_t s) {
+  static bool ready[64] = {false};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !ready[dev]) {
+    e = cudaFuncSetAttribute(attn_kernel<DT, RH>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem<RH>));
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready[dev] = true;
+  }
+  e = launch_pdl(attn_kernel<DT, RH>, dim3(grid), dim3(128), sizeof(Smem<RH>), s, c, a);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(merge_kernel<DT>, dim3(a.Hq, c.B), dim3(128), 0, s, a, c.Hkv, grid, c.B);
+}
+
+int64_t workspace_bytes_of(int grid, int R, int B) {
+  return (int64_t)2 * grid * R * (kD + 2) * 4 + ((int64_t)B + 1) * 4 + 256;
+}
+
+int check_heads(const PagedDev& c, int Hq) {
+  if (Hq <= 0 || Hq % c.Hkv) return set_last_error(INNERQ_ERR_ARG, "%d query heads over %d key heads", Hq, c.Hkv);
+  if (Hq / c.Hkv > 8) return set_last_error(INNERQ_ERR_UNSUPPORTED, "GQA ratio %d (1 to 8 are built)", Hq / c.Hkv);
+  return INNERQ_OK;
 }
 
 }  // namespace
@@ -94,8 +673,8 @@ using namespace innerq;
 
 extern "C" int64_t innerq_paged_attn_workspace(const innerq_paged* cache, int Hq) {
   PagedDev c;
-  if (paged_dev(cache, c)) return -1;
-  return 256;
+  if (paged_dev(cache, c) || check_heads(c, Hq)) return -1;
+  return workspace_bytes_of(grid_size(), Hq / c.Hkv, c.B);
 }
 
 extern "C" int innerq_paged_attn(const innerq_paged* cache, int Hq, const void* q, int64_t q_sb, int64_t q_sh, float scale,
@@ -103,17 +682,34 @@ extern "C" int innerq_paged_attn(const innerq_paged* cache, int Hq, const void* 
                                  float* lse, void* stream) {
   PagedDev c;
   if (int rc = paged_dev(cache, c)) return rc;
-  if (Hq <= 0 || Hq % c.Hkv) return set_last_error(INNERQ_ERR_ARG, "%d query heads over %d key heads", Hq, c.Hkv);
-  if (Hq / c.Hkv > 8) return set_last_error(INNERQ_ERR_UNSUPPORTED, "GQA ratio %d (1 to 8 are built)", Hq / c.Hkv);
+  if (int rc = check_heads(c, Hq)) return rc;
   if (c.B == 0) return INNERQ_OK;
-  if (!q || !out) return set_last_error(INNERQ_ERR_ARG, "null pointer");
-  if (((uintptr_t)q & 15) || ((uintptr_t)out & 15) || q_sb % 8 || q_sh % 8 || o_sb % 8 || o_sh % 8)
-    return set_last_error(INNERQ_ERR_ARG, "rows must be 16-byte aligned");
+  if (!q || !out || !workspace) return set_last_error(INNERQ_ERR_ARG, "null pointer");
+  if (((uintptr_t)q & 15) || ((uintptr_t)workspace & 15) || ((uintptr_t)out & 1) || q_sb % 8 || q_sh % 8)
+    return set_last_error(INNERQ_ERR_ARG, "query rows and workspace must be 16-byte aligned");
   if (c.B > 65535) return set_last_error(INNERQ_ERR_ARG, "more than 65535 sequences");
-  AttnDev a{(const uint16_t*)q, q_sb, q_sh, (uint16_t*)out, o_sb, o_sh, lse, scale * 1.4426950408889634f, Hq, Hq / c.Hkv};
-  const dim3 grid(c.Hkv, c.B);
+  const int64_t cap = (c.w_sink + c.w_recent) / 32 + 1 + (int64_t)c.max_pages * c.page_tiles;
+  if (cap * c.B * c.Hkv > 0x7fffffffll - (1 << 20))
+    return set_last_error(INNERQ_ERR_ARG, "page table of %d x %d is too large for one launch", c.B, c.max_pages);
+  const int grid = grid_size(), R = Hq / c.Hkv;
+  if (workspace_bytes < workspace_bytes_of(grid, R, c.B))
+    return set_last_error(INNERQ_ERR_ARG, "workspace %lld bytes < %lld", (long long)workspace_bytes,
+                          (long long)workspace_bytes_of(grid, R, c.B));
+  AttnDev a;
+  a.q = (const uint16_t*)q;
+  a.q_sb = q_sb; a.q_sh = q_sh;
+  a.out = (uint16_t*)out;
+  a.o_sb = o_sb; a.o_sh = o_sh;
+  a.lse = lse;
+  a.po = (float*)workspace;
+  a.pm = a.po + (int64_t)2 * grid * R * kD;
+  a.pl = a.pm + (int64_t)2 * grid * R;
+  a.starts = (int32_t*)(a.pl + (int64_t)2 * grid * R);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.Hq = Hq; a.R = R; a.cap = (int)cap;
   const cudaStream_t s = (cudaStream_t)stream;
-  const cudaError_t e = cache->dtype == INNERQ_DT_BF16 ? launch_pdl(attn_simple_kernel<BF16>, grid, dim3(128), 0, s, c, a)
-                                                       : launch_pdl(attn_simple_kernel<F16>, grid, dim3(128), 0, s, c, a);
+  const bool bf = cache->dtype == INNERQ_DT_BF16;
+  const cudaError_t e = R <= 4 ? (bf ? launch_attn<BF16, 4>(c, a, grid, s) : launch_attn<F16, 4>(c, a, grid, s))
+                               : (bf ? launch_attn<BF16, 8>(c, a, grid, s) : launch_attn<F16, 8>(c, a, grid, s));
   return e == cudaSuccess ? INNERQ_OK : set_last_error(INNERQ_ERR_CUDA, "paged_attn: %s", cudaGetErrorString(e));
 }
