@@ -32,8 +32,9 @@ namespace innerq {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 2;
-constexpr int kCtasPerSm = 4;
+constexpr int kStages = 3;
+constexpr int kCtasPerSm = 3;
+constexpr int kUnitCost = 12;    // what a unit costs beyond its tiles, in tiles
 constexpr int kHeadPitch = 148;  // floats per head of the combine buffer: conflict-free
 constexpr float kPScale = 15.f;  // probabilities carry 2^15
 
@@ -46,7 +47,7 @@ struct AttnDev {
   float* po;        // [2 grid][R][kD]
   float* pm;        // [2 grid][R]
   float* pl;
-  int32_t* starts;  // [B + 1] first tile of each sequence in the list
+  int32_t* starts;  // [B + 1] first place of each sequence in the list
   float scale_log2;
   int Hq, R, cap;   // cap: most tiles a sequence can have
 };
@@ -61,17 +62,24 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
 }
-// d = a b + (c0, c1, c0, c1)
+// d = a b + c; c stays in its registers, so an accumulator that starts at a
+// value used many times costs no moves
 template <int DT>
-__device__ __forceinline__ void mma_c(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+__device__ __forceinline__ void mma_from(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1, const float c[4]) {
   if constexpr (DT == F16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// the quad (c0, c1, c0, c1), kept as four registers of its own
+__device__ __forceinline__ void quad(float q[4], float c0, float c1) {
+  q[0] = q[2] = c0;
+  q[1] = q[3] = c1;
+  asm("" : "+f"(q[0]), "+f"(q[1]), "+f"(q[2]), "+f"(q[3]));
 }
 template <int DT>
 __device__ __forceinline__ void mma_acc(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
@@ -82,8 +90,21 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-template <int DT> __device__ __forceinline__ float lo_f(uint32_t w) { return to_f<DT>((uint16_t)(w & 0xffff)); }
-template <int DT> __device__ __forceinline__ float hi_f(uint32_t w) { return to_f<DT>((uint16_t)(w >> 16)); }
+// the two halves of a word of the dtype as fp32, one instruction each
+template <int DT> __device__ __forceinline__ float lo_f(uint32_t w) {
+  if constexpr (DT == F16) return __low2float(*reinterpret_cast<const __half2*>(&w));
+  return __uint_as_float(w << 16);
+}
+template <int DT> __device__ __forceinline__ float hi_f(uint32_t w) {
+  if constexpr (DT == F16) return __high2float(*reinterpret_cast<const __half2*>(&w));
+  return __uint_as_float(w & 0xffff0000u);
+}
+// w >> 8, opaque: kept as one shift for both operands taken from it
+__device__ __forceinline__ uint32_t shift8(uint32_t w) {
+  uint32_t r;
+  asm("shr.b32 %0, %1, 8;\n" : "=r"(r) : "r"(w));
+  return r;
+}
 
 // two code words (rows gid and gid + 8 of an A operand) -> the operands of two
 // k-steps: slots 0-7 hold nibbles 0, 4 (2, 6), slots 8-15 nibbles 1, 5 (3, 7)
@@ -92,8 +113,8 @@ __device__ __forceinline__ void code_frags(uint32_t w0, uint32_t w1, uint32_t a[
   a[1] = w1 & 0x000f000fu;
   a[2] = w0 & 0x00f000f0u;
   a[3] = w1 & 0x00f000f0u;
-  w0 >>= 8;
-  w1 >>= 8;
+  w0 = shift8(w0);
+  w1 = shift8(w1);
   b[0] = w0 & 0x000f000fu;
   b[1] = w1 & 0x000f000fu;
   b[2] = w0 & 0x00f000f0u;
@@ -121,8 +142,9 @@ struct State {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = NAN;
   }
-  // raise the running maxima to those of the tile x[row pair][..] and rescale
-  __device__ __forceinline__ void raise(const float x[2][4], float mb[2]) {
+  // raise the running maxima to those of the tile's logits x[row pair][..] f
+  // (f >= 0) and rescale
+  __device__ __forceinline__ void raise(const float x[2][4], float f0, float f1, float mb[2]) {
     float t0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2]));
     float t1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]));
 #pragma unroll
@@ -130,6 +152,8 @@ struct State {
       t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, o));
       t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, o));
     }
+    t0 *= f0;
+    t1 *= f1;
     if (__any_sync(~0u, t0 > m[0] || t1 > m[1])) {
       const float n0 = fmaxf(m[0], t0), n1 = fmaxf(m[1], t1);
       const float c0 = ex2(m[0] - (n0 == -INFINITY ? 0.f : n0)), c1 = ex2(m[1] - (n1 == -INFINITY ? 0.f : n1));
@@ -155,7 +179,7 @@ struct State {
 // 2 tq + {0, 1}) the offset terms and the factor of the logits.
 struct Query {
   uint32_t b[16];
-  float off[4][2], f[2];
+  float off[4][4], f[2];
 };
 
 template <int DT>
@@ -180,7 +204,9 @@ __device__ __forceinline__ void load_query(const AttnDev& a, int b, int h, int l
   top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
   int e = 0;
   if (top > 0.f && top < INFINITY) e = min(100, max(-100, 14 - ilogbf(top)));
-  const float up = exp2f((float)e);
+  // the sign of the softmax scale goes into q, so that f >= 0 and the largest
+  // raw product is the largest logit
+  const float up = a.scale_log2 < 0.f ? -exp2f((float)e) : exp2f((float)e);
   float sum[4];
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
@@ -199,13 +225,16 @@ __device__ __forceinline__ void load_query(const AttnDev& a, int b, int h, int l
     o.b[4 * g + 2] = half2_of(v[2], v[6]);
     o.b[4 * g + 3] = half2_of(v[3] * 0.0625f, v[7] * 0.0625f);
   }
-  const float f = a.scale_log2 * exp2f((float)(24 - e));
+  const float f = fabsf(a.scale_log2) * exp2f((float)(24 - e));
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const int src = (2 * tq + c) * 4;
     o.f[c] = __shfl_sync(~0u, f, src);
+  }
 #pragma unroll
-    for (int g = 0; g < 4; ++g) o.off[g][c] = __shfl_sync(~0u, sum[g], src) * (-8.f / 16777216.f);
+  for (int g = 0; g < 4; ++g) {
+    const float s0 = __shfl_sync(~0u, sum[g], 8 * tq), s1 = __shfl_sync(~0u, sum[g], 8 * tq + 4);
+    quad(o.off[g], s0 * (-8.f / 16777216.f), s1 * (-8.f / 16777216.f));
   }
 }
 
@@ -229,7 +258,7 @@ __device__ __forceinline__ void packed_tile(const uint8_t* blk, int lane, const 
       uint32_t a[4], b[4];
       code_frags(p0[g], p1[g], a, b);
       float d[4];
-      mma_c<F16>(d, a, q.b[4 * g], q.b[4 * g + 1], q.off[g][0], q.off[g][1]);
+      mma_from<F16>(d, a, q.b[4 * g], q.b[4 * g + 1], q.off[g]);
       mma_acc<F16>(d, b, q.b[4 * g + 2], q.b[4 * g + 3]);
       const float s0 = g & 1 ? hi_f<DT>(ps[g >> 1]) : lo_f<DT>(ps[g >> 1]);
       const float s1 = g & 1 ? hi_f<DT>(ps[2 + (g >> 1)]) : lo_f<DT>(ps[2 + (g >> 1)]);
@@ -238,27 +267,27 @@ __device__ __forceinline__ void packed_tile(const uint8_t* blk, int lane, const 
       x[mm][2] = fmaf(s1, d[2], x[mm][2]);
       x[mm][3] = fmaf(s1, d[3], x[mm][3]);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[mm][i] *= q.f[i & 1];
   }
   float mb[2];
-  s.raise(x, mb);
+  s.raise(x, q.f[0], q.f[1], mb);
   const float b0 = kPScale - mb[0], b1 = kPScale - mb[1];
   uint32_t pb[4];
 #pragma unroll
   for (int mm = 0; mm < 2; ++mm) {
-    pb[2 * mm] = transpose8x8(half2_of(ex2(x[mm][0] + b0), ex2(x[mm][1] + b1)));
-    pb[2 * mm + 1] = transpose8x8(half2_of(ex2(x[mm][2] + (b0 - 4.f)), ex2(x[mm][3] + (b1 - 4.f))));
+    pb[2 * mm] = transpose8x8(half2_of(ex2(fmaf(x[mm][0], q.f[0], b0)), ex2(fmaf(x[mm][1], q.f[1], b1))));
+    pb[2 * mm + 1] = transpose8x8(half2_of(ex2(fmaf(x[mm][2], q.f[0], b0 - 4.f)), ex2(fmaf(x[mm][3], q.f[1], b1 - 4.f))));
   }
   float ps[4];
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
   {
     const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u};  // 1 and 16
-    mma_c<F16>(ps, ones, pb[0], pb[1], 0.f, 0.f);
+    mma_from<F16>(ps, ones, pb[0], pb[1], zero);
     mma_acc<F16>(ps, ones, pb[2], pb[3]);
   }
   s.l[0] += ps[0];
   s.l[1] += ps[1];
-  const float o0 = ps[0] * (-8.f / 16777216.f), o1 = ps[1] * (-8.f / 16777216.f);
+  float off[4];
+  quad(off, ps[0] * (-8.f / 16777216.f), ps[1] * (-8.f / 16777216.f));
   const uint4 v0 = reinterpret_cast<const uint4*>(blk + kVScale)[2 * gid];
   const uint4 v1 = reinterpret_cast<const uint4*>(blk + kVScale)[2 * gid + 1];
 #pragma unroll
@@ -271,7 +300,7 @@ __device__ __forceinline__ void packed_tile(const uint8_t* blk, int lane, const 
       uint32_t a[4], b[4];
       code_frags(pw[2 * m], pw[2 * m + 1], a, b);
       float d[4];
-      mma_c<F16>(d, a, pb[0], pb[1], o0, o1);
+      mma_from<F16>(d, a, pb[0], pb[1], off);
       mma_acc<F16>(d, b, pb[2], pb[3]);
       const uint32_t sc = reinterpret_cast<const uint32_t*>(mt < 4 ? &v0 : &v1)[mt & 3];
       const float s0 = lo_f<DT>(sc), s1 = hi_f<DT>(sc);
@@ -317,7 +346,7 @@ __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* v
     x[mm][3] = in1 ? d[3] * a.scale_log2 : -INFINITY;
   }
   float mb[2];
-  s.raise(x, mb);
+  s.raise(x, 1.f, 1.f, mb);
   uint32_t pb[4], pe[4];  // bf16: the rounded probabilities and what the rounding left
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -327,9 +356,10 @@ __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* v
     if constexpr (DT == BF16) pe[i] = transpose8x8(pack2(from_f<DT>(p0 - to_f<DT>(h0)), from_f<DT>(p1 - to_f<DT>(h1))));
   }
   float ps[4];
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
   const uint32_t one = DT == F16 ? 0x3c003c00u : 0x3f803f80u;
   const uint32_t ones[4] = {one, one, one, one};
-  mma_c<DT>(ps, ones, pb[0], pb[1], 0.f, 0.f);
+  mma_from<DT>(ps, ones, pb[0], pb[1], zero);
   mma_acc<DT>(ps, ones, pb[2], pb[3]);
   if constexpr (DT == BF16) {
     mma_acc<DT>(ps, ones, pe[0], pe[1]);
@@ -360,7 +390,7 @@ __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* v
         f[k][3] = __byte_perm(w[4 * k + 2], w[4 * k + 3], 0x7632);
       }
       float d[4];
-      mma_c<DT>(d, f[0], pb[0], pb[1], 0.f, 0.f);
+      mma_from<DT>(d, f[0], pb[0], pb[1], zero);
       mma_acc<DT>(d, f[1], pb[2], pb[3]);
       if constexpr (DT == BF16) {
         mma_acc<DT>(d, f[0], pe[0], pe[1]);
@@ -376,6 +406,11 @@ __device__ __forceinline__ int tiles_of(const PagedDev& c, int b, int cap) {
   const int len = c.lens[b];
   return len <= 0 ? 0 : min((int)(((int64_t)len + 31) >> 5), cap);
 }
+
+// length of a unit of nt tiles in the list: a unit takes time beyond its tiles
+// (its query, its first loads, the join), so it is followed by kUnitCost
+// places that hold no tile
+__device__ __forceinline__ int places_of(int nt) { return nt ? nt + kUnitCost : 0; }
 
 // inclusive scan over the block
 __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
@@ -404,7 +439,7 @@ struct alignas(128) Smem {
   float buf[kWarps][RH][kHeadPitch];
   float m[kWarps][8], l[kWarps][8];
   uint64_t bars[kWarps][kStages];
-  int bad[kWarps][kStages];
+  int bad[kWarps];
   int sums[kWarps];
   int unit_b, unit_start, unit_tiles;
 };
@@ -431,7 +466,7 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
   int total = 0;
   for (int b0 = 0; b0 < c.B; b0 += 128) {
     int sum;
-    block_scan(b0 + tid < c.B ? tiles_of(c, b0 + tid, a.cap) * c.Hkv : 0, sm.sums, sum);
+    block_scan(b0 + tid < c.B ? places_of(tiles_of(c, b0 + tid, a.cap)) * c.Hkv : 0, sm.sums, sum);
     total += sum;
   }
   const int per = range_of(total, gridDim.x);
@@ -440,7 +475,7 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
     for (int b0 = 0, at = 0; b0 < c.B; b0 += 128) {
       int sum;
       const int n = b0 + tid < c.B ? tiles_of(c, b0 + tid, a.cap) : 0;
-      const int end = at + block_scan(n * c.Hkv, sm.sums, sum), start = end - n * c.Hkv;
+      const int places = places_of(n) * c.Hkv, end = at + block_scan(places, sm.sums, sum), start = end - places;
       if (n > 0 && start <= lo && lo < end) {
         sm.unit_b = b0 + tid;
         sm.unit_start = start;
@@ -454,89 +489,137 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
   if (lo >= total) return;
   __syncthreads();
   int b = sm.unit_b, nt = sm.unit_tiles;
-  int h = (lo - sm.unit_start) / nt;
-  int u0 = sm.unit_start + h * nt;
+  int h = (lo - sm.unit_start) / places_of(nt);
+  int u0 = sm.unit_start + h * places_of(nt);
   const int sink_tiles = c.w_sink >> 5;
+  int packed = c.n_packed(c.lens[b]) >> 5;
+  // the unit after (b, h); false when it begins outside the range
+  auto advance = [&]() {
+    u0 += places_of(nt);
+    if (u0 >= hi) return false;
+    if (++h == c.Hkv) {
+      h = 0;
+      do {
+        ++b;
+        nt = tiles_of(c, b, a.cap);
+      } while (nt == 0);
+      packed = c.n_packed(c.lens[b]) >> 5;
+    }
+    return true;
+  };
+  if (lo >= u0 + nt && !advance()) return;
 
-  // the copies of this warp's packed tiles, in order (lane 0)
-  int pb = b, ph = h, pu0 = u0, pnt = nt, pidx = lo + w, ptiles = c.n_packed(c.lens[b]) >> 5;
-  int issued = 0;
-  const uint8_t* next = nullptr;
-  bool have = false;
-  auto find_next = [&]() {
-    have = false;
-    while (pidx < hi) {
-      while (pidx >= pu0 + pnt) {
-        pu0 += pnt;
-        if (++ph == c.Hkv) {
-          ph = 0;
-          do {
-            ++pb;
-            pnt = tiles_of(c, pb, a.cap);
-          } while (pnt == 0);
-          ptiles = c.n_packed(c.lens[pb]) >> 5;
-        }
-      }
-      const int t = pidx - pu0 - sink_tiles;
-      pidx += kWarps;
-      if (t >= 0 && t < ptiles) {
-        next = c.tile(pb, ph, t);
-        have = true;
-        return;
-      }
-    }
-  };
+  // The unit's tiles of this CTA are the places [max(lo, u0), min(hi, u0 + nt))
+  // of the list; of those this warp takes every fourth, the packed ones through
+  // its ring.  Lane 0 keeps the copies ahead; the page number of its next copy
+  // is loaded one tile early, so that no tile waits for the table.
+  int idx = max(lo, u0) + w;
+  int left = 0, in_flight = 0;   // copies of this unit not yet issued, and under way
+  int st_put = 0, st_get = 0;    // ring slots of the next copy and the next tile
+  uint32_t parity = 0;
+  int page = 0, in_page = 0, page_id = -1;
+  const int step_page = kWarps / c.page_tiles, step_tile = kWarps % c.page_tiles;
+  const uint32_t page_bytes = (uint32_t)c.Hkv * c.page_tiles * kBlockBytes;
   auto issue = [&]() {
-    if (!have) return;
-    const int st = issued % kStages;
-    sm.bad[w][st] = next == nullptr;
-    if (next != nullptr) {
-      mbar_arrive_tx(&sm.bars[w][st], kBlockBytes);
-      bulk_g2s(sm.ring[w][st], next, kBlockBytes, &sm.bars[w][st]);
-    } else {
-      mbar_arrive(&sm.bars[w][st]);
+    if (left <= 0) return;
+    if ((unsigned)page_id < (unsigned)c.n_pages) {
+      mbar_arrive_tx(&sm.bars[w][st_put], kBlockBytes);
+      bulk_g2s(sm.ring[w][st_put],
+               c.pages + (uint64_t)page_bytes * (uint32_t)page_id + (uint32_t)((h * c.page_tiles + in_page) * kBlockBytes),
+               kBlockBytes, &sm.bars[w][st_put]);
+    } else {  // no such page: whatever the slot holds is used and the unit becomes NaN
+      sm.bad[w] = 1;
+      mbar_arrive(&sm.bars[w][st_put]);
     }
-    ++issued;
-    find_next();
+    if (++st_put == kStages) st_put = 0;
+    ++in_flight;
+    --left;
+    page += step_page;
+    in_page += step_tile;
+    if (in_page >= c.page_tiles) {
+      in_page -= c.page_tiles;
+      ++page;
+    }
+    page_id = left > 0 && page < c.max_pages ? c.table[b * c.table_stride + page] : -1;
   };
-  if (lane == 0) {
-    find_next();
+  auto begin_unit = [&]() {
+    if (lane) return;
+    const int first = max(idx, u0 + sink_tiles + ((idx - u0 - sink_tiles) & (kWarps - 1)));
+    left = (min(hi, u0 + sink_tiles + packed) - first + kWarps - 1) >> 2;
+    if (left > 0) {
+      const int t = first - u0 - sink_tiles;
+      page = t / c.page_tiles;
+      in_page = t - page * c.page_tiles;
+      page_id = page < c.max_pages ? c.table[b * c.table_stride + page] : -1;
+    }
 #pragma unroll
     for (int i = 0; i < kStages; ++i) issue();
-  }
+  };
+  sm.bad[w] = 0;
+  __syncwarp();
+  begin_unit();
 
-  int used = 0, idx = lo + w;
   bool failed = false;
   State s;
-  Query q;
   while (true) {
-    const int len = c.lens[b], packed = c.n_packed(len) >> 5, end = min(hi, u0 + nt);
-    load_query<DT>(a, b, h, lane, q);
+    const int end = min(hi, u0 + nt);
     s.reset();
+    // sink, packed tiles, window; the query operands live through the middle
+    // part only
+    auto dense = [&](int stop) {
 #pragma unroll 1
-    for (; idx < end; idx += kWarps) {
-      const int t = idx - u0, tp = t - sink_tiles;
-      if (tp >= 0 && tp < packed) {
-        const int st = used % kStages;
-        if (!failed && !mbar_wait_bounded(&sm.bars[w][st], (used / kStages) & 1, kWaitLimit)) failed = true;
-        if (failed) {
+      for (; idx < stop; idx += kWarps) {
+        const int64_t base = c.dense_base(b, h);
+        if (base < 0) {
           s.poison();
-          continue;
+        } else {
+          const int t = idx - u0;
+          const int64_t at = base + (int64_t)c.row_of(32 * t) * kD;
+          dense_tile<DT>(c.dk + at, c.dv + at, c.lens[b] - 32 * t, a, b, h, lane, s);
         }
-        if (sm.bad[w][st])
-          s.poison();
-        else
-          packed_tile<DT>(sm.ring[w][st], lane, q, s);
-        ++used;
-        __syncwarp();
-        if (lane == 0) issue();
-      } else {
-        const int64_t base = c.dense_base(b, h) + (int64_t)c.row_of(32 * t) * kD;
-        if (c.dense_base(b, h) < 0)
-          s.poison();
-        else
-          dense_tile<DT>(c.dk + base, c.dv + base, len - 32 * t, a, b, h, lane, s);
       }
+    };
+    dense(min(end, u0 + sink_tiles));
+    const int packed_end = min(end, u0 + sink_tiles + packed);
+    if (idx < packed_end) {
+      Query q;
+      load_query<DT>(a, b, h, lane, q);
+#pragma unroll 1
+      for (; idx < packed_end; idx += kWarps) {
+        if (failed || !mbar_wait_bounded(&sm.bars[w][st_get], parity, kWaitLimit)) {
+          failed = true;
+          break;
+        }
+        packed_tile<DT>(sm.ring[w][st_get], lane, q, s);
+        if (++st_get == kStages) {
+          st_get = 0;
+          parity ^= 1;
+        }
+        __syncwarp();
+        if (lane == 0) {
+          --in_flight;
+          issue();
+        }
+      }
+      if (failed) {
+        idx = packed_end + ((idx - packed_end) & (kWarps - 1));
+        s.poison();
+      }
+    }
+    dense(end);
+    // the next unit's copies go out before this one is joined
+    const bool whole = lo <= u0 && u0 + nt <= hi;
+    const int slot = 2 * blockIdx.x + (lo > u0 ? 0 : 1), ob = b, oh = h;
+    const bool bad = sm.bad[w];
+    __syncwarp();
+    if (bad) {
+      s.poison();
+      if (lane == 0) sm.bad[w] = 0;
+    }
+    const bool more = advance();
+    if (more) {
+      idx = u0 + w;
+      if (!failed) begin_unit();
     }
     // join the four warps
     const int gid = lane >> 2, tq = lane & 3;
@@ -545,11 +628,11 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
       sm.m[w][2 * tq + 1] = s.m[1];
     }
     __syncthreads();
-    float top[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      top[i] = fmaxf(fmaxf(sm.m[0][2 * tq + i], sm.m[1][2 * tq + i]), fmaxf(sm.m[2][2 * tq + i], sm.m[3][2 * tq + i]));
-      const float f = ex2(s.m[i] - (top[i] == -INFINITY ? 0.f : top[i]));
+      const float top =
+          fmaxf(fmaxf(sm.m[0][2 * tq + i], sm.m[1][2 * tq + i]), fmaxf(sm.m[2][2 * tq + i], sm.m[3][2 * tq + i]));
+      const float f = ex2(s.m[i] - (top == -INFINITY ? 0.f : top));
       if (2 * tq + i < RH) {
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt)
@@ -559,17 +642,15 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
       }
     }
     __syncthreads();
-    const bool whole = lo <= u0 && u0 + nt <= hi;
-    const int slot = 2 * blockIdx.x + (lo > u0 ? 0 : 1);
     for (int r = 0; r < a.R; ++r) {
       const int at = 18 * (tid >> 4) + (tid & 15);
       const float o = (sm.buf[0][r][at] + sm.buf[1][r][at]) + (sm.buf[2][r][at] + sm.buf[3][r][at]);
       const float l = (sm.l[0][r] + sm.l[1][r]) + (sm.l[2][r] + sm.l[3][r]);
       const float m = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
       if (whole) {
-        const int hq = h * a.R + r;
-        a.out[b * a.o_sb + hq * a.o_sh + tid] = from_f<DT>(o * 16777216.f / l);
-        if (a.lse && tid == 0) a.lse[(int64_t)b * a.Hq + hq] = m + log2f(l) - kPScale;
+        const int hq = oh * a.R + r;
+        a.out[ob * a.o_sb + hq * a.o_sh + tid] = from_f<DT>(o * 16777216.f / l);
+        if (a.lse && tid == 0) a.lse[(int64_t)ob * a.Hq + hq] = m + log2f(l) - kPScale;
       } else {
         a.po[((int64_t)slot * a.R + r) * kD + tid] = o;
         if (tid == 0) {
@@ -578,20 +659,17 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
         }
       }
     }
-    u0 += nt;
-    if (u0 >= hi) break;
-    if (++h == c.Hkv) {
-      h = 0;
-      do {
-        ++b;
-        nt = tiles_of(c, b, a.cap);
-      } while (nt == 0);
-    }
+    if (!more) break;
     __syncthreads();
   }
   if (failed && lane == 0) {  // copies still in flight must land before the CTA's memory is given away
-    for (int i = used; i < issued; ++i)
-      mbar_wait_bounded(&sm.bars[w][i % kStages], (i / kStages) & 1, kWaitLimit / 16);
+    for (; in_flight > 0; --in_flight) {
+      mbar_wait_bounded(&sm.bars[w][st_get], parity, kWaitLimit / 16);
+      if (++st_get == kStages) {
+        st_get = 0;
+        parity ^= 1;
+      }
+    }
   }
 }
 
@@ -601,15 +679,15 @@ __global__ void __launch_bounds__(128) merge_kernel(AttnDev a, int Hkv, int grid
   griddep_wait();
   griddep_launch_dependents();
   const int b = blockIdx.y, hq = blockIdx.x, tid = threadIdx.x;
-  const int s0 = a.starts[b], nt = (a.starts[b + 1] - s0) / Hkv;
+  const int s0 = a.starts[b], places = (a.starts[b + 1] - s0) / Hkv, nt = places - kUnitCost;
   uint16_t* out = a.out + b * a.o_sb + hq * a.o_sh + tid;
-  if (nt == 0) {
+  if (places == 0) {
     *out = 0;
     if (a.lse && tid == 0) a.lse[(int64_t)b * a.Hq + hq] = -INFINITY;
     return;
   }
   const int per = range_of(a.starts[B], grid);
-  const int u0 = s0 + hq / a.R * nt, r = hq % a.R;
+  const int u0 = s0 + hq / a.R * places, r = hq % a.R;
   const int c0 = u0 / per, c1 = (u0 + nt - 1) / per;
   if (c0 == c1) return;
   auto slot = [&](int i) { return (2 * i + (i * per > u0 ? 0 : 1)) * a.R + r; };
@@ -689,7 +767,7 @@ extern "C" int innerq_paged_attn(const innerq_paged* cache, int Hq, const void* 
     return set_last_error(INNERQ_ERR_ARG, "query rows and workspace must be 16-byte aligned");
   if (c.B > 65535) return set_last_error(INNERQ_ERR_ARG, "more than 65535 sequences");
   const int64_t cap = (c.w_sink + c.w_recent) / 32 + 1 + (int64_t)c.max_pages * c.page_tiles;
-  if (cap * c.B * c.Hkv > 0x7fffffffll - (1 << 20))
+  if ((cap + kUnitCost) * c.B * c.Hkv > 0x7fffffffll - (1 << 20))
     return set_last_error(INNERQ_ERR_ARG, "page table of %d x %d is too large for one launch", c.B, c.max_pages);
   const int grid = grid_size(), R = Hq / c.Hkv;
   if (workspace_bytes < workspace_bytes_of(grid, R, c.B))
