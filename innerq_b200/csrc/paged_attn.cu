@@ -36,7 +36,10 @@ constexpr int kStages = 3;
 constexpr int kCtasPerSm = 3;
 constexpr int kUnitCost = 12;    // what a unit costs beyond its tiles, in tiles
 constexpr int kHeadPitch = 148;  // floats per head of the combine buffer: conflict-free
-constexpr float kPScale = 15.f;  // probabilities carry 2^15
+constexpr float kPScale = 8.f;   // probabilities carry 2^8 relative to the running maximum,
+constexpr float kSlack = 7.f;    // which may lag behind the true one by 2^7 before it is raised
+constexpr float kOutScale = 16777216.f;  // what the codes' 2^-24 left in the accumulators
+constexpr float kNoMax = -1e30f; // running maximum before the first logit
 
 struct AttnDev {
   const uint16_t* q;
@@ -50,6 +53,8 @@ struct AttnDev {
   int32_t* starts;  // [B + 1] first place of each sequence in the list
   float scale_log2;
   int Hq, R, cap;   // cap: most tiles a sequence can have
+  uint32_t page_bytes;
+  int step_page, step_tile;  // kWarps tiles on, in whole pages and tiles
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -124,7 +129,7 @@ __device__ __forceinline__ void code_frags(uint32_t w0, uint32_t w1, uint32_t a[
 // What one warp has accumulated of a unit.  A lane holds the query heads
 // 2 tq + {0, 1} and, of each, the channels 16 gid + 2 mt + {0, 1}:
 // acc[mt][2 i + c] is channel 16 gid + 2 mt + i of head 2 tq + c, in units of
-// 2^-9 (codes carry 2^-24, probabilities 2^15); l carries 2^15.
+// 2^-16 (codes carry 2^-24, probabilities 2^8); l carries 2^8.
 struct State {
   float acc[8][4], m[2], l[2];
   __device__ __forceinline__ void reset() {
@@ -132,7 +137,7 @@ struct State {
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-    m[0] = m[1] = -INFINITY;
+    m[0] = m[1] = kNoMax;
     l[0] = l[1] = 0.f;
   }
   __device__ __forceinline__ void poison() {
@@ -142,11 +147,10 @@ struct State {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = NAN;
   }
-  // raise the running maxima to those of the tile's logits x[row pair][..] f
-  // (f >= 0) and rescale
-  __device__ __forceinline__ void raise(const float x[2][4], float f0, float f1, float mb[2]) {
-    float t0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2]));
-    float t1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]));
+  // the largest logits of a tile x[row pair][..] f (f >= 0) per column
+  __device__ __forceinline__ void largest(const float x[2][4], float f0, float f1, float& t0, float& t1) const {
+    t0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2]));
+    t1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]));
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
       t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, o));
@@ -154,23 +158,24 @@ struct State {
     }
     t0 *= f0;
     t1 *= f1;
-    if (__any_sync(~0u, t0 > m[0] || t1 > m[1])) {
-      const float n0 = fmaxf(m[0], t0), n1 = fmaxf(m[1], t1);
-      const float c0 = ex2(m[0] - (n0 == -INFINITY ? 0.f : n0)), c1 = ex2(m[1] - (n1 == -INFINITY ? 0.f : n1));
-      m[0] = n0;
-      m[1] = n1;
-      l[0] *= c0;
-      l[1] *= c1;
+  }
+  __device__ __forceinline__ bool fits(float t0, float t1) const {
+    return !__any_sync(~0u, t0 > m[0] + kSlack || t1 > m[1] + kSlack);
+  }
+  // raise the running maxima and rescale
+  __device__ __forceinline__ void raise(float t0, float t1) {
+    const float n0 = fmaxf(m[0], t0), n1 = fmaxf(m[1], t1), c0 = ex2(m[0] - n0), c1 = ex2(m[1] - n1);
+    m[0] = n0;
+    m[1] = n1;
+    l[0] *= c0;
+    l[1] *= c1;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        acc[i][0] *= c0;
-        acc[i][1] *= c1;
-        acc[i][2] *= c0;
-        acc[i][3] *= c1;
-      }
+    for (int i = 0; i < 8; ++i) {
+      acc[i][0] *= c0;
+      acc[i][1] *= c1;
+      acc[i][2] *= c0;
+      acc[i][3] *= c1;
     }
-    mb[0] = m[0] == -INFINITY ? 0.f : m[0];
-    mb[1] = m[1] == -INFINITY ? 0.f : m[1];
   }
 };
 
@@ -179,7 +184,8 @@ struct State {
 // 2 tq + {0, 1}) the offset terms and the factor of the logits.
 struct Query {
   uint32_t b[16];
-  float off[4][4], f[2];
+  float off[4][4];
+  float f[2];
 };
 
 template <int DT>
@@ -226,11 +232,8 @@ __device__ __forceinline__ void load_query(const AttnDev& a, int b, int h, int l
     o.b[4 * g + 3] = half2_of(v[3] * 0.0625f, v[7] * 0.0625f);
   }
   const float f = fabsf(a.scale_log2) * exp2f((float)(24 - e));
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int src = (2 * tq + c) * 4;
-    o.f[c] = __shfl_sync(~0u, f, src);
-  }
+  o.f[0] = __shfl_sync(~0u, f, 8 * tq);
+  o.f[1] = __shfl_sync(~0u, f, 8 * tq + 4);
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const float s0 = __shfl_sync(~0u, sum[g], 8 * tq), s1 = __shfl_sync(~0u, sum[g], 8 * tq + 4);
@@ -238,11 +241,11 @@ __device__ __forceinline__ void load_query(const AttnDev& a, int b, int h, int l
   }
 }
 
-// one packed tile in shared memory
+// logits of a packed tile in shared memory, before the factor q.f
 template <int DT>
-__device__ __forceinline__ void packed_tile(const uint8_t* blk, int lane, const Query& q, State& s) {
+__device__ __forceinline__ void packed_logits(const uint8_t* blk, int lane, const Query& q, float x[2][4]) {
   const int gid = lane >> 2;
-  float x[2][4];
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int mm = 0; mm < 2; ++mm) {
     const uint4 w0 = reinterpret_cast<const uint4*>(blk)[64 * mm + lane];
@@ -268,9 +271,14 @@ __device__ __forceinline__ void packed_tile(const uint8_t* blk, int lane, const 
       x[mm][3] = fmaf(s1, d[3], x[mm][3]);
     }
   }
-  float mb[2];
-  s.raise(x, q.f[0], q.f[1], mb);
-  const float b0 = kPScale - mb[0], b1 = kPScale - mb[1];
+}
+
+// its probabilities and values
+template <int DT>
+__device__ __forceinline__ void packed_values(const uint8_t* blk, int lane, const Query& q, const float x[2][4], State& s) {
+  const int gid = lane >> 2;
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  const float b0 = kPScale - s.m[0], b1 = kPScale - s.m[1];
   uint32_t pb[4];
 #pragma unroll
   for (int mm = 0; mm < 2; ++mm) {
@@ -278,7 +286,6 @@ __device__ __forceinline__ void packed_tile(const uint8_t* blk, int lane, const 
     pb[2 * mm + 1] = transpose8x8(half2_of(ex2(fmaf(x[mm][2], q.f[0], b0 - 4.f)), ex2(fmaf(x[mm][3], q.f[1], b1 - 4.f))));
   }
   float ps[4];
-  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
   {
     const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u};  // 1 and 16
     mma_from<F16>(ps, ones, pb[0], pb[1], zero);
@@ -345,12 +352,13 @@ __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* v
     x[mm][2] = in1 ? d[2] * a.scale_log2 : -INFINITY;
     x[mm][3] = in1 ? d[3] * a.scale_log2 : -INFINITY;
   }
-  float mb[2];
-  s.raise(x, 1.f, 1.f, mb);
+  float t0, t1;
+  s.largest(x, 1.f, 1.f, t0, t1);
+  if (!s.fits(t0, t1)) s.raise(t0, t1);
   uint32_t pb[4], pe[4];  // bf16: the rounded probabilities and what the rounding left
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float p0 = ex2(x[i >> 1][2 * (i & 1)] - mb[0] + kPScale), p1 = ex2(x[i >> 1][2 * (i & 1) + 1] - mb[1] + kPScale);
+    const float p0 = ex2(x[i >> 1][2 * (i & 1)] - s.m[0] + kPScale), p1 = ex2(x[i >> 1][2 * (i & 1) + 1] - s.m[1] + kPScale);
     const uint16_t h0 = from_f<DT>(p0), h1 = from_f<DT>(p1);
     pb[i] = transpose8x8(pack2(h0, h1));
     if constexpr (DT == BF16) pe[i] = transpose8x8(pack2(from_f<DT>(p0 - to_f<DT>(h0)), from_f<DT>(p1 - to_f<DT>(h1))));
@@ -368,19 +376,19 @@ __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* v
   s.l[0] += ps[0];
   s.l[1] += ps[1];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {  // channels 16 gid + 8 half ..: m-tiles 4 half ..
-    uint4 v[8];                           // tokens 2 tq + {0, 1, 8, 9, 16, 17, 24, 25}
+  for (int part = 0; part < 4; ++part) {  // channels 16 gid + 4 part ..: m-tiles 2 part, 2 part + 1
+    uint2 v[8];                           // tokens 2 tq + {0, 1, 8, 9, 16, 17, 24, 25}
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int t = 8 * (i >> 1) + 2 * tq + (i & 1);
-      v[i] = reinterpret_cast<const uint4*>(vr + t * kD)[2 * gid + half];
-      if (t >= valid) v[i] = make_uint4(0, 0, 0, 0);
+      v[i] = reinterpret_cast<const uint2*>(vr + t * kD)[4 * gid + part];
+      if (t >= valid) v[i] = make_uint2(0, 0);
     }
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
+    for (int m = 0; m < 2; ++m) {
       uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const uint32_t*>(&v[i])[m];
+      for (int i = 0; i < 8; ++i) w[i] = m ? v[i].y : v[i].x;
       uint32_t f[2][4];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -397,7 +405,7 @@ __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* v
         mma_acc<DT>(d, f[1], pe[2], pe[3]);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s.acc[4 * half + m][i] = fmaf(d[i], 1.f / 16777216.f, s.acc[4 * half + m][i]);
+      for (int i = 0; i < 4; ++i) s.acc[2 * part + m][i] = fmaf(d[i], 1.f / 16777216.f, s.acc[2 * part + m][i]);
     }
   }
 }
@@ -436,9 +444,10 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
 template <int RH>
 struct alignas(128) Smem {
   uint8_t ring[kWarps][kStages][kBlockBytes];
-  float buf[kWarps][RH][kHeadPitch];
+  float buf[2][RH][kHeadPitch];
   float m[kWarps][8], l[kWarps][8];
   uint64_t bars[kWarps][kStages];
+  int4 put[kWarps];
   int bad[kWarps];
   int sums[kWarps];
   int unit_b, unit_start, unit_tiles;
@@ -514,18 +523,22 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
   // its ring.  Lane 0 keeps the copies ahead; the page number of its next copy
   // is loaded one tile early, so that no tile waits for the table.
   int idx = max(lo, u0) + w;
-  int left = 0, in_flight = 0;   // copies of this unit not yet issued, and under way
+  int in_flight = 0;             // copies under way (lane 0)
   int st_put = 0, st_get = 0;    // ring slots of the next copy and the next tile
   uint32_t parity = 0;
-  int page = 0, in_page = 0, page_id = -1;
-  const int step_page = kWarps / c.page_tiles, step_tile = kWarps % c.page_tiles;
-  const uint32_t page_bytes = (uint32_t)c.Hkv * c.page_tiles * kBlockBytes;
+  // in shared memory: copies of this unit not yet issued, the next one's page,
+  // tile in the page and page number
+  int4& put = sm.put[w];
+  auto page_number = [&](int left, int page) {
+    return left > 0 && page < c.max_pages ? c.table[b * c.table_stride + page] : -1;
+  };
   auto issue = [&]() {
-    if (left <= 0) return;
-    if ((unsigned)page_id < (unsigned)c.n_pages) {
+    int4 p = put;
+    if (p.x <= 0) return;
+    if ((unsigned)p.w < (unsigned)c.n_pages) {
       mbar_arrive_tx(&sm.bars[w][st_put], kBlockBytes);
       bulk_g2s(sm.ring[w][st_put],
-               c.pages + (uint64_t)page_bytes * (uint32_t)page_id + (uint32_t)((h * c.page_tiles + in_page) * kBlockBytes),
+               c.pages + (uint64_t)a.page_bytes * (uint32_t)p.w + (uint32_t)((h * c.page_tiles + p.z) * kBlockBytes),
                kBlockBytes, &sm.bars[w][st_put]);
     } else {  // no such page: whatever the slot holds is used and the unit becomes NaN
       sm.bad[w] = 1;
@@ -533,25 +546,22 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
     }
     if (++st_put == kStages) st_put = 0;
     ++in_flight;
-    --left;
-    page += step_page;
-    in_page += step_tile;
-    if (in_page >= c.page_tiles) {
-      in_page -= c.page_tiles;
-      ++page;
+    --p.x;
+    p.y += a.step_page;
+    p.z += a.step_tile;
+    if (p.z >= c.page_tiles) {
+      p.z -= c.page_tiles;
+      ++p.y;
     }
-    page_id = left > 0 && page < c.max_pages ? c.table[b * c.table_stride + page] : -1;
+    p.w = page_number(p.x, p.y);
+    put = p;
   };
   auto begin_unit = [&]() {
     if (lane) return;
     const int first = max(idx, u0 + sink_tiles + ((idx - u0 - sink_tiles) & (kWarps - 1)));
-    left = (min(hi, u0 + sink_tiles + packed) - first + kWarps - 1) >> 2;
-    if (left > 0) {
-      const int t = first - u0 - sink_tiles;
-      page = t / c.page_tiles;
-      in_page = t - page * c.page_tiles;
-      page_id = page < c.max_pages ? c.table[b * c.table_stride + page] : -1;
-    }
+    const int left = (min(hi, u0 + sink_tiles + packed) - first + kWarps - 1) >> 2;
+    const int t = max(0, first - u0 - sink_tiles), page = t / c.page_tiles;
+    put = make_int4(left, page, t - page * c.page_tiles, page_number(left, page));
 #pragma unroll
     for (int i = 0; i < kStages; ++i) issue();
   };
@@ -564,33 +574,36 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
   while (true) {
     const int end = min(hi, u0 + nt);
     s.reset();
-    // sink, packed tiles, window; the query operands live through the middle
-    // part only
-    auto dense = [&](int stop) {
+    // the 16-bit tiles (sink and window) first, while the copies are under way
+    const int packed_lo = u0 + sink_tiles, packed_end = min(end, packed_lo + packed);
 #pragma unroll 1
-      for (; idx < stop; idx += kWarps) {
-        const int64_t base = c.dense_base(b, h);
-        if (base < 0) {
-          s.poison();
-        } else {
-          const int t = idx - u0;
-          const int64_t at = base + (int64_t)c.row_of(32 * t) * kD;
-          dense_tile<DT>(c.dk + at, c.dv + at, c.lens[b] - 32 * t, a, b, h, lane, s);
-        }
+    for (int p = idx;; p += kWarps) {
+      if (p >= packed_lo && p < packed_end) p = packed_end + ((p - packed_end) & (kWarps - 1));
+      if (p >= end) break;
+      const int64_t base = c.dense_base(b, h);
+      if (base < 0) {
+        s.poison();
+        continue;
       }
-    };
-    dense(min(end, u0 + sink_tiles));
-    const int packed_end = min(end, u0 + sink_tiles + packed);
+      const int t = 32 * (p - u0);
+      const int64_t at = base + (int64_t)c.row_of(t) * kD;
+      dense_tile<DT>(c.dk + at, c.dv + at, c.lens[b] - t, a, b, h, lane, s);
+    }
+    if (idx < packed_lo) idx = packed_lo + ((idx - packed_lo) & (kWarps - 1));
     if (idx < packed_end) {
       Query q;
       load_query<DT>(a, b, h, lane, q);
+      failed = failed || !mbar_wait_bounded(&sm.bars[w][st_get], parity, kWaitLimit);
 #pragma unroll 1
-      for (; idx < packed_end; idx += kWarps) {
-        if (failed || !mbar_wait_bounded(&sm.bars[w][st_get], parity, kWaitLimit)) {
-          failed = true;
-          break;
+      while (!failed) {
+        float x[2][4], t0, t1;
+        packed_logits<DT>(sm.ring[w][st_get], lane, q, x);
+        s.largest(x, q.f[0], q.f[1], t0, t1);
+        if (!s.fits(t0, t1)) {  // seldom after the first tile, which is then read again
+          s.raise(t0, t1);
+          continue;
         }
-        packed_tile<DT>(sm.ring[w][st_get], lane, q, s);
+        packed_values<DT>(sm.ring[w][st_get], lane, q, x, s);
         if (++st_get == kStages) {
           st_get = 0;
           parity ^= 1;
@@ -600,13 +613,12 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
           --in_flight;
           issue();
         }
+        idx += kWarps;
+        if (idx >= packed_end) break;
+        failed = !mbar_wait_bounded(&sm.bars[w][st_get], parity, kWaitLimit);
       }
-      if (failed) {
-        idx = packed_end + ((idx - packed_end) & (kWarps - 1));
-        s.poison();
-      }
+      if (failed) s.poison();
     }
-    dense(end);
     // the next unit's copies go out before this one is joined
     const bool whole = lo <= u0 && u0 + nt <= hi;
     const int slot = 2 * blockIdx.x + (lo > u0 ? 0 : 1), ob = b, oh = h;
@@ -632,24 +644,40 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
     for (int i = 0; i < 2; ++i) {
       const float top =
           fmaxf(fmaxf(sm.m[0][2 * tq + i], sm.m[1][2 * tq + i]), fmaxf(sm.m[2][2 * tq + i], sm.m[3][2 * tq + i]));
-      const float f = ex2(s.m[i] - (top == -INFINITY ? 0.f : top));
-      if (2 * tq + i < RH) {
+      const float f = ex2(s.m[i] - top);
 #pragma unroll
-        for (int mt = 0; mt < 8; ++mt)
-          *reinterpret_cast<float2*>(&sm.buf[w][2 * tq + i][18 * gid + 2 * mt]) =
-              make_float2(s.acc[mt][i] * f, s.acc[mt][i + 2] * f);
-        if (gid == 0) sm.l[w][2 * tq + i] = s.l[i] * f;
+      for (int mt = 0; mt < 8; ++mt) {
+        s.acc[mt][i] *= f;
+        s.acc[mt][i + 2] *= f;
       }
+      if (gid == 0) sm.l[w][2 * tq + i] = s.l[i] * f;
     }
-    __syncthreads();
+    // warps 2 and 3 hand over to 0 and 1, which leave two sums
+#pragma unroll
+    for (int turn = 0; turn < 2; ++turn) {
+      if ((w < 2) == (turn == 1)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (2 * tq + i < RH) {
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+              float2* at = reinterpret_cast<float2*>(&sm.buf[w & 1][2 * tq + i][18 * gid + 2 * mt]);
+              const float2 add = turn ? *at : make_float2(0.f, 0.f);
+              *at = make_float2(s.acc[mt][i] + add.x, s.acc[mt][i + 2] + add.y);
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
     for (int r = 0; r < a.R; ++r) {
       const int at = 18 * (tid >> 4) + (tid & 15);
-      const float o = (sm.buf[0][r][at] + sm.buf[1][r][at]) + (sm.buf[2][r][at] + sm.buf[3][r][at]);
+      const float o = sm.buf[0][r][at] + sm.buf[1][r][at];
       const float l = (sm.l[0][r] + sm.l[1][r]) + (sm.l[2][r] + sm.l[3][r]);
       const float m = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
       if (whole) {
         const int hq = oh * a.R + r;
-        a.out[ob * a.o_sb + hq * a.o_sh + tid] = from_f<DT>(o * 16777216.f / l);
+        a.out[ob * a.o_sb + hq * a.o_sh + tid] = from_f<DT>(o * kOutScale / l);
         if (a.lse && tid == 0) a.lse[(int64_t)ob * a.Hq + hq] = m + log2f(l) - kPScale;
       } else {
         a.po[((int64_t)slot * a.R + r) * kD + tid] = o;
@@ -673,37 +701,74 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
   }
 }
 
-// Joins the partials of the units that were cut; zeros for units without tokens.
+// Joins the partials of the units that were cut; zeros for units without
+// tokens.  One block per (head, sequence): its warps take the partials in
+// turn, four at a time so that their loads overlap, then join.
+constexpr int kMergeWarps = 8;
 template <int DT>
-__global__ void __launch_bounds__(128) merge_kernel(AttnDev a, int Hkv, int grid, int B) {
+__global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(AttnDev a, int Hkv, int grid, int B) {
   griddep_wait();
   griddep_launch_dependents();
-  const int b = blockIdx.y, hq = blockIdx.x, tid = threadIdx.x;
+  __shared__ float4 so[kMergeWarps][32];
+  __shared__ float sm[kMergeWarps], sl[kMergeWarps];
+  const int b = blockIdx.y, hq = blockIdx.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int s0 = a.starts[b], places = (a.starts[b + 1] - s0) / Hkv, nt = places - kUnitCost;
-  uint16_t* out = a.out + b * a.o_sb + hq * a.o_sh + tid;
+  uint16_t* out = a.out + b * a.o_sb + hq * a.o_sh;
   if (places == 0) {
-    *out = 0;
-    if (a.lse && tid == 0) a.lse[(int64_t)b * a.Hq + hq] = -INFINITY;
+    if (threadIdx.x < kD) out[threadIdx.x] = 0;
+    if (a.lse && threadIdx.x == 0) a.lse[(int64_t)b * a.Hq + hq] = -INFINITY;
     return;
   }
   const int per = range_of(a.starts[B], grid);
   const int u0 = s0 + hq / a.R * places, r = hq % a.R;
   const int c0 = u0 / per, c1 = (u0 + nt - 1) / per;
   if (c0 == c1) return;
-  auto slot = [&](int i) { return (2 * i + (i * per > u0 ? 0 : 1)) * a.R + r; };
-  float m = -INFINITY;
-  for (int i = c0; i <= c1; ++i) m = fmaxf(m, a.pm[slot(i)]);
-  const float mb = m == -INFINITY ? 0.f : m;
-  float o = 0.f, l = 0.f;
-#pragma unroll 4
-  for (int i = c0; i <= c1; ++i) {
-    const int s = slot(i);
-    const float f = ex2(a.pm[s] - mb);
-    l = fmaf(f, a.pl[s], l);
-    o = fmaf(f, a.po[(int64_t)s * kD + tid], o);
+  float m = kNoMax, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto join = [&](float pm, float pl, float4 po) {
+    const float n = fmaxf(m, pm), f = ex2(m - n), g = ex2(pm - n);
+    m = n;
+    l = l * f + pl * g;
+    o.x = o.x * f + po.x * g;
+    o.y = o.y * f + po.y * g;
+    o.z = o.z * f + po.z * g;
+    o.w = o.w * f + po.w * g;
+  };
+  for (int i0 = c0 + w; i0 <= c1; i0 += 4 * kMergeWarps) {
+    float pm[4], pl[4];
+    float4 po[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * kMergeWarps;
+      pm[j] = kNoMax;
+      pl[j] = 0.f;
+      po[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i <= c1) {
+        const int64_t s = (int64_t)(2 * i + (i * per > u0 ? 0 : 1)) * a.R + r;
+        pm[j] = a.pm[s];
+        pl[j] = a.pl[s];
+        po[j] = reinterpret_cast<const float4*>(a.po + s * kD)[lane];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) join(pm[j], pl[j], po[j]);
   }
-  *out = from_f<DT>(o * 16777216.f / l);
-  if (a.lse && tid == 0) a.lse[(int64_t)b * a.Hq + hq] = m + log2f(l) - kPScale;
+  so[w][lane] = o;
+  if (lane == 0) {
+    sm[w] = m;
+    sl[w] = l;
+  }
+  __syncthreads();
+  if (w) return;
+#pragma unroll
+  for (int i = 1; i < kMergeWarps; ++i) join(sm[i], sl[i], so[i][lane]);
+  const float inv = kOutScale / l;
+  uint16_t* at = out + 4 * lane;
+  at[0] = from_f<DT>(o.x * inv);
+  at[1] = from_f<DT>(o.y * inv);
+  at[2] = from_f<DT>(o.z * inv);
+  at[3] = from_f<DT>(o.w * inv);
+  if (a.lse && lane == 0) a.lse[(int64_t)b * a.Hq + hq] = m + log2f(l) - kPScale;
 }
 
 int grid_size() {
@@ -731,7 +796,7 @@ cudaError_t launch_attn(const PagedDev& c, const AttnDev& a, int grid, cudaStrea
   }
   e = launch_pdl(attn_kernel<DT, RH>, dim3(grid), dim3(128), sizeof(Smem<RH>), s, c, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(merge_kernel<DT>, dim3(a.Hq, c.B), dim3(128), 0, s, a, c.Hkv, grid, c.B);
+  return launch_pdl(merge_kernel<DT>, dim3(a.Hq, c.B), dim3(32 * kMergeWarps), 0, s, a, c.Hkv, grid, c.B);
 }
 
 int64_t workspace_bytes_of(int grid, int R, int B) {
@@ -767,6 +832,7 @@ extern "C" int innerq_paged_attn(const innerq_paged* cache, int Hq, const void* 
     return set_last_error(INNERQ_ERR_ARG, "query rows and workspace must be 16-byte aligned");
   if (c.B > 65535) return set_last_error(INNERQ_ERR_ARG, "more than 65535 sequences");
   const int64_t cap = (c.w_sink + c.w_recent) / 32 + 1 + (int64_t)c.max_pages * c.page_tiles;
+  if ((int64_t)c.Hkv * c.page_tiles * kBlockBytes > 0xffffffffll) return set_last_error(INNERQ_ERR_ARG, "pages of 4 GiB or more");
   if ((cap + kUnitCost) * c.B * c.Hkv > 0x7fffffffll - (1 << 20))
     return set_last_error(INNERQ_ERR_ARG, "page table of %d x %d is too large for one launch", c.B, c.max_pages);
   const int grid = grid_size(), R = Hq / c.Hkv;
@@ -785,6 +851,9 @@ extern "C" int innerq_paged_attn(const innerq_paged* cache, int Hq, const void* 
   a.starts = (int32_t*)(a.pl + (int64_t)2 * grid * R);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.Hq = Hq; a.R = R; a.cap = (int)cap;
+  a.page_bytes = (uint32_t)c.Hkv * c.page_tiles * kBlockBytes;
+  a.step_page = kWarps / c.page_tiles;
+  a.step_tile = kWarps % c.page_tiles;
   const cudaStream_t s = (cudaStream_t)stream;
   const bool bf = cache->dtype == INNERQ_DT_BF16;
   const cudaError_t e = R <= 4 ? (bf ? launch_attn<BF16, 4>(c, a, grid, s) : launch_attn<F16, 4>(c, a, grid, s))
