@@ -1,10 +1,47 @@
-// Attention of whole prompts packed one behind the other.
+// Attention of whole prompts packed one behind the other, on the tensor cores
+// (tcgen05).
+//
+// Mathematics.  Flash attention: over key tiles of 128, S = Q K^T, running row
+// maximum m and sum l, P = 2^(S scale log2 e - m), O += P V.  m may lag behind
+// the true maximum by 2^8 before O is rescaled, so rescaling is rare; P carries
+// 2^7 so that fp16 keeps 11 bits down to 2^-21 of the largest.  P is rounded to
+// the inputs' type for the second product (its sum l is not); everything else
+// is fp32.
+//
+// A CTA owns 256 queries of one head as two tiles of 128, so that one tile's
+// softmax runs while the tensor core works for the other:
+//   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per query row (no
+//                   shuffles); rescaling and the epilogue too
+//   warp 8          issues every MMA: S_i = Q_i K^T from shared memory, then
+//                   O_i += P_i V with P_i read from tensor memory, where it
+//                   replaces S_i
+//   warp 9          TMA loads: Q once, K and V tiles through a ring
+//   warps 10, 11    look over the V tiles that some row must not see whole: a
+//                   masked probability is 0, but 0 * NaN is NaN, so values
+//                   that are not finite are set to 0 there and added again, in
+//                   the epilogue, to the rows that do see them
+// Tensor memory: S0 | S1 | O0 | O1, 128 columns each.  In-order execution of
+// the MMAs makes "S_i(j + 1) is complete" mean that O_i is at rest too.
+#include <algorithm>
+
 #include "../../include/innerq_b200.h"
 #include "common.cuh"
 #include "innerq_internal.h"
+#include "tcgen05_ptx.cuh"
 
 namespace innerq {
 namespace {
+
+constexpr int kRows = 128;               // queries of a tile, keys of a tile
+constexpr int kPair = 2 * kRows;         // queries of a CTA
+constexpr int kHalfTile = kRows * 128;   // bytes of 64 channels of a tile
+constexpr int kTileBytes = 2 * kHalfTile;
+constexpr int kRing = 5;                 // K and V tiles in flight
+constexpr int kThreads = 384;
+constexpr float kShift = 7.f;            // P carries 2^7
+constexpr float kSlack = 8.f;            // lag of the running maximum
+constexpr float kNoMax = -1e30f;
+constexpr uint32_t kWait = 1u << 14;
 
 struct PromptDev {
   const uint16_t* q;
@@ -15,52 +52,416 @@ struct PromptDev {
   const int32_t* cu_k;
   uint16_t* out;
   float* lse;
-  float scale_log2;
-  int B, Hq, Hkv, Tq, Tk, causal;
+  float scale_log2;  // > 0; `negate` holds the sign
+  int negate;
+  int B, Hq, Hkv, Tq, Tk, causal, slots;
 };
 
-// One warp per (query, head), four channels per lane.
+struct alignas(1024) Smem {
+  uint8_t q[2][kTileBytes];
+  uint8_t ring[kRing][kTileBytes];
+  uint64_t q_full, full[kRing], checked[kRing], empty[kRing], s_full[2], p_ready[2], o_full[2];
+  uint32_t tmem;
+  int seq, dirty;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// two probabilities as one word of the type
+template <int DT> __device__ __forceinline__ uint32_t pack_p(float a, float b) {
+  uint32_t r;
+  if constexpr (DT == F16)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(b), "f"(a));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+
+template <int DT> __device__ __forceinline__ bool not_finite(uint32_t h) {
+  constexpr uint32_t e = DT == F16 ? 0x7c00u : 0x7f80u;
+  return (h & e) == e;
+}
+
+// The work of a CTA: queries q0 .. of sequence b, and how many key tiles each
+// of its two query tiles needs.
+struct Work {
+  int q_base, nq, k_base, nk, q0, off, n[2];
+  // keys that query row `i` of the sequence may see
+  __device__ __forceinline__ int limit(int i, int causal) const { return causal ? min(nk, i + off + 1) : nk; }
+};
+
 template <int DT>
-__global__ void __launch_bounds__(128) prompt_simple_kernel(PromptDev a) {
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                  const __grid_constant__ CUtensorMap mv, PromptDev a) {
+  extern __shared__ __align__(1024) uint8_t raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31, h = blockIdx.y, t = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (t >= a.Tq) return;
-  int b = -1;
-  for (int i = 0; i < a.B; ++i)
-    if (a.cu_q[i] <= t && t < a.cu_q[i + 1]) b = i;
-  if (b < 0) return;
-  const int k0 = max(0, a.cu_k[b]), nk = min(a.cu_k[b + 1], a.Tk) - k0;
-  const int seen = a.causal ? min(nk, t - a.cu_q[b] + 1 + nk - (a.cu_q[b + 1] - a.cu_q[b])) : nk;
-  float qf[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) qf[i] = to_f<DT>(a.q[t * a.q_st + h * a.q_sh + 4 * lane + i]);
-  const int hk = h / (a.Hq / a.Hkv);
-  for (int j = 0; j < seen; ++j) {
-    const uint2 kw = *reinterpret_cast<const uint2*>(a.k + (k0 + j) * a.k_st + hk * a.k_sh + 4 * lane);
-    const uint2 vw = *reinterpret_cast<const uint2*>(a.v + (k0 + j) * a.v_st + hk * a.v_sh + 4 * lane);
-    float s = qf[0] * to_f<DT>(kw.x & 0xffff) + qf[1] * to_f<DT>(kw.x >> 16) + qf[2] * to_f<DT>(kw.y & 0xffff) +
-              qf[3] * to_f<DT>(kw.y >> 16);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    s *= a.scale_log2;
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - base), p = exp2f(s - base);
-    l = l * corr + p;
-    acc[0] = acc[0] * corr + p * to_f<DT>(vw.x & 0xffff);
-    acc[1] = acc[1] * corr + p * to_f<DT>(vw.x >> 16);
-    acc[2] = acc[2] * corr + p * to_f<DT>(vw.y & 0xffff);
-    acc[3] = acc[3] * corr + p * to_f<DT>(vw.y >> 16);
-    m = mn;
+
+  // the last queries of a sequence see the most keys: heavy blocks first
+  const int slot = a.slots - 1 - (int)(blockIdx.x / a.Hq), head = blockIdx.x % a.Hq, kv_head = head / (a.Hq / a.Hkv);
+  if (tid == 0) sm.seq = -1, sm.dirty = 0;
+  __syncthreads();
+  for (int b = tid; b < a.B; b += kThreads) {
+    const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
+    if (lo >= 0 && lo / kPair + b <= slot && slot < lo / kPair + b + (hi - lo + kPair - 1) / kPair) sm.seq = b;
   }
-  const float inv = seen > 0 ? 1.f / l : 0.f;
-  uint2 o;
-  o.x = pack2(from_f<DT>(acc[0] * inv), from_f<DT>(acc[1] * inv));
-  o.y = pack2(from_f<DT>(acc[2] * inv), from_f<DT>(acc[3] * inv));
-  *reinterpret_cast<uint2*>(a.out + t * a.o_st + h * a.o_sh + 4 * lane) = o;
-  if (a.lse && lane == 0) a.lse[(int64_t)t * a.Hq + h] = m + log2f(l);
+  __syncthreads();
+  const int b = sm.seq;
+  if (b < 0) return;
+  Work w;
+  w.q_base = a.cu_q[b];
+  w.nq = min(a.cu_q[b + 1], a.Tq) - w.q_base;
+  w.k_base = max(0, a.cu_k[b]);
+  w.nk = max(0, min(a.cu_k[b + 1], a.Tk) - w.k_base);
+  w.q0 = (slot - (w.q_base / kPair + b)) * kPair;
+  w.off = w.nk - w.nq;
+  if (w.q0 >= w.nq) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int first = w.q0 + i * kRows, last = min(first + kRows, w.nq) - 1;
+    const int keys = first < w.nq ? max(0, w.limit(last, a.causal)) : 0;
+    w.n[i] = (keys + kRows - 1) / kRows;
+  }
+  const int n = max(w.n[0], w.n[1]);
+  // whether some row of the CTA must not see all of key tile j
+  auto masked = [&](int j) {
+    const int end = kRows * (j + 1);
+    return (j < w.n[0] && end > w.limit(w.q0, a.causal)) || (j < w.n[1] && end > w.limit(w.q0 + kRows, a.causal));
+  };
+
+  if (tid == 0) {
+    mbar_init(&sm.q_full, 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.checked[i], 2);
+      mbar_init(&sm.empty[i], 3);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_ready[i], 4);
+      mbar_init(&sm.o_full[i], 1);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 8) tmem_alloc(&sm.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+    if (warp == 9 && lane == 0 && n > 0) {
+      // -------------------------------------------------------- TMA loads
+      const int tiles = w.n[1] > 0 ? 2 : 1;
+      mbar_arrive_tx(&sm.q_full, tiles * kTileBytes);
+      for (int i = 0; i < tiles; ++i)
+        for (int h = 0; h < 2; ++h)
+          tma_load_3d(sm.q[i] + h * kHalfTile, &mq, 64 * h, head, w.q_base + w.q0 + i * kRows, &sm.q_full);
+      bool ok = true;
+      int sent = 0;
+      for (; sent < 2 * n; ++sent) {
+        const int st = sent % kRing;
+        if (sent >= kRing && !(ok = mbar_wait_bounded(&sm.empty[st], (sent / kRing - 1) & 1, kWait))) break;
+        const CUtensorMap* m = sent & 1 ? &mv : &mk;
+        mbar_arrive_tx(&sm.full[st], kTileBytes);
+        for (int h = 0; h < 2; ++h)
+          tma_load_3d(sm.ring[st] + h * kHalfTile, m, 64 * h, kv_head, w.k_base + (sent >> 1) * kRows, &sm.full[st]);
+      }
+      if (!ok) {  // give up: the copies under way must land before the memory is given away
+        mbar_wait_bounded(&sm.q_full, 0, kWait / 16);
+        for (int i = max(0, sent - kRing); i < sent; ++i)
+          mbar_wait_bounded(&sm.full[i % kRing], (i / kRing) & 1, kWait / 16);
+      }
+    } else if (warp == 8 && lane == 0 && n > 0) {
+      // -------------------------------------------------------------- MMAs
+      constexpr uint32_t id_s = mma_idesc(kRows, kRows, DT, 0), id_o = mma_idesc(kRows, 128, DT, 1);
+      const uint32_t q_addr = smem_u32(sm.q[0]), ring_addr = smem_u32(sm.ring[0]);
+      auto scores = [&](int i, int st) {
+        const uint64_t da = smem_desc(q_addr + i * kTileBytes, 16, 1024), db = smem_desc(ring_addr + st * kTileBytes, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t step = (k & 3) * 2 + (k >> 2) * (kHalfTile >> 4);
+          mma_ss(tmem + i * 128, da + step, db + step, id_s, k > 0);
+        }
+      };
+      auto values = [&](int i, int st, bool acc) {
+        const uint64_t db = smem_desc(ring_addr + st * kTileBytes, kHalfTile, 1024);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mma_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, db + k * (2048 >> 4), id_o, acc || k > 0);
+      };
+      // a slot is given back only if a later tile comes into it, so that no
+      // arrival is outstanding when the CTA ends
+      auto release = [&](int item) {
+        if (item + kRing < 2 * n) mma_commit(&sm.empty[item % kRing]);
+      };
+      bool ok = mbar_wait_bounded(&sm.q_full, 0, kWait) && mbar_wait_bounded(&sm.full[0], 0, kWait);
+      if (ok) {
+        tc_fence_after();
+        for (int i = 0; i < 2; ++i)
+          if (w.n[i] > 0) {
+            scores(i, 0);
+            mma_commit(&sm.s_full[i]);
+          }
+        release(0);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const int vi = 2 * j + 1, ki = 2 * j + 2, vs = vi % kRing, ks = ki % kRing;
+        ok = mbar_wait_bounded(&sm.full[vs], (vi / kRing) & 1, kWait);
+        if (ok && masked(j)) ok = mbar_wait_bounded(&sm.checked[vs], (vi / kRing) & 1, kWait);
+        for (int i = 0; ok && i < 2; ++i) {
+          if (j >= w.n[i]) continue;
+          ok = mbar_wait_bounded(&sm.p_ready[i], j & 1, kWait);
+          if (!ok) break;
+          tc_fence_after();
+          values(i, vs, j > 0);
+          if (j + 1 == w.n[i]) {
+            mma_commit(&sm.o_full[i]);
+          } else {
+            ok = mbar_wait_bounded(&sm.full[ks], (ki / kRing) & 1, kWait);
+            if (!ok) break;
+            tc_fence_after();
+            scores(i, ks);
+            mma_commit(&sm.s_full[i]);
+          }
+        }
+        if (ok) {
+          release(vi);
+          release(ki);
+        }
+      }
+    } else if (warp >= 10) {
+      // ------------------------------------------- values that are not finite
+      for (int it = 0; it < 2 * n; ++it) {
+        const int st = it % kRing;
+        if (!__all_sync(~0u, mbar_wait_bounded(&sm.full[st], (it / kRing) & 1, kWait))) break;
+        if ((it & 1) && masked(it >> 1)) {
+          uint4* p = reinterpret_cast<uint4*>(sm.ring[st]) + (warp - 10) * (kTileBytes / 32);
+          bool found = false;
+#pragma unroll 4
+          for (int x = lane; x < kTileBytes / 32; x += 32) {
+            uint4 v = p[x];
+            uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+            bool bad = false;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) bad |= not_finite<DT>(e[y]) | not_finite<DT>(e[y] >> 16);
+            if (bad) {
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                e[y] &= (not_finite<DT>(e[y]) ? 0u : 0xffffu) | (not_finite<DT>(e[y] >> 16) ? 0u : 0xffff0000u);
+              p[x] = v;
+              found = true;
+            }
+          }
+          if (found) {
+            sm.dirty = 1;
+            fence_proxy_async();
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm.checked[st]);
+          mbar_arrive(&sm.empty[st]);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
+    // ------------------------------------------------------------- softmax
+    const int i = warp >> 2, row = tid & 127, qi = w.q0 + i * kRows + row;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 lanes per warp
+    const uint32_t ts = tmem + i * 128 + lanes, to = tmem + 256 + i * 128 + lanes;
+    const int lim = w.limit(qi, a.causal);
+    float m = kNoMax, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < w.n[i]; ++j) {
+      ok = __all_sync(~0u, mbar_wait_bounded(&sm.s_full[i], j & 1, kWait));
+      if (!ok) break;
+      tc_fence_after();
+      float s[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s + 32 * c);
+      tmem_wait_ld();
+      if (a.negate) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) s[c] = -s[c];
+      }
+      const int seen = lim - kRows * j;
+      if (__any_sync(~0u, seen < kRows)) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
+      }
+      float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 128; c += 8) {
+        t0 = fmaxf(fmaxf(s[c], s[c + 1]), t0);
+        t1 = fmaxf(fmaxf(s[c + 2], s[c + 3]), t1);
+        t2 = fmaxf(fmaxf(s[c + 4], s[c + 5]), t2);
+        t3 = fmaxf(fmaxf(s[c + 6], s[c + 7]), t3);
+      }
+      const float t = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * a.scale_log2;
+      if (__any_sync(~0u, t > m + kSlack)) {
+        const float mn = fmaxf(m, t), corr = ex2(m - mn);
+        m = mn;
+        l *= corr;
+        if (j > 0) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            tmem_ld32(to + 32 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] *= corr;
+            tmem_st32(to + 32 * c, o);
+          }
+        }
+      }
+      const float base = kShift - m;
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t p[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const float p0 = ex2(fmaf(s[32 * c + 2 * x], a.scale_log2, base));
+          const float p1 = ex2(fmaf(s[32 * c + 2 * x + 1], a.scale_log2, base));
+          l0 += p0;
+          l1 += p1;
+          p[x] = pack_p<DT>(p0, p1);
+        }
+        tmem_st16(ts + 16 * c, p);
+      }
+      l += l0 + l1;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.p_ready[i]);
+    }
+    // ------------------------------------------------------------ epilogue
+    if (w.q0 + i * kRows < w.nq) {
+      // (without keys of its own, a tile still waits for its Q, whose memory it writes)
+      if (ok && n > 0) ok = __all_sync(~0u, mbar_wait_bounded(w.n[i] > 0 ? &sm.o_full[i] : &sm.q_full, 0, kWait));
+      tc_fence_after();
+      // the finished row goes through this tile's Q memory: chunk x of a row at x ^ (row & 7)
+      uint4* mine = reinterpret_cast<uint4*>(sm.q[i]) + row * 16;
+      const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float o[32];
+        if (w.n[i] > 0) {
+          tmem_ld32(to + 32 * c, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = 0.f;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint4 v;
+          uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float p0 = o[8 * x + 2 * y] * inv, p1 = o[8 * x + 2 * y + 1] * inv;
+            e[y] = l == 0.f && ok ? 0u : pack_p<DT>(p0, p1);
+          }
+          mine[(4 * c + x) ^ (row & 7)] = v;
+        }
+      }
+      if (ok && *(volatile int*)&sm.dirty && qi < w.nq) {
+        // values that were set to 0 and that this row does see
+        const uint16_t* qr = a.q + (int64_t)(w.q_base + qi) * a.q_st + head * a.q_sh;
+        for (int j = 0; j < w.n[i]; ++j) {
+          if (!masked(j)) continue;
+          for (int key = kRows * j; key < min(kRows * (j + 1), lim); ++key) {
+            const uint16_t* vr = a.v + (int64_t)(w.k_base + key) * a.v_st + kv_head * a.v_sh;
+            float p = -1.f;
+            for (int d = 0; d < kD; ++d) {
+              if (!not_finite<DT>(vr[d])) continue;
+              if (p == -1.f) {
+                const uint16_t* kr = a.k + (int64_t)(w.k_base + key) * a.k_st + kv_head * a.k_sh;
+                float dot = 0.f;
+                for (int x = 0; x < kD; ++x) dot = fmaf(to_f<DT>(qr[x]), to_f<DT>(kr[x]), dot);
+                p = ex2(fmaf(a.negate ? -dot : dot, a.scale_log2, kShift - m)) * inv;
+              }
+              uint16_t* at = reinterpret_cast<uint16_t*>(mine + ((d >> 3) ^ (row & 7))) + (d & 7);
+              *at = from_f<DT>(to_f<DT>(*at) + p * to_f<DT>(vr[d]));
+            }
+          }
+        }
+      }
+      if (a.lse && qi < w.nq)
+        a.lse[(int64_t)(w.q_base + qi) * a.Hq + head] = l == 0.f ? -INFINITY : m - kShift + log2f(l);
+      __syncwarp();
+      // two rows per instruction, 16 bytes per lane
+#pragma unroll 4
+      for (int r = 0; r < 32; r += 2) {
+        const int rr = (warp & 3) * 32 + r + (lane >> 4), x = lane & 15, at = w.q0 + i * kRows + rr;
+        if (at < w.nq)
+          *reinterpret_cast<uint4*>(a.out + (int64_t)(w.q_base + at) * a.o_st + head * a.o_sh + 8 * x) =
+              reinterpret_cast<const uint4*>(sm.q[i])[rr * 16 + (x ^ (rr & 7))];
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) tmem_free(tmem, 512);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (EncodeFn)p;
+  }();
+  return fn;
+}
+
+// boxes of 128 tokens x 64 channels of one head of [T][H][128]
+bool encode(CUtensorMap* m, const void* base, int dtype, int H, int T, int64_t sh, int64_t st) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)kD, (cuuint64_t)H, (cuuint64_t)T};
+  // a dimension of one element has no stride of its own
+  const cuuint64_t strides[2] = {(cuuint64_t)(H > 1 ? sh : kD) * 2, (cuuint64_t)(T > 1 ? st : kD) * 2};
+  const cuuint32_t box[3] = {64, 1, kRows}, one[3] = {1, 1, 1};
+  return fn(m, dtype == INNERQ_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DT>
+cudaError_t launch_prompt(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PromptDev& a,
+                          cudaStream_t s) {
+  static bool ready[64] = {false};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  constexpr int smem = sizeof(Smem) + 1024;
+  if (dev >= 64 || !ready[dev]) {
+    e = cudaFuncSetAttribute(prompt_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready[dev] = true;
+  }
+  return launch_pdl(prompt_kernel<DT>, dim3((unsigned)a.slots * a.Hq), dim3(kThreads), smem, s, mq, mk, mv, a);
+}
 
 }  // namespace
 }  // namespace innerq
@@ -80,16 +481,29 @@ extern "C" int innerq_prompt_attn(const innerq_prompt_args* p, void* stream) {
     return set_last_error(INNERQ_ERR_ARG, "null pointer");
   const int64_t st[] = {p->q_st, p->q_sh, p->k_st, p->k_sh, p->v_st, p->v_sh, p->o_st, p->o_sh};
   for (int64_t x : st)
-    if (x % 8) return set_last_error(INNERQ_ERR_ARG, "strides must be multiples of 8 elements");
+    if (x % 8 || x < 0) return set_last_error(INNERQ_ERR_ARG, "strides must be multiples of 8 elements");
   if (!aligned16(p->q) || !aligned16(p->k) || !aligned16(p->v) || !aligned16(p->out))
     return set_last_error(INNERQ_ERR_ARG, "rows must be 16-byte aligned");
-  if (p->Hq > 65535) return set_last_error(INNERQ_ERR_ARG, "more than 65535 heads");
-  PromptDev a{(const uint16_t*)p->q, (const uint16_t*)p->k, (const uint16_t*)p->v, p->q_st, p->q_sh, p->k_st, p->k_sh,
-              p->v_st, p->v_sh, p->o_st, p->o_sh, p->cu_q, p->cu_k, (uint16_t*)p->out, p->lse,
-              p->scale * 1.4426950408889634f, p->B, p->Hq, p->Hkv, p->Tq, p->Tk, p->causal};
-  const dim3 grid((p->Tq + 3) / 4, p->Hq);
+  PromptDev a;
+  a.q = (const uint16_t*)p->q; a.k = (const uint16_t*)p->k; a.v = (const uint16_t*)p->v;
+  a.q_st = p->q_st; a.q_sh = p->q_sh; a.k_st = p->k_st; a.k_sh = p->k_sh;
+  a.v_st = p->v_st; a.v_sh = p->v_sh; a.o_st = p->o_st; a.o_sh = p->o_sh;
+  a.cu_q = p->cu_q; a.cu_k = p->cu_k;
+  a.out = (uint16_t*)p->out;
+  a.lse = p->lse;
+  // a scale of 0 weighs all keys alike; masked logits are -inf, and -inf * 0 is NaN
+  a.scale_log2 = std::max(1e-37f, (p->scale < 0 ? -p->scale : p->scale) * 1.4426950408889634f);
+  a.negate = p->scale < 0;
+  a.B = p->B; a.Hq = p->Hq; a.Hkv = p->Hkv; a.Tq = p->Tq; a.Tk = p->Tk; a.causal = p->causal;
+  a.slots = p->Tq / kPair + p->B;
+  if ((int64_t)a.slots * a.Hq > 0x7fffffff) return set_last_error(INNERQ_ERR_ARG, "too many blocks for one launch");
+  CUtensorMap mq, mk, mv;
+  const bool none = p->Tk == 0;  // no keys: the maps are never used
+  if (!encode(&mq, p->q, p->dtype, p->Hq, p->Tq, p->q_sh, p->q_st) ||
+      !encode(&mk, none ? p->q : p->k, p->dtype, none ? 1 : p->Hkv, none ? 1 : p->Tk, p->k_sh, p->k_st) ||
+      !encode(&mv, none ? p->q : p->v, p->dtype, none ? 1 : p->Hkv, none ? 1 : p->Tk, p->v_sh, p->v_st))
+    return set_last_error(INNERQ_ERR_ARG, "q, k and v: strides or sizes that a tensor map cannot describe");
   const cudaStream_t s = (cudaStream_t)stream;
-  const cudaError_t e = p->dtype == INNERQ_DT_BF16 ? launch_pdl(prompt_simple_kernel<BF16>, grid, dim3(128), 0, s, a)
-                                                   : launch_pdl(prompt_simple_kernel<F16>, grid, dim3(128), 0, s, a);
+  const cudaError_t e = p->dtype == INNERQ_DT_BF16 ? launch_prompt<BF16>(mq, mk, mv, a, s) : launch_prompt<F16>(mq, mk, mv, a, s);
   return e == cudaSuccess ? INNERQ_OK : set_last_error(INNERQ_ERR_CUDA, "prompt_attn: %s", cudaGetErrorString(e));
 }

@@ -29,7 +29,7 @@ def _rows(t: torch.Tensor, what: str, dtype, device) -> torch.Tensor:
     if t.dtype != dtype or t.device != device:
         raise TypeError(f"{what} is {t.dtype} on {t.device}, expected {dtype} on {device}")
     st, sh, sd = t.stride()
-    if sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16:
+    if sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16 or (st == 0 and t.shape[0] > 1) or (sh == 0 and t.shape[1] > 1):
         t = t.contiguous()
         if t.data_ptr() % 16:  # a contiguous view at an odd offset
             t = t.clone()
