@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libinnerq_b200.so")
 
@@ -78,42 +79,12 @@ class AttnArgs(C.Structure):
     ]
 
 
-class Paged(C.Structure):
-    _fields_ = [
-        ("struct_size", C.c_int32), ("dtype", C.c_int32), ("D", C.c_int32), ("Hkv", C.c_int32),
-        ("page_tiles", C.c_int32), ("n_pages", C.c_int32), ("n_slots", C.c_int32),
-        ("w_sink", C.c_int32), ("w_recent", C.c_int32), ("B", C.c_int32), ("max_pages", C.c_int32),
-        ("pages", C.c_void_p), ("dense_k", C.c_void_p), ("dense_v", C.c_void_p),
-        ("table", C.c_void_p), ("table_stride", C.c_int64),
-        ("slots", C.c_void_p), ("seq_lens", C.c_void_p),
-    ]
-
-
-class PagedNew(C.Structure):
-    _fields_ = [
-        ("struct_size", C.c_int32), ("Hq", C.c_int32), ("T", C.c_int32), ("rot_dim", C.c_int32),
-        ("interleaved", C.c_int32), ("max_pos", C.c_int32),
-        ("q", C.c_void_p), ("q_st", C.c_int64), ("q_sh", C.c_int64),
-        ("k", C.c_void_p), ("k_st", C.c_int64), ("k_sh", C.c_int64),
-        ("v", C.c_void_p), ("v_st", C.c_int64), ("v_sh", C.c_int64),
-        ("cu_seqlens", C.c_void_p), ("cos", C.c_void_p), ("sin", C.c_void_p), ("cs_stride", C.c_int64),
-        ("q_out", C.c_void_p), ("qo_st", C.c_int64), ("qo_sh", C.c_int64),
-        ("k_out", C.c_void_p), ("ko_st", C.c_int64), ("ko_sh", C.c_int64),
-    ]
-
-
-class PromptArgs(C.Structure):
-    _fields_ = [
-        ("struct_size", C.c_int32), ("dtype", C.c_int32), ("D", C.c_int32), ("B", C.c_int32),
-        ("Hq", C.c_int32), ("Hkv", C.c_int32), ("Tq", C.c_int32), ("Tk", C.c_int32),
-        ("causal", C.c_int32), ("scale", C.c_float),
-        ("q", C.c_void_p), ("q_st", C.c_int64), ("q_sh", C.c_int64),
-        ("k", C.c_void_p), ("k_st", C.c_int64), ("k_sh", C.c_int64),
-        ("v", C.c_void_p), ("v_st", C.c_int64), ("v_sh", C.c_int64),
-        ("cu_q", C.c_void_p), ("cu_k", C.c_void_p),
-        ("out", C.c_void_p), ("o_st", C.c_int64), ("o_sh", C.c_int64), ("lse", C.c_void_p),
-    ]
-
+# innerq_paged, innerq_paged_new and innerq_prompt_args, field by field in the
+# header's order, as struct formats: packing them in one call instead of
+# assigning ctypes fields keeps host time per launch low.
+PAGED_FORMAT = struct.Struct("@11i4x3PPqPP")
+PAGED_NEW_FORMAT = struct.Struct("@6i" + "Pqq" * 3 + "3Pq" + "Pqq" * 2)
+PROMPT_FORMAT = struct.Struct("@9if" + "Pqq" * 3 + "2P" + "Pqq" + "P")
 
 _lib = None
 
@@ -150,12 +121,12 @@ def load() -> C.CDLL:
         "innerq_lse_merge": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, i64, vp, vp]),
         "innerq_partials_rank_floats": (i64, [i32, i32, i32, i32]),
         "innerq_lse_merge_ranks": (i32, [vp, i32, i64, i32, i32, i32, i32, i32, vp, i64, i64, vp, vp]),
-        "innerq_paged_append": (i32, [C.POINTER(Paged), C.POINTER(PagedNew), vp]),
-        "innerq_paged_read": (i32, [C.POINTER(Paged), vp, vp, i32, vp, vp, vp]),
-        "innerq_paged_attn_workspace": (i64, [C.POINTER(Paged), i32]),
-        "innerq_paged_attn": (i32, [C.POINTER(Paged), i32, vp, i64, i64, C.c_float, vp, i64, vp, i64, i64,
+        "innerq_paged_append": (i32, [C.c_char_p, C.c_char_p, vp]),
+        "innerq_paged_read": (i32, [C.c_char_p, vp, vp, i32, vp, vp, vp]),
+        "innerq_paged_attn_workspace": (i64, [C.c_char_p, i32]),
+        "innerq_paged_attn": (i32, [C.c_char_p, i32, vp, i64, i64, C.c_float, vp, i64, vp, i64, i64,
                                     vp, vp]),
-        "innerq_prompt_attn": (i32, [C.POINTER(PromptArgs), vp]),
+        "innerq_prompt_attn": (i32, [C.c_char_p, vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(lib, name)

@@ -24,7 +24,6 @@ passes the rows of the sequences of a step.  A sequence of L tokens needs
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 
 import torch
@@ -46,27 +45,30 @@ class PagedCache:
 
     def __init__(self, pages: torch.Tensor, dense_k: torch.Tensor, dense_v: torch.Tensor, w_sink: int, w_recent: int):
         require_cuda(pages, "pages")
-        n_slots, hkv, rows, d = dense_k.shape
+        dshape, pshape = dense_k.shape, pages.shape
+        if len(dshape) != 4 or len(pshape) != 4:
+            raise ValueError(f"pages {tuple(pshape)} and slots {tuple(dshape)} must have four dimensions")
+        n_slots, hkv, rows, d = dshape
         if d != D_SUPPORTED:
             raise NotImplementedError(f"head_dim {d} is not built (128 is)")
         if w_sink < 0 or w_recent < 0 or w_sink % TILE or w_recent % TILE:
             raise ValueError(f"sink {w_sink} and recent window {w_recent} must be multiples of {TILE}")
-        if rows != w_sink + w_recent + TILE or dense_v.shape != dense_k.shape or dense_v.dtype != dense_k.dtype:
+        dtype = dense_k.dtype
+        if rows != w_sink + w_recent + TILE or dense_v.shape != dshape or dense_v.dtype != dtype:
             raise ValueError(f"slots must hold {w_sink + w_recent + TILE} rows of keys and of values, "
-                             f"got {tuple(dense_k.shape)} and {tuple(dense_v.shape)}")
-        if pages.dtype != torch.uint8 or pages.dim() != 4 or pages.shape[1] != hkv or pages.shape[3] != BLOCK_BYTES:
-            raise ValueError(f"pages must be uint8 [pages, {hkv}, tiles, {BLOCK_BYTES}], got {pages.dtype} {tuple(pages.shape)}")
+                             f"got {tuple(dshape)} and {tuple(dense_v.shape)}")
+        if pages.dtype != torch.uint8 or pshape[1] != hkv or pshape[3] != BLOCK_BYTES:
+            raise ValueError(f"pages must be uint8 [pages, {hkv}, tiles, {BLOCK_BYTES}], got {pages.dtype} {tuple(pshape)}")
         if not (pages.is_contiguous() and dense_k.is_contiguous() and dense_v.is_contiguous()):
             raise ValueError("pages and slots must be contiguous")
-        if not (pages.device == dense_k.device == dense_v.device):
+        device = pages.device
+        if not (device == dense_k.device == dense_v.device):
             raise ValueError("pages and slots must be on one device")
         self.pages, self.dense_k, self.dense_v = pages, dense_k, dense_v
         self.w_sink, self.w_recent = w_sink, w_recent
-        self.dtype, self.device = dense_k.dtype, pages.device
-        self.n_kv_heads, self.page_size = hkv, pages.shape[2] * TILE
-        self._c = _lib.Paged(
-            C.sizeof(_lib.Paged), dtype_code(dense_k.dtype), d, hkv, pages.shape[2], pages.shape[0], n_slots, w_sink,
-            w_recent, 0, 0, pages.data_ptr(), dense_k.data_ptr(), dense_v.data_ptr(), None, 0, None, None)
+        self.dtype, self.device = dtype, device
+        self.n_kv_heads, self.page_size = hkv, pshape[2] * TILE
+        self._head = (_lib.PAGED_FORMAT.size, dtype_code(dtype), d, hkv, pshape[2], pshape[0], n_slots, w_sink, w_recent)
 
     @classmethod
     def allocate(cls, n_pages: int, n_kv_heads: int, n_slots: int, page_size: int = 64, w_sink: int = 32,
@@ -88,20 +90,23 @@ class PagedCache:
         return -(-self.packed_tokens(length) // self.page_size)
 
     # ---------------------------------------------------------------- steps
-    def _args(self, page_table, slots, seq_lens) -> _lib.Paged:
-        if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != self.device:
-            raise TypeError(f"page_table must be int32 [sequences, pages] on {self.device}")
+    def _args(self, page_table, slots, seq_lens):
+        """(innerq_paged as bytes, number of sequences, tensors that must live
+        until the launch)."""
+        device = self.device
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != device:
+            raise TypeError(f"page_table must be int32 [sequences, pages] on {device}")
         B, columns = page_table.shape
-        if columns > 1 and page_table.stride(1) != 1:
+        stride, step = page_table.stride()
+        if columns > 1 and step != 1:
             page_table = page_table.contiguous()
-        slots = _index(slots, "slots", B, self.device)
-        seq_lens = _index(seq_lens, "seq_lens", B, self.device)
-        c = _lib.Paged.from_buffer_copy(self._c)
-        c.B, c.max_pages = B, columns
-        c.table, c.table_stride = page_table.data_ptr(), page_table.stride(0)
-        c.slots, c.seq_lens = slots.data_ptr(), seq_lens.data_ptr()
-        c._keep = (page_table, slots, seq_lens)  # copies live until the launch
-        return c
+            stride = columns
+        slots = _index(slots, "slots", B, device)
+        seq_lens = _index(seq_lens, "seq_lens", B, device)
+        c = _lib.PAGED_FORMAT.pack(*self._head, B, columns, self.pages.data_ptr(), self.dense_k.data_ptr(),
+                                   self.dense_v.data_ptr(), page_table.data_ptr(), stride, slots.data_ptr(),
+                                   seq_lens.data_ptr())
+        return c, B, (page_table, slots, seq_lens)
 
     def append(self, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
                slots: torch.Tensor, seq_lens: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
@@ -119,45 +124,52 @@ class PagedCache:
         rotated.  Returns the rotated q (None without q), with return_k the
         pair (q, rotated k): the 16-bit keys that attention over the prompt
         reads."""
-        k = _rows(k, "key", self.dtype, self.device)
-        v = _rows(v, "value", self.dtype, self.device)
-        T = k.shape[0]
-        if k.shape != (T, self.n_kv_heads, D_SUPPORTED) or v.shape != k.shape:
-            raise ValueError(f"key {tuple(k.shape)} and value {tuple(v.shape)} must be [tokens, {self.n_kv_heads}, 128]")
-        c = self._args(page_table, slots, seq_lens)
-        a = _lib.PagedNew()
-        a.struct_size, a.T = C.sizeof(_lib.PagedNew), T
+        dtype, device, hkv = self.dtype, self.device, self.n_kv_heads
+        k, v = _rows(k, "key", dtype, device), _rows(v, "value", dtype, device)
+        shape = k.shape
+        T = shape[0]
+        if shape[1] != hkv or shape[2] != D_SUPPORTED or v.shape != shape:
+            raise ValueError(f"key {tuple(shape)} and value {tuple(v.shape)} must be [tokens, {hkv}, 128]")
+        c, B, keep = self._args(page_table, slots, seq_lens)
+        k_st, k_sh, _ = k.stride()
+        v_st, v_sh, _ = v.stride()
         q_out = k_out = None
+        Hq = q_ptr = q_st = q_sh = qo_ptr = ko_ptr = 0
         if q is not None:
-            q = _rows(q, "query", self.dtype, self.device)
-            if q.shape[0] != T or q.shape[2] != D_SUPPORTED:
+            q = _rows(q, "query", dtype, device)
+            n, Hq, d = q.shape
+            if n != T or d != D_SUPPORTED:
                 raise ValueError(f"query {tuple(q.shape)} must be [{T}, heads, 128]")
-            q_out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
-            a.Hq, a.q, a.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
-            a.q_st, a.q_sh, _ = q.stride()
-            a.qo_st, a.qo_sh = q.shape[1] * D_SUPPORTED, D_SUPPORTED
-        a.k, a.v = k.data_ptr(), v.data_ptr()
-        a.k_st, a.k_sh, _ = k.stride()
-        a.v_st, a.v_sh, _ = v.stride()
+            q_out = q.new_empty((T, Hq, d))
+            q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
+            q_st, q_sh, _ = q.stride()
         if return_k:
-            k_out = torch.empty(k.shape, dtype=self.dtype, device=self.device)
-            a.k_out = k_out.data_ptr()
-            a.ko_st, a.ko_sh = self.n_kv_heads * D_SUPPORTED, D_SUPPORTED
+            k_out = k.new_empty(shape)
+            ko_ptr = k_out.data_ptr()
+        cu = 0
         if cu_seqlens is not None:
-            cu_seqlens = _index(cu_seqlens, "cu_seqlens", c.B + 1, self.device)
-            a.cu_seqlens = cu_seqlens.data_ptr()
-        elif T != c.B:
-            raise ValueError(f"{T} tokens for {c.B} sequences need cu_seqlens")
-        if (cos is None) != (sin is None):
-            raise ValueError("cos and sin come together")
-        if cos is not None:
+            cu_seqlens = _index(cu_seqlens, "cu_seqlens", B + 1, device)
+            cu = cu_seqlens.data_ptr()
+        elif T != B:
+            raise ValueError(f"{T} tokens for {B} sequences need cu_seqlens")
+        rot = max_pos = c_ptr = s_ptr = c_stride = 0
+        if cos is not None and sin is not None:
             cos, sin = self._table(cos), self._table(sin)
-            if cos.shape != sin.shape or cos.stride(0) != sin.stride(0):
-                raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} differ")
-            a.rot_dim, a.max_pos, a.cs_stride = 2 * cos.shape[1], cos.shape[0], cos.stride(0)
-            a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
-            a.interleaved = int(bool(interleaved))
-        _lib.call("innerq_paged_append", C.byref(c), C.byref(a), stream_ptr(self.device))
+            max_pos, half = cos.shape
+            c_stride = cos.stride(0)
+            if sin.shape != cos.shape or sin.stride(0) != c_stride:
+                cos, sin = cos.contiguous(), sin.contiguous()
+                c_stride = half
+                if sin.shape != cos.shape:
+                    raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} differ")
+            rot, c_ptr, s_ptr = 2 * half, cos.data_ptr(), sin.data_ptr()
+        elif cos is not None or sin is not None:
+            raise ValueError("cos and sin come together")
+        a = _lib.PAGED_NEW_FORMAT.pack(
+            _lib.PAGED_NEW_FORMAT.size, Hq, T, rot, 1 if interleaved else 0, max_pos, q_ptr, q_st, q_sh, k.data_ptr(), k_st,
+            k_sh, v.data_ptr(), v_st, v_sh, cu, c_ptr, s_ptr, c_stride, qo_ptr, Hq * D_SUPPORTED, D_SUPPORTED, ko_ptr,
+            hkv * D_SUPPORTED, D_SUPPORTED)
+        _lib.call("innerq_paged_append", c, a, stream_ptr(device))
         return (q_out, k_out) if return_k else q_out
 
     def _table(self, t: torch.Tensor) -> torch.Tensor:
@@ -174,25 +186,28 @@ class PagedCache:
         over its seq_lens[b] cached tokens (this step's included) -> out
         [B, Hq, 128].  A sequence without tokens gets zeros.  lse (optional,
         fp32 [B, Hq]): log2-sum-exp2 of the scaled logits."""
-        q = _rows(q, "query", self.dtype, self.device)
-        c = self._args(page_table, slots, seq_lens)
+        dtype, device = self.dtype, self.device
+        q = _rows(q, "query", dtype, device)
+        c, n, keep = self._args(page_table, slots, seq_lens)
         B, Hq, D = q.shape
-        if B != c.B or D != D_SUPPORTED:
-            raise ValueError(f"query {tuple(q.shape)} must be [{c.B}, heads, 128]")
+        if B != n or D != D_SUPPORTED:
+            raise ValueError(f"query {tuple(q.shape)} must be [{n}, heads, 128]")
         if out is None:
-            out = torch.empty((B, Hq, D), dtype=self.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype != self.dtype or out.device != self.device or out.stride(2) != 1:
+            out = q.new_empty((B, Hq, D))
+        elif out.shape != q.shape or out.dtype != dtype or out.device != device or out.stride(2) != 1:
             raise ValueError("out must be like the query, with contiguous rows")
         if lse is not None and (lse.shape != (B, Hq) or lse.dtype != torch.float32 or not lse.is_contiguous()
-                                or lse.device != self.device):
+                                or lse.device != device):
             raise ValueError("lse must be a contiguous fp32 [sequences, heads] tensor")
-        ws_bytes = _lib.load().innerq_paged_attn_workspace(C.byref(c), Hq)
+        ws_bytes = _lib.load().innerq_paged_attn_workspace(c, Hq)
         if ws_bytes < 0:
             raise _lib.InnerqError("innerq_paged_attn_workspace", -1, _lib.last_error())
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=self.device)  # of this stream
-        _lib.call("innerq_paged_attn", C.byref(c), Hq, q.data_ptr(), q.stride(0), q.stride(1),
-                  float(scale if scale is not None else 1.0 / math.sqrt(D)), ws.data_ptr(), ws_bytes, out.data_ptr(),
-                  out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), stream_ptr(self.device))
+        ws = self.pages.new_empty(ws_bytes)  # bytes of this stream's own
+        q_sb, q_sh, _ = q.stride()
+        o_sb, o_sh, _ = out.stride()
+        _lib.call("innerq_paged_attn", c, Hq, q.data_ptr(), q_sb, q_sh,
+                  1.0 / math.sqrt(D) if scale is None else float(scale), ws.data_ptr(), ws_bytes, out.data_ptr(),
+                  o_sb, o_sh, None if lse is None else lse.data_ptr(), stream_ptr(device))
         return out
 
     def read(self, page_table: torch.Tensor, slots: torch.Tensor, seq_lens: torch.Tensor, starts: torch.Tensor,
@@ -202,11 +217,11 @@ class PagedCache:
         [n_tokens, Hkv, 128] is token starts[b] + i of sequence b.  n_tokens is
         cu_seqlens[-1], known to the caller; positions outside a sequence read
         as NaN.  Feeds prompt_attention with the tokens before a chunk."""
-        c = self._args(page_table, slots, seq_lens)
-        starts = _index(starts, "starts", c.B, self.device)
-        cu_seqlens = _index(cu_seqlens, "cu_seqlens", c.B + 1, self.device)
+        c, B, keep = self._args(page_table, slots, seq_lens)
+        starts = _index(starts, "starts", B, self.device)
+        cu_seqlens = _index(cu_seqlens, "cu_seqlens", B + 1, self.device)
         shape = (n_tokens, self.n_kv_heads, D_SUPPORTED)
-        k, v = (torch.empty(shape, dtype=self.dtype, device=self.device) for _ in range(2))
-        _lib.call("innerq_paged_read", C.byref(c), starts.data_ptr(), cu_seqlens.data_ptr(), n_tokens, k.data_ptr(),
+        k, v = self.dense_k.new_empty(shape), self.dense_k.new_empty(shape)
+        _lib.call("innerq_paged_read", c, starts.data_ptr(), cu_seqlens.data_ptr(), n_tokens, k.data_ptr(),
                   v.data_ptr(), stream_ptr(self.device))
         return k, v

@@ -11,7 +11,6 @@ prefills through Hugging Face sdpa, one length for the whole batch
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 
 import torch
@@ -74,17 +73,16 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         raise ValueError("cu_seqlens must have at least one element")
     cu_k = cu if cu_seqlens_k is None else _index(cu_seqlens_k, "cu_seqlens_k", B + 1, q.device)
     if out is None:
-        out = torch.empty((Tq, Hq, D), dtype=q.dtype, device=q.device)
+        out = q.new_empty((Tq, Hq, D))
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
         raise ValueError("out must be like the query, with contiguous rows")
     if lse is not None and (lse.shape != (Tq, Hq) or lse.dtype != torch.float32 or not lse.is_contiguous()
                             or lse.device != q.device):
         raise ValueError("lse must be a contiguous fp32 [tokens, heads] tensor")
-    a = _lib.PromptArgs(
-        C.sizeof(_lib.PromptArgs), dt, D, B, Hq, Hkv, Tq, Tk, int(bool(causal)),
-        float(scale if scale is not None else 1.0 / math.sqrt(D)),
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-        v.data_ptr(), v.stride(0), v.stride(1), cu.data_ptr(), cu_k.data_ptr(),
-        out.data_ptr(), out.stride(0), out.stride(1), None if lse is None else lse.data_ptr())
-    _lib.call("innerq_prompt_attn", C.byref(a), stream_ptr(q.device))
+    a = _lib.PROMPT_FORMAT.pack(
+        _lib.PROMPT_FORMAT.size, dt, D, B, Hq, Hkv, Tq, Tk, 1 if causal else 0,
+        1.0 / math.sqrt(D) if scale is None else float(scale), q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2],
+        v.data_ptr(), *v.stride()[:2], cu.data_ptr(), cu_k.data_ptr(), out.data_ptr(), *out.stride()[:2],
+        0 if lse is None else lse.data_ptr())
+    _lib.call("innerq_prompt_attn", a, stream_ptr(q.device))
     return out

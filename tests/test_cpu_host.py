@@ -206,3 +206,39 @@ def test_cache_state_format_without_gpu():
         c2.load_state_dict(dict(sd, format="other"))
     with pytest.raises(ValueError):
         c2.load_state_dict(dict(sd, layers=sd["layers"][:2]))
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="needs gcc")
+def test_struct_formats_match_c_layout(tmp_path):
+    """The packed argument blocks of the paged cache and of prompt attention:
+    every field's offset and the size, as a C compiler lays them out."""
+    from innerq_b200 import _lib
+    src = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    fmts = {"innerq_paged": _lib.PAGED_FORMAT, "innerq_paged_new": _lib.PAGED_NEW_FORMAT,
+            "innerq_prompt_args": _lib.PROMPT_FORMAT}
+    body = '#include "innerq_b200.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(){\n'
+    for name in fmts:
+        decl = re.search(r"typedef struct \{([^}]*)\} %s;" % name, src).group(1)
+        fields = [re.sub(r"^.*[ *]", "", f.strip()) for part in decl.split(";") for f in part.split(",") if f.strip()]
+        fields = [f for f in fields if f]
+        body += f'printf("{name} %zu", sizeof({name}));\n'
+        body += "".join(f'printf(" %zu:%zu", offsetof({name}, {f}), sizeof((({name}*)0)->{f}));\n' for f in fields)
+        body += 'printf("\\n");\n'
+    c = tmp_path / "t.c"
+    c.write_text(body + "return 0;}\n")
+    exe = tmp_path / "t"
+    subprocess.run(["gcc", "-I", os.path.dirname(HEADER), str(c), "-o", str(exe)], check=True)
+    for line in subprocess.run([str(exe)], capture_output=True, text=True).stdout.splitlines():
+        name, size, *fields = line.split()
+        fmt = fmts[name]
+        assert int(size) == fmt.size, name
+        # a value of ones in one field at a time lands where C reads it
+        values = re.findall(r"(\d*)([iPqf])", fmt.format.replace("4x", ""))
+        kinds = "".join(k * (int(n) if n else 1) for n, k in values)
+        assert len(kinds) == len(fields), (name, kinds, fields)
+        for i, f in enumerate(fields):
+            off, width = map(int, f.split(":"))
+            args = [0.0 if k == "f" else 0 for k in kinds]
+            args[i] = 1.0 if kinds[i] == "f" else 1
+            packed = fmt.pack(*args)
+            assert any(packed[off:off + width]) and not any(packed[:off] + packed[off + width:]), (name, i)
