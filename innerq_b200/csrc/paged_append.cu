@@ -70,66 +70,69 @@ __device__ __forceinline__ void unit_chunks(const NewDev& n, int u, int& d0, int
   }
 }
 
-template <int DT>
-__device__ __forceinline__ void rotate_unit(const NewDev& n, int u, int d0, int pos, uint4& x, uint4& y) {
-  if (n.rot == 0) return;
-  if (d0 >= n.rot) return;
-  uint32_t* xa = reinterpret_cast<uint32_t*>(&x);
-  uint32_t* ya = reinterpret_cast<uint32_t*>(&y);
-  if ((unsigned)pos >= (unsigned)n.max_pos) {  // beyond the table: NaN, never a wrong angle
-    const uint32_t nan2 = nan16<DT>() * 0x00010001u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) xa[i] = ya[i] = nan2;
-    return;
-  }
-  const float* c = n.cos + pos * n.cs_stride + 8 * u;
-  const float* s = n.sin + pos * n.cs_stride + 8 * u;
-  float cs[8], sn[8];
+// two fp32 values rounded to the dtype, as one word
+template <int DT> __device__ __forceinline__ uint32_t round2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (DT == F16)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// the halves of a word of the dtype as fp32
+template <int DT> __device__ __forceinline__ float lo_f(uint32_t w) {
+  if constexpr (DT == F16) return __low2float(as_pair<F16>(w));
+  return __uint_as_float(w << 16);
+}
+template <int DT> __device__ __forceinline__ float hi_f(uint32_t w) {
+  if constexpr (DT == F16) return __high2float(as_pair<F16>(w));
+  return __uint_as_float(w & 0xffff0000u);
+}
+
+// the angles of a unit at one position
+struct Angles {
+  float c[8], s[8];
+  bool rotated, known;
+};
+
+__device__ __forceinline__ void load_angles(const NewDev& n, int u, int d0, int pos, Angles& g) {
+  g.rotated = d0 < n.rot;
+  g.known = (unsigned)pos < (unsigned)n.max_pos;
+  if (!g.rotated || !g.known) return;
+  const float4* c = reinterpret_cast<const float4*>(n.cos + pos * n.cs_stride + 8 * u);
+  const float4* s = reinterpret_cast<const float4*>(n.sin + pos * n.cs_stride + 8 * u);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float4 c4 = __ldg(reinterpret_cast<const float4*>(c) + i);
-    const float4 s4 = __ldg(reinterpret_cast<const float4*>(s) + i);
-    cs[4 * i] = c4.x; cs[4 * i + 1] = c4.y; cs[4 * i + 2] = c4.z; cs[4 * i + 3] = c4.w;
-    sn[4 * i] = s4.x; sn[4 * i + 1] = s4.y; sn[4 * i + 2] = s4.z; sn[4 * i + 3] = s4.w;
-  }
-  if (!n.interleaved) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float a0 = to_f<DT>(xa[i] & 0xffff), a1 = to_f<DT>(xa[i] >> 16);
-      float b0 = to_f<DT>(ya[i] & 0xffff), b1 = to_f<DT>(ya[i] >> 16);
-      rotate(a0, b0, cs[2 * i], sn[2 * i]);
-      rotate(a1, b1, cs[2 * i + 1], sn[2 * i + 1]);
-      xa[i] = pack2(from_f<DT>(a0), from_f<DT>(a1));
-      ya[i] = pack2(from_f<DT>(b0), from_f<DT>(b1));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float a = to_f<DT>(xa[i] & 0xffff), b = to_f<DT>(xa[i] >> 16);
-      rotate(a, b, cs[i], sn[i]);
-      xa[i] = pack2(from_f<DT>(a), from_f<DT>(b));
-      a = to_f<DT>(ya[i] & 0xffff), b = to_f<DT>(ya[i] >> 16);
-      rotate(a, b, cs[4 + i], sn[4 + i]);
-      ya[i] = pack2(from_f<DT>(a), from_f<DT>(b));
-    }
+    const float4 c4 = __ldg(c + i), s4 = __ldg(s + i);
+    g.c[4 * i] = c4.x; g.c[4 * i + 1] = c4.y; g.c[4 * i + 2] = c4.z; g.c[4 * i + 3] = c4.w;
+    g.s[4 * i] = s4.x; g.s[4 * i + 1] = s4.y; g.s[4 * i + 2] = s4.z; g.s[4 * i + 3] = s4.w;
   }
 }
 
-// One 8-channel chunk d0.. of a rotated key (the partner chunk is read too).
+// rotate the two chunks of a unit
 template <int DT>
-__device__ __forceinline__ uint4 key_chunk(const NewDev& n, const uint16_t* row, int d0, int pos) {
-  const int half = n.rot >> 1;
-  if (d0 >= n.rot) return *reinterpret_cast<const uint4*>(row + d0);
-  if (n.interleaved) {
-    const int u = d0 >> 4;
-    uint4 x = *reinterpret_cast<const uint4*>(row + 16 * u), y = *reinterpret_cast<const uint4*>(row + 16 * u + 8);
-    rotate_unit<DT>(n, u, 16 * u, pos, x, y);
-    return (d0 & 8) ? y : x;
+__device__ __forceinline__ void rotate_unit(const Angles& g, int interleaved, uint4& x, uint4& y) {
+  if (!g.rotated) return;
+  uint32_t* xa = reinterpret_cast<uint32_t*>(&x);
+  uint32_t* ya = reinterpret_cast<uint32_t*>(&y);
+  if (!g.known) {  // beyond the table: NaN, never a wrong angle
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xa[i] = ya[i] = nan16<DT>() * 0x00010001u;
+    return;
   }
-  const int u = (d0 < half ? d0 : d0 - half) >> 3;
-  uint4 x = *reinterpret_cast<const uint4*>(row + 8 * u), y = *reinterpret_cast<const uint4*>(row + 8 * u + half);
-  rotate_unit<DT>(n, u, 8 * u, pos, x, y);
-  return d0 < half ? x : y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a0 = lo_f<DT>(xa[i]), a1 = hi_f<DT>(xa[i]), b0 = lo_f<DT>(ya[i]), b1 = hi_f<DT>(ya[i]);
+    if (interleaved) {
+      rotate(a0, a1, g.c[i], g.s[i]);
+      rotate(b0, b1, g.c[4 + i], g.s[4 + i]);
+    } else {
+      rotate(a0, b0, g.c[2 * i], g.s[2 * i]);
+      rotate(a1, b1, g.c[2 * i + 1], g.s[2 * i + 1]);
+    }
+    xa[i] = round2<DT>(a0, a1);
+    ya[i] = round2<DT>(b0, b1);
+  }
 }
 
 // the scale of a group from the bits of its largest magnitude
@@ -151,93 +154,115 @@ __device__ __forceinline__ uint32_t maxbits2(uint32_t a, uint32_t b) {
   return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu);
 }
 
-// quantize the 32-token tile `t` (32-token units after the sink) of sequence
-// b, head h; 128 threads
+__device__ __forceinline__ uint32_t max4(const uint4& v) {
+  const uint32_t m = maxbits2(maxbits2(v.x, v.y), maxbits2(v.z, v.w));
+  return max(m & 0xffff, m >> 16);
+}
+
+// The scale of a group and its seven cuts (rounded up to the dtype) as eight
+// 16-bit values: cuts 0-6, then the scale.
+template <int DT> __device__ __forceinline__ uint4 group_of(uint16_t amax) {
+  const uint16_t scale = scale_of<DT>(amax);
+  uint32_t c[7];
+  cuts_of<DT>(scale, c);
+  return make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | (uint32_t)scale << 16);
+}
+
+constexpr int kAppendThreads = 256;  // 32 tokens x 8 units, or 64 channel pairs x 4 l
+
+// Quantize the 32-token tile `t` (32-token units after the sink) of sequence b
+// for heads h0 .. h1.  A thread is a unit (two chunks of 8 channels) of one
+// token for the keys, whose angles it keeps over the heads, and 8 tokens of a
+// pair of channels for the values.  Maxima meet in shared memory, one thread
+// per group turns them into the group's cuts, and every thread codes its
+// values against them.
 template <int DT>
-__device__ void pack_tile(const PagedDev& c, const NewDev& n, int b, int h, int t, int len0, int cu0) {
-  uint8_t* blk = c.tile(b, h, t);
-  const int64_t base = c.dense_base(b, h);
-  if (blk == nullptr || base < 0) return;
-  const int first = c.w_sink + 32 * t;
-  const int tid = threadIdx.x;
-  __shared__ uint32_t vmax[2][64];
-  {  // keys: one thread per (token, group of 32 channels)
-    const int r = tid >> 2, g = tid & 3, pos = first + r;
-    uint4 x[4];
-    if (pos >= len0) {
-      const uint16_t* row = n.k + (int64_t)(cu0 + pos - len0) * n.k_st + h * n.k_sh;
+__device__ void pack_tile(const PagedDev& c, const NewDev& n, int b, int h0, int h1, int t, int len0, int cu0) {
+  __shared__ __align__(16) uint16_t kmax[32][16];
+  __shared__ uint32_t vmax[4][64];
+  __shared__ uint4 kgroup[32][4], vgroup[128];
+  const int first = c.w_sink + 32 * t, tid = threadIdx.x;
+  const int r = tid >> 3, u = tid & 7, pos = first + r;  // keys
+  const int dp = tid & 63, l = tid >> 6;                 // values
+  if (c.tile(b, h0, t) == nullptr || c.dense_base(b, h0) < 0) return;
+  int d0, d1;
+  unit_chunks(n, u, d0, d1);
+  const bool fresh = pos >= len0;
+  Angles g;
+  g.rotated = false;
+  if (fresh) load_angles(n, u, d0, pos, g);
+#pragma unroll 1
+  for (int h = h0; h < h1; ++h) {
+    uint8_t* blk = c.tile(b, h, t);
+    const int64_t base = c.dense_base(b, h);
+    const uint16_t* row = fresh ? n.k + (int64_t)(cu0 + pos - len0) * n.k_st + h * n.k_sh
+                                : c.dk + base + (int64_t)c.row_of(pos) * kD;
+    uint4 k[2] = {*reinterpret_cast<const uint4*>(row + d0), *reinterpret_cast<const uint4*>(row + d1)};
+    uint32_t vv[8], m = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = key_chunk<DT>(n, row, 32 * g + 8 * i, pos);
-    } else {
-      const uint4* row = reinterpret_cast<const uint4*>(c.dk + base + (int64_t)c.row_of(pos) * kD + 32 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = row[i];
+    for (int i = 0; i < 8; ++i) {  // nibble i: token 8 (i & 3) + 2 l + (i >> 2)
+      const int p = first + 8 * (i & 3) + 2 * l + (i >> 2);
+      const uint16_t* vr = p >= len0 ? n.v + (int64_t)(cu0 + p - len0) * n.v_st + h * n.v_sh
+                                     : c.dv + base + (int64_t)c.row_of(p) * kD;
+      vv[i] = *reinterpret_cast<const uint32_t*>(vr + 2 * dp);
     }
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
-    uint32_t m = 0;
+    rotate_unit<DT>(g, n.interleaved, k[0], k[1]);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = maxbits2(m, w[i]);
-    const uint16_t scale = scale_of<DT>(max(m & 0xffff, m >> 16));
-    uint32_t cut[7];
-    cuts_of<DT>(scale, cut);
+    for (int i = 0; i < 8; ++i) m = maxbits2(m, vv[i]);
+    kmax[r][d0 >> 3] = (uint16_t)max4(k[0]);
+    kmax[r][d1 >> 3] = (uint16_t)max4(k[1]);
+    vmax[l][dp] = m;
+    __syncthreads();
+    if (tid < 128) {
+      const uint2 m4 = reinterpret_cast<const uint2*>(kmax[tid >> 2])[tid & 3];
+      const uint32_t mm = maxbits2(m4.x, m4.y);
+      const uint4 q = group_of<DT>((uint16_t)max(mm & 0xffff, mm >> 16));
+      kgroup[tid >> 2][tid & 3] = q;
+      reinterpret_cast<uint16_t*>(blk + kKScale)[((tid >> 2) & 7) * 16 + (tid >> 5) * 4 + (tid & 3)] = (uint16_t)(q.w >> 16);
+    } else {
+      const int d = tid - 128;
+      const uint32_t mm = maxbits2(maxbits2(vmax[0][d >> 1], vmax[1][d >> 1]), maxbits2(vmax[2][d >> 1], vmax[3][d >> 1]));
+      const uint4 q = group_of<DT>((uint16_t)(d & 1 ? mm >> 16 : mm & 0xffff));
+      vgroup[d] = q;
+      reinterpret_cast<uint16_t*>(blk + kVScale)[d] = (uint16_t)(q.w >> 16);
+    }
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 7; ++i) cut[i] *= 0x00010001u;
-    uint32_t* words = reinterpret_cast<uint32_t*>(blk);
-#pragma unroll
-    for (int l = 0; l < 4; ++l) {
+    for (int i = 0; i < 2; ++i) {
+      const int d = i ? d1 : d0;
+      const uint4 q = kgroup[r][d >> 5];
+      const uint32_t cut[7] = {__byte_perm(q.x, 0, 0x1010), __byte_perm(q.x, 0, 0x3232), __byte_perm(q.y, 0, 0x1010),
+                               __byte_perm(q.y, 0, 0x3232), __byte_perm(q.z, 0, 0x1010), __byte_perm(q.z, 0, 0x3232),
+                               __byte_perm(q.w, 0, 0x1010)};
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&k[i]);
       uint32_t o = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t u = sym_codes2<DT, 4>(w[4 * l + i], cut);
-        o |= ((u & 15u) | ((u >> 12) & 0xf0u)) << (8 * i);
-      }
-      words[(r * 4 + l) * 4 + g] = o;
-    }
-    reinterpret_cast<uint16_t*>(blk + kKScale)[(r & 7) * 16 + (r >> 3) * 4 + g] = scale;
-  }
-  {  // values: two threads per pair of channels, each with the 16 tokens of two l
-    const int dp = tid & 63, th = tid >> 6;
-    uint32_t x[16];  // [n & 3][token within the four]
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int pos = first + 8 * a + 4 * th + e;
-        const uint16_t* row = pos >= len0 ? n.v + (int64_t)(cu0 + pos - len0) * n.v_st + h * n.v_sh
-                                          : c.dv + base + (int64_t)c.row_of(pos) * kD;
-        x[4 * a + e] = *reinterpret_cast<const uint32_t*>(row + 2 * dp);
+        const uint32_t code = sym_codes2<DT, 4>(w[e], cut);
+        o |= ((code & 15u) | ((code >> 12) & 0xf0u)) << (8 * e);
       }
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m = maxbits2(m, x[i]);
-    vmax[th][dp] = m;
-    __syncthreads();
-    m = maxbits2(m, vmax[th ^ 1][dp]);
-    const uint16_t s0 = scale_of<DT>(m & 0xffff), s1 = scale_of<DT>(m >> 16);
-    uint32_t cut[7], cut1[7];
-    cuts_of<DT>(s0, cut);
-    cuts_of<DT>(s1, cut1);
-#pragma unroll
-    for (int i = 0; i < 7; ++i) cut[i] |= cut1[i] << 16;
-    const int d = 2 * dp, i8 = d >> 4, p = (d >> 2) & 3, mm = (d >> 1) & 1;
-#pragma unroll
-    for (int ll = 0; ll < 2; ++ll) {
-      uint32_t o0 = 0, o1 = 0;
-#pragma unroll
-      for (int nn = 0; nn < 8; ++nn) {
-        const uint32_t u = sym_codes2<DT, 4>(x[4 * (nn & 3) + 2 * ll + (nn >> 2)], cut);
-        o0 |= (u & 15u) << (4 * nn);
-        o1 |= ((u >> 16) & 15u) << (4 * nn);
-      }
-      uint2* words = reinterpret_cast<uint2*>(blk + kVCodes);
-      words[((p * 8 + i8) * 4 + 2 * th + ll) * 2 + mm] = make_uint2(o0, o1);
+      reinterpret_cast<uint32_t*>(blk)[(r * 4 + ((d >> 3) & 3)) * 4 + (d >> 5)] = o;
     }
-    if (th == 0) reinterpret_cast<uint32_t*>(blk + kVScale)[dp] = pack2(s0, s1);
+    const uint4 q0 = vgroup[2 * dp], q1 = vgroup[2 * dp + 1];
+    const uint32_t cut[7] = {__byte_perm(q0.x, q1.x, 0x5410), __byte_perm(q0.x, q1.x, 0x7632), __byte_perm(q0.y, q1.y, 0x5410),
+                             __byte_perm(q0.y, q1.y, 0x7632), __byte_perm(q0.z, q1.z, 0x5410), __byte_perm(q0.z, q1.z, 0x7632),
+                             __byte_perm(q0.w, q1.w, 0x5410)};
+    uint32_t o0 = 0, o1 = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t code = sym_codes2<DT, 4>(vv[i], cut);
+      o0 |= (code & 15u) << (4 * i);
+      o1 |= ((code >> 16) & 15u) << (4 * i);
+    }
+    const int d = 2 * dp;
+    reinterpret_cast<uint2*>(blk + kVCodes)[((((d >> 2) & 3) * 8 + (d >> 4)) * 4 + l) * 2 + ((d >> 1) & 1)] = make_uint2(o0, o1);
   }
 }
 
+constexpr int kPackHeads = 2;  // heads of a pack block
+
 template <int DT>
-__device__ __forceinline__ void pack_block(const PagedDev& c, const NewDev& n, int item, int h) {
+__device__ __forceinline__ void pack_block(const PagedDev& c, const NewDev& n, int item, int part) {
   __shared__ int sb;
   int b = item, t, len0, cu0;
   if (n.cu) {
@@ -260,117 +285,191 @@ __device__ __forceinline__ void pack_block(const PagedDev& c, const NewDev& n, i
     t = c.n_packed(len0) >> 5;
     if (len0 < 0 || 32 * t >= c.n_packed(len0 + 1)) return;
   }
-  pack_tile<DT>(c, n, b, h, t, len0, cu0);
+  pack_tile<DT>(c, n, b, part * kPackHeads, min(c.Hkv, (part + 1) * kPackHeads), t, len0, cu0);
 }
 
-// rotate and store the q, k and v rows of one token
+// Rotate and store the q, k and v rows of one token.  A thread is one unit of
+// the token, keeps its angles over the heads h0, h0 + step, .. and has the
+// loads of kBatch of them under way at a time.
+constexpr int kBatch = 4;
 template <int DT>
-__device__ __forceinline__ void dense_token(const PagedDev& c, const NewDev& n, int tok, int b, int pos, int after) {
+__device__ __forceinline__ void dense_token(const PagedDev& c, const NewDev& n, int tok, int b, int pos, int after, int h0,
+                                            int step) {
   const bool keep = pos < c.w_sink || pos >= c.w_sink + c.n_packed(after);
-  const int heads = n.Hq + 2 * c.Hkv;
-  for (int i = threadIdx.x; i < heads * 8; i += blockDim.x) {
-    const int row = i >> 3, u = i & 7;
-    int d0, d1;
-    unit_chunks(n, u, d0, d1);
-    if (row < n.Hq) {
-      const uint16_t* src = n.q + (int64_t)tok * n.q_st + row * n.q_sh;
-      uint4 x = *reinterpret_cast<const uint4*>(src + d0), y = *reinterpret_cast<const uint4*>(src + d1);
-      rotate_unit<DT>(n, u, d0, pos, x, y);
-      uint16_t* dst = n.q_out + (int64_t)tok * n.qo_st + row * n.qo_sh;
-      *reinterpret_cast<uint4*>(dst + d0) = x;
-      *reinterpret_cast<uint4*>(dst + d1) = y;
-      continue;
+  const int u = threadIdx.x & 7;
+  int d0, d1;
+  unit_chunks(n, u, d0, d1);
+  Angles g;
+  load_angles(n, u, d0, pos, g);
+  auto store = [&](uint16_t* p, const uint4& x, const uint4& y) {
+    *reinterpret_cast<uint4*>(p + d0) = x;
+    *reinterpret_cast<uint4*>(p + d1) = y;
+  };
+  const uint16_t* src = n.q + (int64_t)tok * n.q_st;
+  uint16_t* dst = n.q_out + (int64_t)tok * n.qo_st;
+#pragma unroll 1
+  for (int h = h0; h < n.Hq; h += kBatch * step) {
+    uint4 x[kBatch], y[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const uint16_t* p = src + min(h + i * step, n.Hq - 1) * n.q_sh;
+      x[i] = *reinterpret_cast<const uint4*>(p + d0);
+      y[i] = *reinterpret_cast<const uint4*>(p + d1);
     }
-    const bool is_k = row < n.Hq + c.Hkv;
-    const int h = row - n.Hq - (is_k ? 0 : c.Hkv);
-    if (!keep && !(is_k && n.k_out)) continue;
-    const uint16_t* src = is_k ? n.k + (int64_t)tok * n.k_st + h * n.k_sh : n.v + (int64_t)tok * n.v_st + h * n.v_sh;
-    uint4 x = *reinterpret_cast<const uint4*>(src + d0), y = *reinterpret_cast<const uint4*>(src + d1);
-    if (is_k) rotate_unit<DT>(n, u, d0, pos, x, y);
-    if (is_k && n.k_out) {
-      uint16_t* dst = n.k_out + (int64_t)tok * n.ko_st + h * n.ko_sh;
-      *reinterpret_cast<uint4*>(dst + d0) = x;
-      *reinterpret_cast<uint4*>(dst + d1) = y;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      rotate_unit<DT>(g, n.interleaved, x[i], y[i]);
+      if (h + i * step < n.Hq) store(dst + (h + i * step) * n.qo_sh, x[i], y[i]);
     }
-    const int64_t base = c.dense_base(b, h);
-    if (keep && base >= 0) {
-      uint16_t* dst = (is_k ? c.dk : c.dv) + base + (int64_t)c.row_of(pos) * kD;
-      *reinterpret_cast<uint4*>(dst + d0) = x;
-      *reinterpret_cast<uint4*>(dst + d1) = y;
+  }
+  if (!keep && !n.k_out) return;
+  const int64_t row = (int64_t)c.row_of(pos) * kD;
+  for (int h = h0; h < c.Hkv; h += step) {
+    const uint16_t* p = n.k + (int64_t)tok * n.k_st + h * n.k_sh;
+    uint4 x = *reinterpret_cast<const uint4*>(p + d0), y = *reinterpret_cast<const uint4*>(p + d1), v0, v1;
+    if (keep) {
+      p = n.v + (int64_t)tok * n.v_st + h * n.v_sh;
+      v0 = *reinterpret_cast<const uint4*>(p + d0);
+      v1 = *reinterpret_cast<const uint4*>(p + d1);
+    }
+    rotate_unit<DT>(g, n.interleaved, x, y);
+    if (n.k_out) store(n.k_out + (int64_t)tok * n.ko_st + h * n.ko_sh, x, y);
+    const int64_t base = keep ? c.dense_base(b, h) : -1;
+    if (base >= 0) {
+      store(c.dk + base + row, x, y);
+      store(c.dv + base + row, v0, v1);
     }
   }
 }
+
+constexpr int kTokens = 4;  // tokens of a dense block of prompts: one per quarter warp
 
 // role 0: both (one token per sequence); 1: pack; 2: dense
 template <int DT, int ROLE>
-__global__ void __launch_bounds__(128) append_kernel(PagedDev c, NewDev n, int n_pack) {
+__global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(PagedDev c, NewDev n, int n_pack, int split) {
   griddep_wait();
   griddep_launch_dependents();
-  const int blk = blockIdx.x;
+  const int blk = blockIdx.x, parts = (c.Hkv + kPackHeads - 1) / kPackHeads;
   if (ROLE == 1 || (ROLE == 0 && blk < n_pack)) {
-    pack_block<DT>(c, n, blk / c.Hkv, blk % c.Hkv);
+    pack_block<DT>(c, n, blk / parts, blk % parts);
     return;
   }
-  const int tok = ROLE == 0 ? blk - n_pack : blk;
-  if (ROLE == 0) {
-    const int len0 = c.lens[tok];
-    if (len0 >= 0) dense_token<DT>(c, n, tok, tok, len0, len0 + 1);
+  if (ROLE == 0) {  // `split` blocks share a token's heads
+    const int rows = kAppendThreads / 8, tok = (blk - n_pack) / split, part = (blk - n_pack) % split, len0 = c.lens[tok];
+    if (len0 >= 0) dense_token<DT>(c, n, tok, tok, len0, len0 + 1, (threadIdx.x >> 3) + part * rows, rows * split);
     return;
   }
   __shared__ int sb;
-  find_seq(n.cu, c.B, tok, &sb);
-  const int b = sb;
-  if (b < 0 || c.lens[b] < 0) return;
+  const int tok0 = blk * kTokens, tok = tok0 + ((threadIdx.x >> 3) & (kTokens - 1));
+  find_seq(n.cu, c.B, tok0, &sb);
+  int b = max(sb, 0);
+  while (b < c.B && tok >= n.cu[b + 1]) ++b;
+  if (b >= c.B || tok >= n.T) return;
   const int len0 = c.lens[b], cu0 = n.cu[b];
-  dense_token<DT>(c, n, tok, b, len0 + tok - cu0, len0 + min(n.cu[b + 1], n.T) - cu0);
+  if (len0 < 0 || tok < cu0) return;
+  dense_token<DT>(c, n, tok, b, len0 + tok - cu0, len0 + min(n.cu[b + 1], n.T) - cu0, threadIdx.x / (8 * kTokens),
+                  kAppendThreads / (8 * kTokens));
 }
 
-// read-back: one block per token
+// (u - 8) s of the codes in bits 0-3 and 16-19 of w: exact in the dtype before
+// the one rounding of the product, as the fp32 product of the definition
+template <int DT> __device__ __forceinline__ uint32_t value2(uint32_t w, uint32_t s2) {
+  constexpr uint32_t magic = DT == F16 ? 0x64006400u : 0x43004300u;  // 1024, 128: the code is the last digits
+  constexpr uint32_t bias = DT == F16 ? 0x64086408u : 0x43084308u;
+  const auto c = __hsub2(as_pair<DT>((w & 0x000f000fu) | magic), as_pair<DT>(bias));
+  return pair_bits<DT>(__hmul2(c, as_pair<DT>(s2)));
+}
+
+// Read-back: one block per head and tile of 32 positions.  Sink, packed part and
+// window begin and end at multiples of 32, so a tile is of one kind.
 template <int DT>
-__global__ void __launch_bounds__(128) read_kernel(PagedDev c, const int32_t* starts, const int32_t* cu, uint16_t* ko,
-                                                   uint16_t* vo) {
+__global__ void __launch_bounds__(128, 8)
+    read_kernel(PagedDev c, const int32_t* starts, const int32_t* cu, int n_tokens, uint16_t* ko, uint16_t* vo) {
   griddep_wait();
   griddep_launch_dependents();
   __shared__ int sb;
-  const int tok = blockIdx.x;
-  find_seq(cu, c.B, tok, &sb);
+  const int item = blockIdx.x / c.Hkv, h = blockIdx.x % c.Hkv, tid = threadIdx.x;
+  // items of sequence b start at cu[b] / 32 + 2 b: room for tiles cut at both ends
+  if (tid == 0) sb = -1;
+  __syncthreads();
+  for (int i = tid; i < c.B; i += 128)
+    if (cu[i] / 32 + 2 * i <= item && item < cu[i + 1] / 32 + 2 * i + 2) sb = i;
+  __syncthreads();
   const int b = sb;
   if (b < 0) return;
-  const int len = c.lens[b], pos = starts[b] + tok - cu[b], u = pos - c.w_sink;
-  const bool inside = pos >= 0 && pos < len, packed = u >= 0 && u < c.n_packed(len);
-  for (int i = threadIdx.x; i < c.Hkv * 32; i += blockDim.x) {
-    const int h = i >> 5, side = (i >> 4) & 1, d0 = 8 * (i & 15);
-    uint4 o;
-    uint16_t* e = reinterpret_cast<uint16_t*>(&o);
+  const int cu0 = cu[b], count = min(cu[b + 1], n_tokens) - cu0, start = starts[b], len = c.lens[b];
+  if (cu0 < 0 || count <= 0) return;
+  const int p0 = (start >= 0 ? start & ~31 : -((-start + 31) & ~31)) + 32 * (item - (cu0 / 32 + 2 * b));
+  if (p0 >= start + count) return;
+  // position p of the tile goes to row cu0 - start + p, if start <= p < start + count
+  const int64_t pitch = (int64_t)c.Hkv * kD, out0 = ((int64_t)cu0 - start + p0) * pitch;
+  const int lo = start - p0, hi = start + count - p0;
+  auto put = [&](uint16_t* o, int r, int d, uint4 v) {
+    if (r >= lo && r < hi) *reinterpret_cast<uint4*>(o + r * pitch + d) = v;
+  };
+  constexpr uint32_t nan2 = nan16<DT>() * 0x00010001u;
+  const uint4 nan4 = make_uint4(nan2, nan2, nan2, nan2);
+  const int u0 = p0 - c.w_sink;
+  const bool packed = u0 >= 0 && u0 < c.n_packed(len);
+  const int row = packed || p0 < 0 ? 0 : c.row_of(p0);
+  uint16_t* kr = ko + out0 + h * kD;
+  uint16_t* vr = vo + out0 + h * kD;
+  const uint8_t* blk = packed ? c.tile(b, h, u0 >> 5) : nullptr;
+  const int64_t base = packed ? -1 : c.dense_base(b, h);
+  if (p0 < 0 || p0 >= len || (packed ? blk == nullptr : base < 0)) {
 #pragma unroll
-    for (int x = 0; x < 8; ++x) e[x] = nan16<DT>();
-    if (inside && !packed) {
-      const int64_t base = c.dense_base(b, h);
-      if (base >= 0)
-        o = *reinterpret_cast<const uint4*>((side ? c.dv : c.dk) + base + (int64_t)c.row_of(pos) * kD + d0);
-    } else if (inside) {
-      const uint8_t* blk = c.tile(b, h, u >> 5);
-      const int r = u & 31;
-      if (blk != nullptr && side == 0) {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(blk)[(r * 4 + ((d0 >> 3) & 3)) * 4 + (d0 >> 5)];
-        const float s = to_f<DT>(reinterpret_cast<const uint16_t*>(blk + kKScale)[(r & 7) * 16 + (r >> 3) * 4 + (d0 >> 5)]);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) e[x] = from_f<DT>((float)((int)((w >> (4 * x)) & 15u) - 8) * s);
-      } else if (blk != nullptr) {
-        const int nib = (r >> 3) + 4 * (r & 1), l = (r >> 1) & 3, i8 = d0 >> 4, p = (d0 >> 2) & 3;
-        const uint4 s4 = *reinterpret_cast<const uint4*>(blk + kVScale + 2 * d0);
-        const uint16_t* s = reinterpret_cast<const uint16_t*>(&s4);
-#pragma unroll
-        for (int hp = 0; hp < 2; ++hp) {
-          const uint4 w4 = reinterpret_cast<const uint4*>(blk + kVCodes)[((p + hp) * 8 + i8) * 4 + l];
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(&w4);
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            e[4 * hp + x] = from_f<DT>((float)((int)((w[x] >> (4 * nib)) & 15u) - 8) * to_f<DT>(s[4 * hp + x]));
-        }
-      }
+    for (int i = 0; i < 4; ++i) {
+      put(kr, 8 * i + (tid >> 4), 8 * (tid & 15), nan4);
+      put(vr, 8 * i + (tid >> 4), 8 * (tid & 15), nan4);
     }
-    *reinterpret_cast<uint4*>((side ? vo : ko) + ((int64_t)tok * c.Hkv + h) * kD + d0) = o;
+  } else if (!packed) {
+    const int64_t at = base + (int64_t)row * kD;
+    uint4 k[4], v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (tid >> 4), d = 8 * (tid & 15);
+      const bool in = p0 + r < len && r >= lo && r < hi;
+      k[i] = in ? *reinterpret_cast<const uint4*>(c.dk + at + r * kD + d) : nan4;
+      v[i] = in ? *reinterpret_cast<const uint4*>(c.dv + at + r * kD + d) : nan4;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      put(kr, 8 * i + (tid >> 4), 8 * (tid & 15), k[i]);
+      put(vr, 8 * i + (tid >> 4), 8 * (tid & 15), v[i]);
+    }
+  } else {
+    // keys: token r, channels 32 g + 8 l ..; values: channels 4 q .., tokens 8 (n & 3) + 2 vl + (n >> 2)
+    const int r = tid >> 2, l = tid & 3, vl = tid >> 5, q = tid & 31;
+    const uint4 kw = reinterpret_cast<const uint4*>(blk)[tid];
+    const uint4 vw = reinterpret_cast<const uint4*>(blk + kVCodes)[((q & 3) * 8 + (q >> 2)) * 4 + vl];
+    const uint2 ks = reinterpret_cast<const uint2*>(blk + kKScale)[(r & 7) * 4 + (r >> 3)];
+    const uint2 vs = reinterpret_cast<const uint2*>(blk + kVScale)[q];
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&kw);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const uint32_t s2 = __byte_perm(g & 2 ? ks.y : ks.x, 0, g & 1 ? 0x3232 : 0x1010);
+      uint32_t e[4];  // channels (x, x + 4)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) e[x] = value2<DT>(w[g] >> (4 * x), s2);
+      put(kr, r, 32 * g + 8 * l,
+          make_uint4(__byte_perm(e[0], e[1], 0x5410), __byte_perm(e[2], e[3], 0x5410), __byte_perm(e[0], e[1], 0x7632),
+                     __byte_perm(e[2], e[3], 0x7632)));
+    }
+    w = reinterpret_cast<const uint32_t*>(&vw);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      uint32_t e[4];  // channel y of tokens 8 x + 2 vl and the one after it
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        e[y] = value2<DT>(w[y] >> (4 * x), __byte_perm(y & 2 ? vs.y : vs.x, 0, y & 1 ? 0x3232 : 0x1010));
+      const int t = 8 * x + 2 * vl;
+      if (t >= lo && t < hi)
+        *reinterpret_cast<uint2*>(vr + t * pitch + 4 * q) =
+            make_uint2(__byte_perm(e[0], e[1], 0x5410), __byte_perm(e[2], e[3], 0x5410));
+      if (t + 1 >= lo && t + 1 < hi)
+        *reinterpret_cast<uint2*>(vr + (t + 1) * pitch + 4 * q) =
+            make_uint2(__byte_perm(e[0], e[1], 0x7632), __byte_perm(e[2], e[3], 0x7632));
+    }
   }
 }
 
@@ -380,16 +479,24 @@ int cuda_rc(cudaError_t e, const char* what) {
   return e == cudaSuccess ? INNERQ_OK : set_last_error(INNERQ_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+// pack blocks of a call: an upper bound of the tiles it can complete, by heads
+int64_t pack_blocks(const PagedDev& c, const NewDev& n) {
+  const int64_t items = n.cu ? n.T / 32 + c.B : c.B;
+  return items * ((c.Hkv + kPackHeads - 1) / kPackHeads);
+}
+
 template <int DT>
 cudaError_t launch_append(const PagedDev& c, const NewDev& n, cudaStream_t s) {
+  const int n_pack = (int)pack_blocks(c, n);
+  const dim3 block(kAppendThreads);
   if (n.cu == nullptr) {
-    const int n_pack = c.B * c.Hkv;
-    return launch_pdl(append_kernel<DT, 0>, dim3(n_pack + n.T), dim3(128), 0, s, c, n, n_pack);
+    // few tokens: several blocks per token, so that a thread has one row
+    const int per = kAppendThreads / 8, split = n.T < 256 ? (std::max(n.Hq, c.Hkv) + per - 1) / per : 1;
+    return launch_pdl(append_kernel<DT, 0>, dim3(n_pack + n.T * split), block, 0, s, c, n, n_pack, split);
   }
-  const int64_t items = (int64_t)(n.T / 32 + c.B) * c.Hkv;
-  cudaError_t e = launch_pdl(append_kernel<DT, 1>, dim3((unsigned)items), dim3(128), 0, s, c, n, (int)items);
+  cudaError_t e = launch_pdl(append_kernel<DT, 1>, dim3(n_pack), block, 0, s, c, n, n_pack, 1);
   if (e != cudaSuccess) return e;
-  return launch_pdl(append_kernel<DT, 2>, dim3(n.T), dim3(128), 0, s, c, n, 0);
+  return launch_pdl(append_kernel<DT, 2>, dim3((n.T + kTokens - 1) / kTokens), block, 0, s, c, n, 0, 1);
 }
 
 }  // namespace
@@ -447,8 +554,6 @@ extern "C" int innerq_paged_append(const innerq_paged* cache, const innerq_paged
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->q_out) || !aligned16(a->k_out) ||
       (a->rot_dim && (!aligned16(a->cos) || !aligned16(a->sin) || a->cs_stride % 4)))
     return set_last_error(INNERQ_ERR_ARG, "rows must be 16-byte aligned");
-  const int64_t items = (int64_t)(a->T / 32 + c.B) * c.Hkv;
-  if (items + a->T > 0x7fffffff) return set_last_error(INNERQ_ERR_ARG, "too many tokens for one launch");
   NewDev n;
   n.q = (const uint16_t*)a->q; n.k = (const uint16_t*)a->k; n.v = (const uint16_t*)a->v;
   n.q_st = a->q_st; n.q_sh = a->q_sh; n.k_st = a->k_st; n.k_sh = a->k_sh; n.v_st = a->v_st; n.v_sh = a->v_sh;
@@ -457,6 +562,8 @@ extern "C" int innerq_paged_append(const innerq_paged* cache, const innerq_paged
   n.q_out = (uint16_t*)a->q_out; n.k_out = (uint16_t*)a->k_out;
   n.qo_st = a->qo_st; n.qo_sh = a->qo_sh; n.ko_st = a->ko_st; n.ko_sh = a->ko_sh;
   n.Hq = a->Hq; n.T = a->T; n.rot = a->rot_dim; n.interleaved = a->interleaved; n.max_pos = a->max_pos;
+  if (pack_blocks(c, n) + (int64_t)a->T * 64 > 0x7fffffff)
+    return set_last_error(INNERQ_ERR_ARG, "too many tokens for one launch");
   const cudaStream_t s = (cudaStream_t)stream;
   return cuda_rc(cache->dtype == INNERQ_DT_BF16 ? launch_append<BF16>(c, n, s) : launch_append<F16>(c, n, s), "paged_append");
 }
@@ -472,8 +579,11 @@ extern "C" int innerq_paged_read(const innerq_paged* cache, const int32_t* start
   const cudaStream_t s = (cudaStream_t)stream;
   uint16_t* ko = (uint16_t*)k_out;
   uint16_t* vo = (uint16_t*)v_out;
+  const int64_t blocks = ((int64_t)n_tokens / 32 + 2ll * c.B) * c.Hkv;
+  if (blocks > 0x7fffffff) return set_last_error(INNERQ_ERR_ARG, "too many tokens for one launch");
+  const dim3 grid((unsigned)blocks), block(128);
   return cuda_rc(cache->dtype == INNERQ_DT_BF16
-                     ? launch_pdl(read_kernel<BF16>, dim3(n_tokens), dim3(128), 0, s, c, starts, cu_seqlens, ko, vo)
-                     : launch_pdl(read_kernel<F16>, dim3(n_tokens), dim3(128), 0, s, c, starts, cu_seqlens, ko, vo),
+                     ? launch_pdl(read_kernel<BF16>, grid, block, 0, s, c, starts, cu_seqlens, n_tokens, ko, vo)
+                     : launch_pdl(read_kernel<F16>, grid, block, 0, s, c, starts, cu_seqlens, n_tokens, ko, vo),
                  "paged_read");
 }
