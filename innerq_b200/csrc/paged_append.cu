@@ -6,12 +6,11 @@
 // fp32 (no FMA) and the result once to the dtype, so the stored keys do not
 // depend on how a compiler contracts the expression.
 //
-// A call does two things: "dense" rotates q (and k) and writes the sink's and
-// the window's tokens; "pack" quantizes the tiles that leave the window, whose
-// tokens are new or still in the ring.  Ring rows that pack reads are
-// overwritten by dense only when a call brings more than one token, so one
-// token per sequence takes a single launch with both kinds of blocks and
-// prompts take two launches, pack first.
+// A call rotates q (and k where it is asked for), quantizes the tiles that
+// leave the window, whose tokens are new or still in the ring, and writes the
+// sink's and the window's new rows.  A row that packing reads from the ring is
+// overwritten only when a call brings more than one token, so a decode step
+// is a single launch, and prompts take a second one for the rows.
 #include <algorithm>
 
 #include "innerq_internal.h"
@@ -92,13 +91,14 @@ template <int DT> __device__ __forceinline__ float hi_f(uint32_t w) {
 // the angles of a unit at one position
 struct Angles {
   float c[8], s[8];
-  bool rotated, known;
+  enum { kNone, kHalves, kPairs, kNaN } mode;
 };
 
 __device__ __forceinline__ void load_angles(const NewDev& n, int u, int d0, int pos, Angles& g) {
-  g.rotated = d0 < n.rot;
-  g.known = (unsigned)pos < (unsigned)n.max_pos;
-  if (!g.rotated || !g.known) return;
+  g.mode = d0 >= n.rot ? Angles::kNone
+           : (unsigned)pos >= (unsigned)n.max_pos ? Angles::kNaN  // beyond the table: NaN, never a wrong angle
+           : n.interleaved ? Angles::kPairs : Angles::kHalves;
+  if (g.mode == Angles::kNone || g.mode == Angles::kNaN) return;
   const float4* c = reinterpret_cast<const float4*>(n.cos + pos * n.cs_stride + 8 * u);
   const float4* s = reinterpret_cast<const float4*>(n.sin + pos * n.cs_stride + 8 * u);
 #pragma unroll
@@ -111,27 +111,30 @@ __device__ __forceinline__ void load_angles(const NewDev& n, int u, int d0, int 
 
 // rotate the two chunks of a unit
 template <int DT>
-__device__ __forceinline__ void rotate_unit(const Angles& g, int interleaved, uint4& x, uint4& y) {
-  if (!g.rotated) return;
+__device__ __forceinline__ void rotate_unit(const Angles& g, uint4& x, uint4& y) {
   uint32_t* xa = reinterpret_cast<uint32_t*>(&x);
   uint32_t* ya = reinterpret_cast<uint32_t*>(&y);
-  if (!g.known) {  // beyond the table: NaN, never a wrong angle
+  if (g.mode == Angles::kHalves) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) xa[i] = ya[i] = nan16<DT>() * 0x00010001u;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float a0 = lo_f<DT>(xa[i]), a1 = hi_f<DT>(xa[i]), b0 = lo_f<DT>(ya[i]), b1 = hi_f<DT>(ya[i]);
-    if (interleaved) {
-      rotate(a0, a1, g.c[i], g.s[i]);
-      rotate(b0, b1, g.c[4 + i], g.s[4 + i]);
-    } else {
+    for (int i = 0; i < 4; ++i) {
+      float a0 = lo_f<DT>(xa[i]), a1 = hi_f<DT>(xa[i]), b0 = lo_f<DT>(ya[i]), b1 = hi_f<DT>(ya[i]);
       rotate(a0, b0, g.c[2 * i], g.s[2 * i]);
       rotate(a1, b1, g.c[2 * i + 1], g.s[2 * i + 1]);
+      xa[i] = round2<DT>(a0, a1);
+      ya[i] = round2<DT>(b0, b1);
     }
-    xa[i] = round2<DT>(a0, a1);
-    ya[i] = round2<DT>(b0, b1);
+  } else if (g.mode == Angles::kPairs) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a0 = lo_f<DT>(xa[i]), a1 = hi_f<DT>(xa[i]), b0 = lo_f<DT>(ya[i]), b1 = hi_f<DT>(ya[i]);
+      rotate(a0, a1, g.c[i], g.s[i]);
+      rotate(b0, b1, g.c[4 + i], g.s[4 + i]);
+      xa[i] = round2<DT>(a0, a1);
+      ya[i] = round2<DT>(b0, b1);
+    }
+  } else if (g.mode == Angles::kNaN) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xa[i] = ya[i] = nan16<DT>() * 0x00010001u;
   }
 }
 
@@ -184,29 +187,42 @@ __device__ void pack_tile(const PagedDev& c, const NewDev& n, int b, int h0, int
   const int first = c.w_sink + 32 * t, tid = threadIdx.x;
   const int r = tid >> 3, u = tid & 7, pos = first + r;  // keys
   const int dp = tid & 63, l = tid >> 6;                 // values
-  if (c.tile(b, h0, t) == nullptr || c.dense_base(b, h0) < 0) return;
+  uint8_t* blk = c.tile(b, h0, t);
+  int64_t base = c.dense_base(b, h0);
+  if (blk == nullptr || base < 0) return;
   int d0, d1;
   unit_chunks(n, u, d0, d1);
-  const bool fresh = pos >= len0;
+  const bool fresh = pos >= len0, all_fresh = first >= len0;
   Angles g;
-  g.rotated = false;
+  g.mode = Angles::kNone;
   if (fresh) load_angles(n, u, d0, pos, g);
+  const int64_t tok = (int64_t)cu0 + first - len0;
+  const uint16_t* row = fresh ? n.k + (tok + r) * n.k_st + h0 * n.k_sh : c.dk + base + (int64_t)c.row_of(pos) * kD;
+  const int64_t row_step = fresh ? n.k_sh : (int64_t)c.dense_rows() * kD;
+  const uint16_t* vrow = n.v + (tok + 2 * l) * n.v_st + h0 * n.v_sh + 2 * dp;
 #pragma unroll 1
   for (int h = h0; h < h1; ++h) {
-    uint8_t* blk = c.tile(b, h, t);
-    const int64_t base = c.dense_base(b, h);
-    const uint16_t* row = fresh ? n.k + (int64_t)(cu0 + pos - len0) * n.k_st + h * n.k_sh
-                                : c.dk + base + (int64_t)c.row_of(pos) * kD;
     uint4 k[2] = {*reinterpret_cast<const uint4*>(row + d0), *reinterpret_cast<const uint4*>(row + d1)};
-    uint32_t vv[8], m = 0;
+    uint32_t vv[8], m = 0;  // nibble i: token 8 (i & 3) + 2 l + (i >> 2)
+    if (all_fresh) {
+      const uint16_t* p = vrow;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {  // nibble i: token 8 (i & 3) + 2 l + (i >> 2)
-      const int p = first + 8 * (i & 3) + 2 * l + (i >> 2);
-      const uint16_t* vr = p >= len0 ? n.v + (int64_t)(cu0 + p - len0) * n.v_st + h * n.v_sh
-                                     : c.dv + base + (int64_t)c.row_of(p) * kD;
-      vv[i] = *reinterpret_cast<const uint32_t*>(vr + 2 * dp);
+      for (int i = 0; i < 4; ++i, p += 8 * n.v_st) {
+        vv[i] = *reinterpret_cast<const uint32_t*>(p);
+        vv[i + 4] = *reinterpret_cast<const uint32_t*>(p + n.v_st);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int o = 8 * (i & 3) + 2 * l + (i >> 2);
+        const uint16_t* p = first + o >= len0 ? n.v + (tok + o) * n.v_st + h * n.v_sh : c.dv + base + (int64_t)c.row_of(first + o) * kD;
+        vv[i] = *reinterpret_cast<const uint32_t*>(p + 2 * dp);
+      }
     }
-    rotate_unit<DT>(g, n.interleaved, k[0], k[1]);
+    row += row_step;
+    vrow += n.v_sh;
+    base += (int64_t)c.dense_rows() * kD;
+    rotate_unit<DT>(g, k[0], k[1]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = maxbits2(m, vv[i]);
     kmax[r][d0 >> 3] = (uint16_t)max4(k[0]);
@@ -256,6 +272,7 @@ __device__ void pack_tile(const PagedDev& c, const NewDev& n, int b, int h0, int
     }
     const int d = 2 * dp;
     reinterpret_cast<uint2*>(blk + kVCodes)[((((d >> 2) & 3) * 8 + (d >> 4)) * 4 + l) * 2 + ((d >> 1) & 1)] = make_uint2(o0, o1);
+    blk += (int64_t)c.page_tiles * kBlockBytes;  // the same tile of the next head
   }
 }
 
@@ -288,87 +305,126 @@ __device__ __forceinline__ void pack_block(const PagedDev& c, const NewDev& n, i
   pack_tile<DT>(c, n, b, part * kPackHeads, min(c.Hkv, (part + 1) * kPackHeads), t, len0, cu0);
 }
 
-// Rotate and store the q, k and v rows of one token.  A thread is one unit of
-// the token, keeps its angles over the heads h0, h0 + step, .. and has the
-// loads of kBatch of them under way at a time.
-constexpr int kBatch = 4;
+// Rotate the rows of heads h0, h0 + step, .. of one token.  A thread is one
+// unit of the token, keeps its angles over the heads and has the loads of
+// N heads under way at a time.
+template <int DT, int N>
+__device__ __forceinline__ void rotate_batch(const Angles& g, int d0, int d1, const uint16_t* src, int64_t src_step, uint16_t* dst,
+                                             int64_t dst_step) {
+  uint4 x[N], y[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] = *reinterpret_cast<const uint4*>(src + i * src_step + d0);
+    y[i] = *reinterpret_cast<const uint4*>(src + i * src_step + d1);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    rotate_unit<DT>(g, x[i], y[i]);
+    *reinterpret_cast<uint4*>(dst + i * dst_step + d0) = x[i];
+    *reinterpret_cast<uint4*>(dst + i * dst_step + d1) = y[i];
+  }
+}
 template <int DT>
-__device__ __forceinline__ void dense_token(const PagedDev& c, const NewDev& n, int tok, int b, int pos, int after, int h0,
-                                            int step) {
-  const bool keep = pos < c.w_sink || pos >= c.w_sink + c.n_packed(after);
+__device__ __forceinline__ void rotate_rows(const Angles& g, int d0, int d1, const uint16_t* src, int64_t src_sh, uint16_t* dst,
+                                            int64_t dst_sh, int heads, int h0, int step) {
+  constexpr int kBatch = 4;
+  int left = heads > h0 ? (heads - h0 + step - 1) / step : 0;
+  const int64_t ss = step * src_sh, ds = step * dst_sh;
+  src += h0 * src_sh;
+  dst += h0 * dst_sh;
+#pragma unroll 1
+  for (; left >= kBatch; left -= kBatch, src += kBatch * ss, dst += kBatch * ds) rotate_batch<DT, kBatch>(g, d0, d1, src, ss, dst, ds);
+#pragma unroll 1
+  for (; left > 0; --left, src += ss, dst += ds) rotate_batch<DT, 1>(g, d0, d1, src, ss, dst, ds);
+}
+
+// the rotated q, and k where it is asked for, of one token
+template <int DT>
+__device__ __forceinline__ void rotate_token(const NewDev& n, int Hkv, int tok, int pos, int h0, int step) {
   const int u = threadIdx.x & 7;
   int d0, d1;
   unit_chunks(n, u, d0, d1);
   Angles g;
   load_angles(n, u, d0, pos, g);
-  auto store = [&](uint16_t* p, const uint4& x, const uint4& y) {
-    *reinterpret_cast<uint4*>(p + d0) = x;
-    *reinterpret_cast<uint4*>(p + d1) = y;
-  };
-  const uint16_t* src = n.q + (int64_t)tok * n.q_st;
-  uint16_t* dst = n.q_out + (int64_t)tok * n.qo_st;
-#pragma unroll 1
-  for (int h = h0; h < n.Hq; h += kBatch * step) {
-    uint4 x[kBatch], y[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const uint16_t* p = src + min(h + i * step, n.Hq - 1) * n.q_sh;
-      x[i] = *reinterpret_cast<const uint4*>(p + d0);
-      y[i] = *reinterpret_cast<const uint4*>(p + d1);
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      rotate_unit<DT>(g, n.interleaved, x[i], y[i]);
-      if (h + i * step < n.Hq) store(dst + (h + i * step) * n.qo_sh, x[i], y[i]);
-    }
-  }
-  if (!keep && !n.k_out) return;
-  const int64_t row = (int64_t)c.row_of(pos) * kD;
+  rotate_rows<DT>(g, d0, d1, n.q + (int64_t)tok * n.q_st, n.q_sh, n.q_out + (int64_t)tok * n.qo_st, n.qo_sh, n.Hq, h0, step);
+  if (n.k_out)
+    rotate_rows<DT>(g, d0, d1, n.k + (int64_t)tok * n.k_st, n.k_sh, n.k_out + (int64_t)tok * n.ko_st, n.ko_sh, Hkv, h0, step);
+}
+
+// the row that a token of the sink or the window gets in its slot
+template <int DT>
+__device__ __forceinline__ void keep_token(const PagedDev& c, const NewDev& n, int tok, int b, int pos, int row, int h0, int step) {
+  const int u = threadIdx.x & 7;
+  int d0, d1;
+  unit_chunks(n, u, d0, d1);
+  Angles g;
+  load_angles(n, u, d0, pos, g);
   for (int h = h0; h < c.Hkv; h += step) {
     const uint16_t* p = n.k + (int64_t)tok * n.k_st + h * n.k_sh;
-    uint4 x = *reinterpret_cast<const uint4*>(p + d0), y = *reinterpret_cast<const uint4*>(p + d1), v0, v1;
-    if (keep) {
-      p = n.v + (int64_t)tok * n.v_st + h * n.v_sh;
-      v0 = *reinterpret_cast<const uint4*>(p + d0);
-      v1 = *reinterpret_cast<const uint4*>(p + d1);
-    }
-    rotate_unit<DT>(g, n.interleaved, x, y);
-    if (n.k_out) store(n.k_out + (int64_t)tok * n.ko_st + h * n.ko_sh, x, y);
-    const int64_t base = keep ? c.dense_base(b, h) : -1;
-    if (base >= 0) {
-      store(c.dk + base + row, x, y);
-      store(c.dv + base + row, v0, v1);
-    }
+    const uint16_t* r = n.v + (int64_t)tok * n.v_st + h * n.v_sh;
+    uint4 x = *reinterpret_cast<const uint4*>(p + d0), y = *reinterpret_cast<const uint4*>(p + d1);
+    const uint4 v0 = *reinterpret_cast<const uint4*>(r + d0), v1 = *reinterpret_cast<const uint4*>(r + d1);
+    rotate_unit<DT>(g, x, y);
+    const int64_t at = c.dense_base(b, h);
+    if (at < 0) return;
+    uint16_t* k = c.dk + at + (int64_t)row * kD;
+    uint16_t* v = c.dv + at + (int64_t)row * kD;
+    *reinterpret_cast<uint4*>(k + d0) = x;
+    *reinterpret_cast<uint4*>(k + d1) = y;
+    *reinterpret_cast<uint4*>(v + d0) = v0;
+    *reinterpret_cast<uint4*>(v + d1) = v1;
   }
 }
 
-constexpr int kTokens = 4;  // tokens of a dense block of prompts: one per quarter warp
+constexpr int kTokens = 4;                                // tokens of a block of prompts: one per quarter warp
+constexpr int kTokenHeads = kAppendThreads / 8 / kTokens;  // heads that its threads take at once
 
-// role 0: both (one token per sequence); 1: pack; 2: dense
+// role 0: a decode step, one token per sequence; 1: prompts, rotation and
+// packing; 2: prompts, the sink's and the window's rows (after the packing,
+// which may read what they overwrite)
 template <int DT, int ROLE>
 __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(PagedDev c, NewDev n, int n_pack, int split) {
   griddep_wait();
   griddep_launch_dependents();
   const int blk = blockIdx.x, parts = (c.Hkv + kPackHeads - 1) / kPackHeads;
-  if (ROLE == 1 || (ROLE == 0 && blk < n_pack)) {
-    pack_block<DT>(c, n, blk / parts, blk % parts);
+  if (ROLE == 2) {
+    const int groups = (c.dense_rows() + kTokens - 1) / kTokens, b = blk / groups;
+    const int row = blk % groups * kTokens + ((threadIdx.x >> 3) & (kTokens - 1));
+    const int len0 = c.lens[b], cu0 = n.cu[b], after = len0 + min(n.cu[b + 1], n.T) - cu0;
+    if (len0 < 0 || cu0 < 0 || row >= c.dense_rows()) return;
+    // the position whose row this is: of the window's the one at or after its first
+    const int np = c.n_packed(after), j = row - c.w_sink;
+    int place = (j - np) % c.ring();
+    if (place < 0) place += c.ring();
+    const int pos = j < 0 ? row : c.w_sink + np + place;
+    if (pos < len0 || pos >= after) return;
+    keep_token<DT>(c, n, cu0 + pos - len0, b, pos, row, threadIdx.x / (8 * kTokens), kTokenHeads);
     return;
   }
+  // packing (bound by instructions) and rotation (by memory) blocks alternate
+  const int packs = (int)((int64_t)blk * n_pack / gridDim.x);
+  if ((int)((int64_t)(blk + 1) * n_pack / gridDim.x) > packs) {
+    pack_block<DT>(c, n, packs / parts, packs % parts);
+    return;
+  }
+  const int rest = blk - packs;
   if (ROLE == 0) {  // `split` blocks share a token's heads
-    const int rows = kAppendThreads / 8, tok = (blk - n_pack) / split, part = (blk - n_pack) % split, len0 = c.lens[tok];
-    if (len0 >= 0) dense_token<DT>(c, n, tok, tok, len0, len0 + 1, (threadIdx.x >> 3) + part * rows, rows * split);
+    const int rows = kAppendThreads / 8, tok = rest / split, len0 = c.lens[tok];
+    if (len0 < 0) return;
+    const int h0 = (threadIdx.x >> 3) + rest % split * rows;
+    rotate_token<DT>(n, c.Hkv, tok, len0, h0, rows * split);
+    keep_token<DT>(c, n, tok, tok, len0, c.row_of(len0), h0, rows * split);
     return;
   }
   __shared__ int sb;
-  const int tok0 = blk * kTokens, tok = tok0 + ((threadIdx.x >> 3) & (kTokens - 1));
+  const int tok0 = rest * kTokens, tok = tok0 + ((threadIdx.x >> 3) & (kTokens - 1));
   find_seq(n.cu, c.B, tok0, &sb);
   int b = max(sb, 0);
   while (b < c.B && tok >= n.cu[b + 1]) ++b;
   if (b >= c.B || tok >= n.T) return;
   const int len0 = c.lens[b], cu0 = n.cu[b];
   if (len0 < 0 || tok < cu0) return;
-  dense_token<DT>(c, n, tok, b, len0 + tok - cu0, len0 + min(n.cu[b + 1], n.T) - cu0, threadIdx.x / (8 * kTokens),
-                  kAppendThreads / (8 * kTokens));
+  rotate_token<DT>(n, c.Hkv, tok, len0 + tok - cu0, threadIdx.x / (8 * kTokens), kTokenHeads);
 }
 
 // (u - 8) s of the codes in bits 0-3 and 16-19 of w: exact in the dtype before
@@ -494,9 +550,10 @@ cudaError_t launch_append(const PagedDev& c, const NewDev& n, cudaStream_t s) {
     const int per = kAppendThreads / 8, split = n.T < 256 ? (std::max(n.Hq, c.Hkv) + per - 1) / per : 1;
     return launch_pdl(append_kernel<DT, 0>, dim3(n_pack + n.T * split), block, 0, s, c, n, n_pack, split);
   }
-  cudaError_t e = launch_pdl(append_kernel<DT, 1>, dim3(n_pack), block, 0, s, c, n, n_pack, 1);
+  const int n_rotate = (n.T + kTokens - 1) / kTokens, rows = c.w_sink + c.w_recent + 32;
+  cudaError_t e = launch_pdl(append_kernel<DT, 1>, dim3(n_pack + n_rotate), block, 0, s, c, n, n_pack, 1);
   if (e != cudaSuccess) return e;
-  return launch_pdl(append_kernel<DT, 2>, dim3((n.T + kTokens - 1) / kTokens), block, 0, s, c, n, 0, 1);
+  return launch_pdl(append_kernel<DT, 2>, dim3(c.B * ((rows + kTokens - 1) / kTokens)), block, 0, s, c, n, 0, 1);
 }
 
 }  // namespace
@@ -562,7 +619,7 @@ extern "C" int innerq_paged_append(const innerq_paged* cache, const innerq_paged
   n.q_out = (uint16_t*)a->q_out; n.k_out = (uint16_t*)a->k_out;
   n.qo_st = a->qo_st; n.qo_sh = a->qo_sh; n.ko_st = a->ko_st; n.ko_sh = a->ko_sh;
   n.Hq = a->Hq; n.T = a->T; n.rot = a->rot_dim; n.interleaved = a->interleaved; n.max_pos = a->max_pos;
-  if (pack_blocks(c, n) + (int64_t)a->T * 64 > 0x7fffffff)
+  if (pack_blocks(c, n) + (int64_t)a->T * 64 > 0x7fffffff || (int64_t)c.B * 4096 > 0x7fffffff)
     return set_last_error(INNERQ_ERR_ARG, "too many tokens for one launch");
   const cudaStream_t s = (cudaStream_t)stream;
   return cuda_rc(cache->dtype == INNERQ_DT_BF16 ? launch_append<BF16>(c, n, s) : launch_append<F16>(c, n, s), "paged_append");
