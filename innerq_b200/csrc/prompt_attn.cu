@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const __grid_constant__ CUtensorMap mv, PromptDev a) {
   extern __shared__ __align__(1024) uint8_t raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;  // warp: uniform, and known to be
   griddep_wait();
   griddep_launch_dependents();
 
@@ -129,12 +129,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int keys = first < w.nq ? max(0, w.limit(last, a.causal)) : 0;
     w.n[i] = (keys + kRows - 1) / kRows;
   }
-  const int n = max(w.n[0], w.n[1]);
-  // whether some row of the CTA must not see all of key tile j
-  auto masked = [&](int j) {
-    const int end = kRows * (j + 1);
-    return (j < w.n[0] && end > w.limit(w.q0, a.causal)) || (j < w.n[1] && end > w.limit(w.q0 + kRows, a.causal));
-  };
+  const int n = __shfl_sync(~0u, max(w.n[0], w.n[1]), 0), n0 = __shfl_sync(~0u, w.n[0], 0), n1 = __shfl_sync(~0u, w.n[1], 0);
+  // from this key tile on, some row of the CTA must not see all of a tile
+  const int cut = __shfl_sync(~0u, max(0, w.limit(w.q0 + (w.n[0] > 0 ? 0 : kRows), a.causal)) / kRows, 0);
 
   if (tid == 0) {
     mbar_init(&sm.q_full, 1);
@@ -180,70 +177,77 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = max(0, sent - kRing); i < sent; ++i)
           mbar_wait_bounded(&sm.full[i % kRing], (i / kRing) & 1, kWait / 16);
       }
-    } else if (warp == 8 && lane == 0 && n > 0) {
+    } else if (warp == 8 && n > 0) {
       // -------------------------------------------------------------- MMAs
-      constexpr uint32_t id_s = mma_idesc(kRows, kRows, DT, 0), id_o = mma_idesc(kRows, 128, DT, 1);
-      const uint32_t q_addr = smem_u32(sm.q[0]), ring_addr = smem_u32(sm.ring[0]);
+      constexpr uint32_t id_s = mma_idesc(kRows, kRows, DT, 0), id_o = mma_idesc(kRows, 128, DT, 1), hi = desc_hi(1024);
+      const uint32_t leader = elect_one();
+      const uint32_t tm = __shfl_sync(~0u, tmem, 0), q_lo = __shfl_sync(~0u, desc_lo(smem_u32(sm.q[0]), 16), 0),
+                     k_lo = __shfl_sync(~0u, desc_lo(smem_u32(sm.ring[0]), 16), 0),
+                     v_lo = __shfl_sync(~0u, desc_lo(smem_u32(sm.ring[0]), kHalfTile), 0);
       auto scores = [&](int i, int st) {
-        const uint64_t da = smem_desc(q_addr + i * kTileBytes, 16, 1024), db = smem_desc(ring_addr + st * kTileBytes, 16, 1024);
+        const uint32_t da = q_lo + i * (kTileBytes >> 4), db = k_lo + st * (kTileBytes >> 4);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint32_t step = (k & 3) * 2 + (k >> 2) * (kHalfTile >> 4);
-          mma_ss(tmem + i * 128, da + step, db + step, id_s, k > 0);
+          mma_ss<hi, hi>(leader, tm + i * 128, da + step, db + step, id_s, k > 0);
         }
+        mma_commit(leader, &sm.s_full[i]);
       };
-      auto values = [&](int i, int st, bool acc) {
-        const uint64_t db = smem_desc(ring_addr + st * kTileBytes, kHalfTile, 1024);
+      auto values = [&](int i, int st, uint32_t acc) {
+        const uint32_t db = v_lo + st * (kTileBytes >> 4);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          mma_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, db + k * (2048 >> 4), id_o, acc || k > 0);
-      };
-      // a slot is given back only if a later tile comes into it, so that no
-      // arrival is outstanding when the CTA ends
-      auto release = [&](int item) {
-        if (item + kRing < 2 * n) mma_commit(&sm.empty[item % kRing]);
+          mma_ts<hi>(leader, tm + 256 + i * 128, tm + i * 128 + 8 * k, db + k * (2048 >> 4), id_o, k > 0 ? 1u : acc);
       };
       bool ok = mbar_wait_bounded(&sm.q_full, 0, kWait) && mbar_wait_bounded(&sm.full[0], 0, kWait);
+      ok = __all_sync(~0u, ok);
+      // ring slots of V_j and K_(j+1), and the parities of their fillings.  A
+      // slot is given back only if a later tile comes into it, so that no
+      // arrival is outstanding when the CTA ends.
+      int vs = 1, ks = 2;
+      uint32_t vp = 0, kp = 0;
       if (ok) {
         tc_fence_after();
-        for (int i = 0; i < 2; ++i)
-          if (w.n[i] > 0) {
-            scores(i, 0);
-            mma_commit(&sm.s_full[i]);
-          }
-        release(0);
+        if (n0 > 0) scores(0, 0);
+        if (n1 > 0) scores(1, 0);
+        if (kRing < 2 * n) mma_commit(leader, &sm.empty[0]);
       }
+#pragma unroll 1
       for (int j = 0; ok && j < n; ++j) {
-        const int vi = 2 * j + 1, ki = 2 * j + 2, vs = vi % kRing, ks = ki % kRing;
-        ok = mbar_wait_bounded(&sm.full[vs], (vi / kRing) & 1, kWait);
-        if (ok && masked(j)) ok = mbar_wait_bounded(&sm.checked[vs], (vi / kRing) & 1, kWait);
-        for (int i = 0; ok && i < 2; ++i) {
-          if (j >= w.n[i]) continue;
-          ok = mbar_wait_bounded(&sm.p_ready[i], j & 1, kWait);
-          if (!ok) break;
-          tc_fence_after();
-          values(i, vs, j > 0);
-          if (j + 1 == w.n[i]) {
-            mma_commit(&sm.o_full[i]);
-          } else {
-            ok = mbar_wait_bounded(&sm.full[ks], (ki / kRing) & 1, kWait);
-            if (!ok) break;
-            tc_fence_after();
-            scores(i, ks);
-            mma_commit(&sm.s_full[i]);
+        ok = mbar_wait_bounded(&sm.full[vs], vp, kWait);
+        if (j >= cut) ok = ok && mbar_wait_bounded(&sm.checked[vs], vp, kWait);
+        if (!__all_sync(~0u, ok)) break;
+        const uint32_t acc = j > 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int ni = i ? n1 : n0;
+          if (j < ni) {
+            ok = ok && mbar_wait_bounded(&sm.p_ready[i], j & 1, kWait);
+            if (j + 1 < ni) ok = ok && mbar_wait_bounded(&sm.full[ks], kp, kWait);
+            ok = __all_sync(~0u, ok);
+            if (ok) {
+              tc_fence_after();
+              values(i, vs, acc);
+              if (j + 1 < ni)
+                scores(i, ks);
+              else
+                mma_commit(leader, &sm.o_full[i]);
+            }
           }
         }
-        if (ok) {
-          release(vi);
-          release(ki);
-        }
+        if (2 * j + 1 + kRing < 2 * n) mma_commit(leader, &sm.empty[vs]);
+        if (2 * j + 2 + kRing < 2 * n) mma_commit(leader, &sm.empty[ks]);
+        vs += 2;
+        ks += 2;
+        if (vs >= kRing) vs -= kRing, vp ^= 1;
+        if (ks >= kRing) ks -= kRing, kp ^= 1;
       }
     } else if (warp >= 10) {
       // ------------------------------------------- values that are not finite
       for (int it = 0; it < 2 * n; ++it) {
         const int st = it % kRing;
         if (!__all_sync(~0u, mbar_wait_bounded(&sm.full[st], (it / kRing) & 1, kWait))) break;
-        if ((it & 1) && masked(it >> 1)) {
+        if ((it & 1) && (it >> 1) >= cut) {
           uint4* p = reinterpret_cast<uint4*>(sm.ring[st]) + (warp - 10) * (kTileBytes / 32);
           bool found = false;
 #pragma unroll 4
@@ -379,8 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && *(volatile int*)&sm.dirty && qi < w.nq) {
         // values that were set to 0 and that this row does see
         const uint16_t* qr = a.q + (int64_t)(w.q_base + qi) * a.q_st + head * a.q_sh;
-        for (int j = 0; j < w.n[i]; ++j) {
-          if (!masked(j)) continue;
+        for (int j = cut; j < w.n[i]; ++j) {
           for (int key = kRows * j; key < min(kRows * (j + 1), lim); ++key) {
             const uint16_t* vr = a.v + (int64_t)(w.k_base + key) * a.v_st + kv_head * a.v_sh;
             float p = -1.f;

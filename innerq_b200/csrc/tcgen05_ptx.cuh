@@ -62,11 +62,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* u) {
 // Shared-memory operand in 128-byte-swizzled atoms of 8 rows x 128 bytes.
 // K-major (rows along M / N, K contiguous): sbo = bytes between 8-row groups.
 // MN-major (rows along K, M / N contiguous): lbo = bytes between 128-byte
-// column blocks, sbo = bytes between 8-row groups.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lbo >> 4) & 0x3fff) << 16 | (uint64_t)((sbo >> 4) & 0x3fff) << 32 |
-         1ull << 46 | 2ull << 61;
-}
+// column blocks, sbo = bytes between 8-row groups.  The descriptor's low word
+// holds address and lbo in units of 16 bytes (adding to it moves the operand),
+// the high word is a constant.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4 & 0x3fff) | (lbo >> 4) << 16; }
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t sbo) { return sbo >> 4 | 1u << 14 | 2u << 29; }
 // kind::f16 instruction: fp32 accumulator, A and B both f16 (0) or bf16 (1),
 // A K-major, B K-major or MN-major
 __host__ __device__ constexpr uint32_t mma_idesc(int M, int N, int dtype, int b_mn_major) {
@@ -74,25 +74,40 @@ __host__ __device__ constexpr uint32_t mma_idesc(int M, int N, int dtype, int b_
          (uint32_t)(M >> 4) << 24;
 }
 
-// D (tensor memory) = A B (+ D); issued by one thread
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// One lane of a converged warp.  The warp that issues MMAs stays converged and
+// its instructions carry this predicate: operands that are uniform over the
+// warp then live in uniform registers, where tcgen05 wants them.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r;
+}
+// D (tensor memory) = A B (+ D)
+template <uint32_t AHI, uint32_t BHI>
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      "{\n .reg .pred p, q;\n .reg .b64 a, b;\n setp.ne.u32 p, %5, 0;\n setp.ne.u32 q, %4, 0;\n"
+      " mov.b64 a, {%1, %6};\n mov.b64 b, {%2, %7};\n"
+      " @p tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "r"(leader), "n"(AHI), "n"(BHI)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+template <uint32_t BHI>
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      "{\n .reg .pred p, q;\n .reg .b64 b;\n setp.ne.u32 p, %5, 0;\n setp.ne.u32 q, %4, 0;\n"
+      " mov.b64 b, {%2, %6};\n"
+      " @p tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, q;\n}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(idesc), "r"(acc), "r"(leader), "n"(BHI)
       : "memory");
 }
-// the barrier gets one arrival when every MMA this thread issued is complete
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar))
-               : "memory");
+// the barrier gets one arrival when every MMA the leader issued is complete
+__device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %1, 0;\n"
+      " @p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(leader)
+      : "memory");
 }
 
 // ----------------------------------------------------------------- TMA ---
