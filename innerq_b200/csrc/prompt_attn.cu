@@ -23,6 +23,7 @@
 // Tensor memory: S0 | S1 | O0 | O1, 128 columns each.  In-order execution of
 // the MMAs makes "S_i(j + 1) is complete" mean that O_i is at rest too.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/innerq_b200.h"
 #include "common.cuh"
@@ -42,6 +43,7 @@ constexpr float kShift = 7.f;            // P carries 2^7
 constexpr float kSlack = 8.f;            // lag of the running maximum
 constexpr float kNoMax = -1e30f;
 constexpr uint32_t kWait = 1u << 14;
+constexpr int kPolyOf = 4;               // one pair of exponentials of this many goes to the FMA pipe
 
 struct PromptDev {
   const uint16_t* q;
@@ -69,6 +71,53 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+
+// two fp32 values at a time
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_split(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// the larger of three; NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^y of two finite values on the FMA pipe, which the special-function unit's
+// 2^x leaves idle: y = n + f with n the nearest integer, a polynomial of
+// degree 4 for 2^f on [-1/2, 1/2] (minimax of the relative error, 2.6e-6, from
+// the Remez exchange), and n added to the exponent.  Values below -125 count
+// as -125.
+__device__ __forceinline__ void exp2_poly(uint64_t y, float& a, float& b) {
+  float y0, y1;
+  f2_split(y, y0, y1);
+  y = f2(fmaxf(y0, -125.f), fmaxf(y1, -125.f));
+  const float big = 12582912.f;  // 1.5 2^23: a sum with it is rounded to an integer
+  const uint64_t t = add2(y, f2(big, big)), n = add2(t, f2(-big, -big));
+  const uint64_t f = fma2(n, f2(-1.f, -1.f), y);
+  uint64_t p = fma2(f, f2(0.009570102207362652f, 0.009570102207362652f), f2(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(p, f, f2(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1, p0, p1;
+  f2_split(t, t0, t1);
+  f2_split(p, p0, p1);
+  a = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  b = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
 // two probabilities as one word of the type
@@ -300,19 +349,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 128; ++c) s[c] = -s[c];
       }
       const int seen = lim - kRows * j;
-      if (__any_sync(~0u, seen < kRows)) {
+      const bool whole = __all_sync(~0u, seen >= kRows);
+      if (!whole) {
 #pragma unroll
         for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
       }
-      float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+      float t4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 0; c < 128; c += 8) {
-        t0 = fmaxf(fmaxf(s[c], s[c + 1]), t0);
-        t1 = fmaxf(fmaxf(s[c + 2], s[c + 3]), t1);
-        t2 = fmaxf(fmaxf(s[c + 4], s[c + 5]), t2);
-        t3 = fmaxf(fmaxf(s[c + 6], s[c + 7]), t3);
+      for (int c = 4; c < 124; c += 8) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) t4[x] = max3(t4[x], s[c + 2 * x], s[c + 2 * x + 1]);
       }
-      const float t = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * a.scale_log2;
+      t4[0] = max3(t4[0], s[124], s[125]);
+      t4[1] = max3(t4[1], s[126], s[127]);
+      const float t = max3(max3(t4[0], t4[1], t4[2]), t4[3], t4[3]) * a.scale_log2;
+      // finite logits throughout: some exponentials may take the FMA pipe
+      const bool mixed = !whole ? false : __all_sync(~0u, t < INFINITY);
       if (__any_sync(~0u, t > m + kSlack)) {
         const float mn = fmaxf(m, t), corr = ex2(m - mn);
         m = mn;
@@ -329,21 +381,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      const float base = kShift - m;
-      float l0 = 0.f, l1 = 0.f;
+      const uint64_t base = f2(kShift - m, kShift - m), scale = f2(a.scale_log2, a.scale_log2);
+      uint64_t sum[2] = {0, 0};
+      auto probabilities = [&](auto poly) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t p[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const float p0 = ex2(fmaf(s[32 * c + 2 * x], a.scale_log2, base));
-          const float p1 = ex2(fmaf(s[32 * c + 2 * x + 1], a.scale_log2, base));
-          l0 += p0;
-          l1 += p1;
-          p[x] = pack_p<DT>(p0, p1);
+          for (int x = 0; x < 16; ++x) {
+            const uint64_t y = fma2(f2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale, base);
+            float p0, p1;
+            if (decltype(poly)::value && x % kPolyOf == kPolyOf - 1) {
+              exp2_poly(y, p0, p1);
+            } else {
+              f2_split(y, p0, p1);
+              p0 = ex2(p0);
+              p1 = ex2(p1);
+            }
+            sum[x & 1] = add2(sum[x & 1], f2(p0, p1));
+            p[x] = pack_p<DT>(p0, p1);
+          }
+          tmem_st16(ts + 16 * c, p);
         }
-        tmem_st16(ts + 16 * c, p);
-      }
+      };
+      if (mixed)
+        probabilities(std::true_type{});
+      else
+        probabilities(std::false_type{});
+      float l0, l1;
+      f2_split(add2(sum[0], sum[1]), l0, l1);
       l += l0 + l1;
       tmem_wait_st();
       tc_fence_before();
