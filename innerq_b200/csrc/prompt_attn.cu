@@ -43,6 +43,7 @@ constexpr float kShift = 7.f;            // P carries 2^7
 constexpr float kSlack = 8.f;            // lag of the running maximum
 constexpr float kNoMax = -1e30f;
 constexpr uint32_t kWait = 1u << 14;
+constexpr int kParts = 2;                // P is handed over in parts, so that P V starts before P is complete
 constexpr int kPolyOf = 4;               // one pair of exponentials of this many goes to the FMA pipe
 
 struct PromptDev {
@@ -62,7 +63,7 @@ struct PromptDev {
 struct alignas(1024) Smem {
   uint8_t q[2][kTileBytes];
   uint8_t ring[kRing][kTileBytes];
-  uint64_t q_full, full[kRing], checked[kRing], empty[kRing], s_full[2], p_ready[2], o_full[2];
+  uint64_t q_full, full[kRing], checked[kRing], empty[kRing], s_full[2], p_ready[2][kParts], o_full[2];
   uint32_t tmem;
   int seq, dirty;
 };
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_ready[i], 4);
+      for (int x = 0; x < kParts; ++x) mbar_init(&sm.p_ready[i][x], 4);
       mbar_init(&sm.o_full[i], 1);
     }
     mbar_fence_init();
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = sm.tmem;
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
     if (warp == 9 && lane == 0 && n > 0) {
       // -------------------------------------------------------- TMA loads
       const int tiles = w.n[1] > 0 ? 2 : 1;
@@ -242,10 +243,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mma_commit(leader, &sm.s_full[i]);
       };
-      auto values = [&](int i, int st, uint32_t acc) {
+      auto values = [&](int i, int st, int part, uint32_t acc) {
         const uint32_t db = v_lo + st * (kTileBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = part * (8 / kParts); k < (part + 1) * (8 / kParts); ++k)
           mma_ts<hi>(leader, tm + 256 + i * 128, tm + i * 128 + 8 * k, db + k * (2048 >> 4), id_o, k > 0 ? 1u : acc);
       };
       bool ok = mbar_wait_bounded(&sm.q_full, 0, kWait) && mbar_wait_bounded(&sm.full[0], 0, kWait);
@@ -271,12 +272,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2; ++i) {
           const int ni = i ? n1 : n0;
           if (j < ni) {
-            ok = ok && mbar_wait_bounded(&sm.p_ready[i], j & 1, kWait);
-            if (j + 1 < ni) ok = ok && mbar_wait_bounded(&sm.full[ks], kp, kWait);
-            ok = __all_sync(~0u, ok);
+#pragma unroll
+            for (int x = 0; x < kParts; ++x) {
+              ok = ok && mbar_wait_bounded(&sm.p_ready[i][x], j & 1, kWait);
+              if (x == kParts - 1 && j + 1 < ni) ok = ok && mbar_wait_bounded(&sm.full[ks], kp, kWait);
+              ok = __all_sync(~0u, ok);
+              if (ok) {
+                tc_fence_after();
+                values(i, vs, x, acc);
+              }
+            }
             if (ok) {
-              tc_fence_after();
-              values(i, vs, acc);
               if (j + 1 < ni)
                 scores(i, ks);
               else
@@ -328,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
     // ------------------------------------------------------------- softmax
     const int i = warp >> 2, row = tid & 127, qi = w.q0 + i * kRows + row;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 lanes per warp
@@ -341,6 +347,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       tc_fence_after();
       float s[128];
+      const int seen = lim - kRows * j;
+      const bool whole = __all_sync(~0u, seen >= kRows);
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s + 32 * c);
       tmem_wait_ld();
@@ -348,20 +356,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 128; ++c) s[c] = -s[c];
       }
-      const int seen = lim - kRows * j;
-      const bool whole = __all_sync(~0u, seen >= kRows);
       if (!whole) {
 #pragma unroll
         for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
       }
-      float t4[4] = {s[0], s[1], s[2], s[3]};
+      float t4[4];
 #pragma unroll
-      for (int c = 4; c < 124; c += 8) {
+      for (int c = 0; c < 128; c += 8) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) t4[x] = max3(t4[x], s[c + 2 * x], s[c + 2 * x + 1]);
+        for (int x = 0; x < 4; ++x) t4[x] = max3(c ? t4[x] : s[2 * x], s[c + 2 * x], s[c + 2 * x + 1]);
       }
-      t4[0] = max3(t4[0], s[124], s[125]);
-      t4[1] = max3(t4[1], s[126], s[127]);
       const float t = max3(max3(t4[0], t4[1], t4[2]), t4[3], t4[3]) * a.scale_log2;
       // finite logits throughout: some exponentials may take the FMA pipe
       const bool mixed = !whole ? false : __all_sync(~0u, t < INFINITY);
@@ -402,6 +406,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             p[x] = pack_p<DT>(p0, p1);
           }
           tmem_st16(ts + 16 * c, p);
+          if ((c + 1) % (4 / kParts) == 0) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.p_ready[i][c / (4 / kParts)]);
+          }
         }
       };
       if (mixed)
@@ -411,10 +421,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       float l0, l1;
       f2_split(add2(sum[0], sum[1]), l0, l1);
       l += l0 + l1;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.p_ready[i]);
     }
     // ------------------------------------------------------------ epilogue
     if (w.q0 + i * kRows < w.nq) {
