@@ -15,11 +15,14 @@
 //   warp 8          issues every MMA: S_i = Q_i K^T from shared memory, then
 //                   O_i += P_i V with P_i read from tensor memory, where it
 //                   replaces S_i
-//   warp 9          TMA loads: Q once, K and V tiles through a ring
+//   warp 9          TMA loads: Q, and K and V tiles through a ring
 //   warps 10, 11    look over the V tiles that some row must not see whole: a
 //                   masked probability is 0, but 0 * NaN is NaN, so values
 //                   that are not finite are set to 0 there and added again, in
 //                   the epilogue, to the rows that do see them
+// A CTA stays and takes over blocks that have not started (the grid is one block
+// per pair of query tiles and head, heavy ones first), so the loads and scores
+// of the next piece of work run under the epilogue of the last; warp 11 asks.
 // Tensor memory: S0 | S1 | O0 | O1, 128 columns each.  In-order execution of
 // the MMAs makes "S_i(j + 1) is complete" mean that O_i is at rest too.
 #include <algorithm>
@@ -60,12 +63,25 @@ struct PromptDev {
   int B, Hq, Hkv, Tq, Tk, causal, slots;
 };
 
+// One piece of work: 256 queries of one head of one sequence, and how many key
+// tiles each of its two query tiles needs (n0 < 0: there is no more work).
+struct Work {
+  int head, q_base, nq, k_base, nk, q0, n0, n1;
+  int cut;    // from this key tile on, some row must not see all of a tile
+  int dirty;  // the scan found values that are not finite
+  // keys that query row i of the sequence may see
+  __device__ __forceinline__ int limit(int i, int causal) const { return causal ? min(nk, i + nk - nq + 1) : nk; }
+};
+constexpr int kWorks = 4;  // pieces of work that the CTA's warps may be apart
+
 struct alignas(1024) Smem {
   uint8_t q[2][kTileBytes];
   uint8_t ring[kRing][kTileBytes];
-  uint64_t q_full, full[kRing], checked[kRing], empty[kRing], s_full[2], p_ready[2][kParts], o_full[2];
+  Work work[kWorks];
+  uint4 answer;
+  uint64_t work_full[kWorks], work_empty[kWorks], asked;
+  uint64_t q_full, q_empty, full[kRing], checked[kRing], empty[kRing], s_full[2], p_ready[2][kParts], o_full[2], drained;
   uint32_t tmem;
-  int seq, dirty;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -136,13 +152,84 @@ template <int DT> __device__ __forceinline__ bool not_finite(uint32_t h) {
   return (h & e) == e;
 }
 
-// The work of a CTA: queries q0 .. of sequence b, and how many key tiles each
-// of its two query tiles needs.
-struct Work {
-  int q_base, nq, k_base, nk, q0, off, n[2];
-  // keys that query row `i` of the sequence may see
-  __device__ __forceinline__ int limit(int i, int causal) const { return causal ? min(nk, i + off + 1) : nk; }
+// The work of block `block` (the last queries of a sequence see the most keys:
+// heavy blocks first); one warp.  False: none, the grid is an upper bound.
+__device__ __forceinline__ bool decode(const PromptDev& a, int block, int lane, Work& w) {
+  const int slot = a.slots - 1 - block / a.Hq;
+  w.head = block % a.Hq;
+  // slots of sequence b start at cu_q[b] / 256 + b: room for its pairs of tiles
+  int found = -1;
+  for (int b = lane; b < a.B; b += 32) {
+    const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
+    if (lo >= 0 && lo / kPair + b <= slot && slot < lo / kPair + b + (hi - lo + kPair - 1) / kPair) found = b;
+  }
+  const int b = __reduce_max_sync(~0u, found);
+  if (b < 0) return false;
+  w.q_base = a.cu_q[b];
+  w.nq = min(a.cu_q[b + 1], a.Tq) - w.q_base;
+  w.k_base = max(0, a.cu_k[b]);
+  w.nk = max(0, min(a.cu_k[b + 1], a.Tk) - w.k_base);
+  w.q0 = (slot - (w.q_base / kPair + b)) * kPair;
+  if (w.q0 >= w.nq) return false;
+  int n[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int first = w.q0 + i * kRows, last = min(first + kRows, w.nq) - 1;
+    n[i] = ((first < w.nq ? max(0, w.limit(last, a.causal)) : 0) + kRows - 1) / kRows;
+  }
+  w.n0 = n[0];
+  w.n1 = n[1];
+  w.cut = max(0, w.limit(w.q0 + (n[0] > 0 ? 0 : kRows), a.causal)) / kRows;
+  w.dirty = 0;
+  return true;
+}
+
+// A warp's way through the CTA's pieces of work.
+struct Pieces {
+  Smem& sm;
+  int slot = 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  __device__ __forceinline__ Pieces(Smem& s) : sm(s) {}
+  // the next piece; null: no more (or, with ok false, a wait that ran out)
+  __device__ __forceinline__ Work* next() {
+    ok = __all_sync(~0u, mbar_wait_bounded(&sm.work_full[slot], parity, kWait));
+    Work* w = &sm.work[slot];
+    return ok && w->n0 >= 0 ? w : nullptr;
+  }
+  __device__ __forceinline__ void step() {
+    if (++slot == kWorks) slot = 0, parity ^= 1;
+  }
+  __device__ __forceinline__ void done(int lane) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.work_empty[slot]);
+    step();
+  }
 };
+
+// the finished row of this thread: O / l, or zeros where there is no O
+template <int DT>
+__device__ __forceinline__ void write_row(uint32_t to, bool any, float inv, uint16_t* out) {
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    float o[32];
+    if (any) {
+      tmem_ld32(to + 32 * c, o);
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int x = 0; x < 32; ++x) o[x] = 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      uint4 v;
+      uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) e[y] = inv == 0.f ? 0u : pack_p<DT>(o[8 * x + 2 * y] * inv, o[8 * x + 2 * y + 1] * inv);
+      if (out) *reinterpret_cast<uint4*>(out + 32 * c + 8 * x) = v;
+    }
+  }
+}
 
 template <int DT>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -151,40 +238,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;  // warp: uniform, and known to be
-  griddep_wait();
-  griddep_launch_dependents();
-
-  // the last queries of a sequence see the most keys: heavy blocks first
-  const int slot = a.slots - 1 - (int)(blockIdx.x / a.Hq), head = blockIdx.x % a.Hq, kv_head = head / (a.Hq / a.Hkv);
-  if (tid == 0) sm.seq = -1, sm.dirty = 0;
-  __syncthreads();
-  for (int b = tid; b < a.B; b += kThreads) {
-    const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
-    if (lo >= 0 && lo / kPair + b <= slot && slot < lo / kPair + b + (hi - lo + kPair - 1) / kPair) sm.seq = b;
-  }
-  __syncthreads();
-  const int b = sm.seq;
-  if (b < 0) return;
-  Work w;
-  w.q_base = a.cu_q[b];
-  w.nq = min(a.cu_q[b + 1], a.Tq) - w.q_base;
-  w.k_base = max(0, a.cu_k[b]);
-  w.nk = max(0, min(a.cu_k[b + 1], a.Tk) - w.k_base);
-  w.q0 = (slot - (w.q_base / kPair + b)) * kPair;
-  w.off = w.nk - w.nq;
-  if (w.q0 >= w.nq) return;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int first = w.q0 + i * kRows, last = min(first + kRows, w.nq) - 1;
-    const int keys = first < w.nq ? max(0, w.limit(last, a.causal)) : 0;
-    w.n[i] = (keys + kRows - 1) / kRows;
-  }
-  const int n = __shfl_sync(~0u, max(w.n[0], w.n[1]), 0), n0 = __shfl_sync(~0u, w.n[0], 0), n1 = __shfl_sync(~0u, w.n[1], 0);
-  // from this key tile on, some row of the CTA must not see all of a tile
-  const int cut = __shfl_sync(~0u, max(0, w.limit(w.q0 + (w.n[0] > 0 ? 0 : kRows), a.causal)) / kRows, 0);
 
   if (tid == 0) {
+    for (int i = 0; i < kWorks; ++i) {
+      mbar_init(&sm.work_full[i], 1);
+      mbar_init(&sm.work_empty[i], 11);
+    }
+    mbar_init(&sm.asked, 1);
     mbar_init(&sm.q_full, 1);
+    mbar_init(&sm.q_empty, 1);
+    mbar_init(&sm.drained, 1);
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.checked[i], 2);
@@ -202,32 +265,53 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
+  griddep_wait();
+  griddep_launch_dependents();
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
-    if (warp == 9 && lane == 0 && n > 0) {
+    Pieces pieces(sm);
+    if (warp == 9) {
       // -------------------------------------------------------- TMA loads
-      const int tiles = w.n[1] > 0 ? 2 : 1;
-      mbar_arrive_tx(&sm.q_full, tiles * kTileBytes);
-      for (int i = 0; i < tiles; ++i)
-        for (int h = 0; h < 2; ++h)
-          tma_load_3d(sm.q[i] + h * kHalfTile, &mq, 64 * h, head, w.q_base + w.q0 + i * kRows, &sm.q_full);
+      int st = 0, filled = 0, q_count = 0;  // ring slot of the next tile, how many are in use at most
+      uint32_t parity = 1;                  // of the slot's last release
       bool ok = true;
-      int sent = 0;
-      for (; sent < 2 * n; ++sent) {
-        const int st = sent % kRing;
-        if (sent >= kRing && !(ok = mbar_wait_bounded(&sm.empty[st], (sent / kRing - 1) & 1, kWait))) break;
-        const CUtensorMap* m = sent & 1 ? &mv : &mk;
-        mbar_arrive_tx(&sm.full[st], kTileBytes);
-        for (int h = 0; h < 2; ++h)
-          tma_load_3d(sm.ring[st] + h * kHalfTile, m, 64 * h, kv_head, w.k_base + (sent >> 1) * kRows, &sm.full[st]);
+      while (Work* w = pieces.next()) {
+        const int n = max(w->n0, w->n1), tiles = w->n1 > 0 ? 2 : 1, head = w->head, q_row = w->q_base + w->q0, k_base = w->k_base;
+        pieces.done(lane);
+        if (n == 0) continue;
+        const int kv_head = head / (a.Hq / a.Hkv);
+        if (q_count > 0) ok = __all_sync(~0u, mbar_wait_bounded(&sm.q_empty, (q_count - 1) & 1, kWait));
+        if (!ok) break;
+        ++q_count;
+        if (lane == 0) {
+          mbar_arrive_tx(&sm.q_full, tiles * kTileBytes);
+          for (int i = 0; i < tiles; ++i)
+            for (int h = 0; h < 2; ++h) tma_load_3d(sm.q[i] + h * kHalfTile, &mq, 64 * h, head, q_row + i * kRows, &sm.q_full);
+        }
+        for (int it = 0; ok && it < 2 * n; ++it) {
+          if (filled == kRing)
+            ok = __all_sync(~0u, mbar_wait_bounded(&sm.empty[st], parity, kWait));
+          else
+            ++filled;
+          if (ok && lane == 0) {
+            const CUtensorMap* m = it & 1 ? &mv : &mk;
+            mbar_arrive_tx(&sm.full[st], kTileBytes);
+            for (int h = 0; h < 2; ++h)
+              tma_load_3d(sm.ring[st] + h * kHalfTile, m, 64 * h, kv_head, k_base + (it >> 1) * kRows, &sm.full[st]);
+          }
+          if (++st == kRing) st = 0, parity ^= 1;
+        }
+        if (!ok) break;
       }
-      if (!ok) {  // give up: the copies under way must land before the memory is given away
-        mbar_wait_bounded(&sm.q_full, 0, kWait / 16);
-        for (int i = max(0, sent - kRing); i < sent; ++i)
-          mbar_wait_bounded(&sm.full[i % kRing], (i / kRing) & 1, kWait / 16);
+      if (!ok || !pieces.ok) {
+        // give up: the copies under way must land before the memory is given
+        // away.  `parity` is that of the releases; the fillings before slot st
+        // have the same one, those from st on the other.
+        if (q_count > 0) mbar_wait_bounded(&sm.q_full, (q_count - 1) & 1, kWait / 16);
+        for (int i = 0; i < filled; ++i) mbar_wait_bounded(&sm.full[i], i < st ? parity ^ 1 : parity, kWait / 16);
       }
-    } else if (warp == 8 && n > 0) {
+    } else if (warp == 8) {
       // -------------------------------------------------------------- MMAs
       constexpr uint32_t id_s = mma_idesc(kRows, kRows, DT, 0), id_o = mma_idesc(kRows, 128, DT, 1), hi = desc_hi(1024);
       const uint32_t leader = elect_one();
@@ -249,241 +333,286 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int k = part * (8 / kParts); k < (part + 1) * (8 / kParts); ++k)
           mma_ts<hi>(leader, tm + 256 + i * 128, tm + i * 128 + 8 * k, db + k * (2048 >> 4), id_o, k > 0 ? 1u : acc);
       };
-      bool ok = mbar_wait_bounded(&sm.q_full, 0, kWait) && mbar_wait_bounded(&sm.full[0], 0, kWait);
-      ok = __all_sync(~0u, ok);
-      // ring slots of V_j and K_(j+1), and the parities of their fillings.  A
-      // slot is given back only if a later tile comes into it, so that no
-      // arrival is outstanding when the CTA ends.
-      int vs = 1, ks = 2;
-      uint32_t vp = 0, kp = 0;
-      if (ok) {
+      // ring slots of K_j / V_j in turn, with the parities of their fillings
+      int st = 0;
+      uint32_t par = 0, q_par = 0, p_par[2] = {0, 0};
+      auto advance = [&]() {
+        if (++st == kRing) st = 0, par ^= 1;
+      };
+      bool ok = true;
+      while (Work* w = pieces.next()) {
+        const int n0 = __shfl_sync(~0u, w->n0, 0), n1 = __shfl_sync(~0u, w->n1, 0), cut = __shfl_sync(~0u, w->cut, 0);
+        const int n = max(n0, n1);
+        pieces.done(lane);
+        if (n == 0) continue;
+        ok = mbar_wait_bounded(&sm.q_full, q_par, kWait) && mbar_wait_bounded(&sm.full[st], par, kWait);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        q_par ^= 1;
         tc_fence_after();
-        if (n0 > 0) scores(0, 0);
-        if (n1 > 0) scores(1, 0);
-        if (kRing < 2 * n) mma_commit(leader, &sm.empty[0]);
-      }
+        if (n0 > 0) scores(0, st);
+        if (n1 > 0) scores(1, st);
+        mma_commit(leader, &sm.empty[st]);
+        if (n == 1) mma_commit(leader, &sm.q_empty);
+        advance();
 #pragma unroll 1
-      for (int j = 0; ok && j < n; ++j) {
-        ok = mbar_wait_bounded(&sm.full[vs], vp, kWait);
-        if (j >= cut) ok = ok && mbar_wait_bounded(&sm.checked[vs], vp, kWait);
-        if (!__all_sync(~0u, ok)) break;
-        const uint32_t acc = j > 0;
+        for (int j = 0; j < n; ++j) {
+          const int vs = st;
+          const uint32_t vp = par;
+          advance();
+          const int ks = st;
+          const uint32_t kp = par;
+          ok = mbar_wait_bounded(&sm.full[vs], vp, kWait);
+          if (j >= cut) ok = ok && mbar_wait_bounded(&sm.checked[vs], vp, kWait);
+          const uint32_t acc = j > 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int ni = i ? n1 : n0;
-          if (j < ni) {
+          for (int i = 0; i < 2; ++i) {
+            const int ni = i ? n1 : n0;
+            if (j < ni) {
 #pragma unroll
-            for (int x = 0; x < kParts; ++x) {
-              ok = ok && mbar_wait_bounded(&sm.p_ready[i][x], j & 1, kWait);
-              if (x == kParts - 1 && j + 1 < ni) ok = ok && mbar_wait_bounded(&sm.full[ks], kp, kWait);
-              ok = __all_sync(~0u, ok);
+              for (int x = 0; x < kParts; ++x) {
+                ok = ok && mbar_wait_bounded(&sm.p_ready[i][x], p_par[i], kWait);
+                if (x == kParts - 1 && j + 1 < ni) ok = ok && mbar_wait_bounded(&sm.full[ks], kp, kWait);
+                ok = __all_sync(~0u, ok);
+                if (ok) {
+                  tc_fence_after();
+                  values(i, vs, x, acc);
+                }
+              }
+              p_par[i] ^= 1;
               if (ok) {
-                tc_fence_after();
-                values(i, vs, x, acc);
+                if (j + 1 < ni)
+                  scores(i, ks);
+                else
+                  mma_commit(leader, &sm.o_full[i]);
               }
             }
-            if (ok) {
-              if (j + 1 < ni)
-                scores(i, ks);
-              else
-                mma_commit(leader, &sm.o_full[i]);
-            }
+          }
+          if (!ok) break;
+          mma_commit(leader, &sm.empty[vs]);
+          if (j + 1 < n) {
+            mma_commit(leader, &sm.empty[ks]);
+            if (j + 2 == n) mma_commit(leader, &sm.q_empty);  // the last scores are under way
+            advance();
           }
         }
-        if (2 * j + 1 + kRing < 2 * n) mma_commit(leader, &sm.empty[vs]);
-        if (2 * j + 2 + kRing < 2 * n) mma_commit(leader, &sm.empty[ks]);
-        vs += 2;
-        ks += 2;
-        if (vs >= kRing) vs -= kRing, vp ^= 1;
-        if (ks >= kRing) ks -= kRing, kp ^= 1;
+        if (!ok) break;
       }
-    } else if (warp >= 10) {
-      // ------------------------------------------- values that are not finite
-      for (int it = 0; it < 2 * n; ++it) {
-        const int st = it % kRing;
-        if (!__all_sync(~0u, mbar_wait_bounded(&sm.full[st], (it / kRing) & 1, kWait))) break;
-        if ((it & 1) && (it >> 1) >= cut) {
-          uint4* p = reinterpret_cast<uint4*>(sm.ring[st]) + (warp - 10) * (kTileBytes / 32);
-          bool found = false;
-#pragma unroll 4
-          for (int x = lane; x < kTileBytes / 32; x += 32) {
-            uint4 v = p[x];
-            uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-            bool bad = false;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) bad |= not_finite<DT>(e[y]) | not_finite<DT>(e[y] >> 16);
-            if (bad) {
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-                e[y] &= (not_finite<DT>(e[y]) ? 0u : 0xffffu) | (not_finite<DT>(e[y] >> 16) ? 0u : 0xffff0000u);
-              p[x] = v;
-              found = true;
-            }
+      // no arrival may be outstanding when the CTA ends
+      mma_commit(leader, &sm.drained);
+      mbar_wait_bounded(&sm.drained, 0, kWait);
+    } else {
+      // ------------------ warps 10, 11: values that are not finite; 11: more work
+      bool asking = true;
+      uint32_t asked_par = 0;
+      int put = 0;
+      uint32_t put_par = 1;
+      // publish the next piece of work; the first is this block's own
+      auto publish = [&](int block) {
+        Work w;
+        bool any = block >= 0 && decode(a, block, lane, w);
+        while (!any && asking) {
+          if (lane == 0) {
+            mbar_arrive_tx(&sm.asked, 16);
+            next_block_ask(&sm.answer, &sm.asked);
           }
-          if (found) {
-            sm.dirty = 1;
-            fence_proxy_async();
-          }
+          __syncwarp();
+          asking = __all_sync(~0u, mbar_wait_bounded(&sm.asked, asked_par, kWait));
+          asked_par ^= 1;
+          const int x = asking ? next_block_get(&sm.answer) : -1;
+          fence_proxy_async();
+          __syncwarp();
+          asking = x >= 0;
+          any = asking && decode(a, x, lane, w);
+        }
+        if (!any) w.n0 = -1;
+        if (!__all_sync(~0u, mbar_wait_bounded(&sm.work_empty[put], put_par, kWait))) return;
+        if (lane == 0) {
+          sm.work[put] = w;
+          mbar_arrive(&sm.work_full[put]);
         }
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&sm.checked[st]);
-          mbar_arrive(&sm.empty[st]);
+        if (++put == kWorks) put = 0, put_par ^= 1;
+      };
+      if (warp == 11) publish(blockIdx.x);
+      int st = 0;
+      uint32_t par = 0;
+      bool ok = true;
+      while (Work* w = pieces.next()) {
+        const int n = max(w->n0, w->n1), cut = w->cut;
+        if (warp == 11) publish(-1);
+        for (int it = 0; ok && it < 2 * n; ++it) {
+          ok = __all_sync(~0u, mbar_wait_bounded(&sm.full[st], par, kWait));
+          if (!ok) break;
+          if ((it & 1) && (it >> 1) >= cut) {
+            uint4* p = reinterpret_cast<uint4*>(sm.ring[st]) + (warp - 10) * (kTileBytes / 32);
+            bool found = false;
+#pragma unroll 4
+            for (int x = lane; x < kTileBytes / 32; x += 32) {
+              uint4 v = p[x];
+              uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+              bool bad = false;
+#pragma unroll
+              for (int y = 0; y < 4; ++y) bad |= not_finite<DT>(e[y]) | not_finite<DT>(e[y] >> 16);
+              if (bad) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  e[y] &= (not_finite<DT>(e[y]) ? 0u : 0xffffu) | (not_finite<DT>(e[y] >> 16) ? 0u : 0xffff0000u);
+                p[x] = v;
+                found = true;
+              }
+            }
+            if (found) {
+              w->dirty = 1;
+              fence_proxy_async();
+            }
+          }
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&sm.checked[st]);
+            mbar_arrive(&sm.empty[st]);
+          }
+          if (++st == kRing) st = 0, par ^= 1;
         }
+        if (!ok) break;
+        if (warp == 10)
+          pieces.done(lane);
+        else
+          pieces.step();
       }
     }
     __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
     // ------------------------------------------------------------- softmax
-    const int i = warp >> 2, row = tid & 127, qi = w.q0 + i * kRows + row;
+    const int i = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 lanes per warp
     const uint32_t ts = tmem + i * 128 + lanes, to = tmem + 256 + i * 128 + lanes;
-    const int lim = w.limit(qi, a.causal);
-    float m = kNoMax, l = 0.f;
-    bool ok = true;
-    for (int j = 0; j < w.n[i]; ++j) {
-      ok = __all_sync(~0u, mbar_wait_bounded(&sm.s_full[i], j & 1, kWait));
-      if (!ok) break;
-      tc_fence_after();
-      float s[128];
-      const int seen = lim - kRows * j;
-      const bool whole = __all_sync(~0u, seen >= kRows);
+    const uint64_t scale = f2(a.scale_log2, a.scale_log2);
+    Pieces pieces(sm);
+    uint32_t s_par = 0, o_par = 0;
+    while (Work* w = pieces.next()) {
+      const int first = w->q0 + i * kRows, n = i ? w->n1 : w->n0, qi = first + row;
+      const int lim = w->limit(qi, a.causal);
+      float m = kNoMax, l = 0.f;
+      bool ok = true;
+#pragma unroll 1
+      for (int j = 0; j < n; ++j) {
+        ok = __all_sync(~0u, mbar_wait_bounded(&sm.s_full[i], s_par, kWait));
+        if (!ok) break;
+        s_par ^= 1;
+        tc_fence_after();
+        float s[128];
+        const int seen = lim - kRows * j;
+        const bool whole = __all_sync(~0u, seen >= kRows);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s + 32 * c);
-      tmem_wait_ld();
-      if (a.negate) {
+        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s + 32 * c);
+        tmem_wait_ld();
+        if (a.negate) {
 #pragma unroll
-        for (int c = 0; c < 128; ++c) s[c] = -s[c];
-      }
-      if (!whole) {
+          for (int c = 0; c < 128; ++c) s[c] = -s[c];
+        }
+        if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
-      }
-      float t4[4];
+          for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
+        }
+        float t4[4];
 #pragma unroll
-      for (int c = 0; c < 128; c += 8) {
+        for (int c = 0; c < 128; c += 8) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) t4[x] = max3(c ? t4[x] : s[2 * x], s[c + 2 * x], s[c + 2 * x + 1]);
-      }
-      const float t = max3(max3(t4[0], t4[1], t4[2]), t4[3], t4[3]) * a.scale_log2;
-      // finite logits throughout: some exponentials may take the FMA pipe
-      const bool mixed = !whole ? false : __all_sync(~0u, t < INFINITY);
-      if (__any_sync(~0u, t > m + kSlack)) {
-        const float mn = fmaxf(m, t), corr = ex2(m - mn);
-        m = mn;
-        l *= corr;
-        if (j > 0) {
+          for (int x = 0; x < 4; ++x) t4[x] = max3(c ? t4[x] : s[2 * x], s[c + 2 * x], s[c + 2 * x + 1]);
+        }
+        const float t = max3(max3(t4[0], t4[1], t4[2]), t4[3], t4[3]) * a.scale_log2;
+        // finite logits throughout: some exponentials may take the FMA pipe
+        const bool mixed = !whole ? false : __all_sync(~0u, t < INFINITY);
+        if (__any_sync(~0u, t > m + kSlack)) {
+          const float mn = fmaxf(m, t), corr = ex2(m - mn);
+          m = mn;
+          l *= corr;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float o[32];
+              tmem_ld32(to + 32 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] *= corr;
+              tmem_st32(to + 32 * c, o);
+            }
+          }
+        }
+        const uint64_t base = f2(kShift - m, kShift - m);
+        uint64_t sum[2] = {0, 0};
+        auto probabilities = [&](auto poly) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            float o[32];
-            tmem_ld32(to + 32 * c, o);
-            tmem_wait_ld();
+            uint32_t p[16];
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] *= corr;
-            tmem_st32(to + 32 * c, o);
-          }
-        }
-      }
-      const uint64_t base = f2(kShift - m, kShift - m), scale = f2(a.scale_log2, a.scale_log2);
-      uint64_t sum[2] = {0, 0};
-      auto probabilities = [&](auto poly) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
-#pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const uint64_t y = fma2(f2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale, base);
-            float p0, p1;
-            if (decltype(poly)::value && x % kPolyOf == kPolyOf - 1) {
-              exp2_poly(y, p0, p1);
-            } else {
-              f2_split(y, p0, p1);
-              p0 = ex2(p0);
-              p1 = ex2(p1);
+            for (int x = 0; x < 16; ++x) {
+              const uint64_t y = fma2(f2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale, base);
+              float p0, p1;
+              if (decltype(poly)::value && x % kPolyOf == kPolyOf - 1) {
+                exp2_poly(y, p0, p1);
+              } else {
+                f2_split(y, p0, p1);
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+              }
+              sum[x & 1] = add2(sum[x & 1], f2(p0, p1));
+              p[x] = pack_p<DT>(p0, p1);
             }
-            sum[x & 1] = add2(sum[x & 1], f2(p0, p1));
-            p[x] = pack_p<DT>(p0, p1);
+            tmem_st16(ts + 16 * c, p);
+            if ((c + 1) % (4 / kParts) == 0) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sm.p_ready[i][c / (4 / kParts)]);
+            }
           }
-          tmem_st16(ts + 16 * c, p);
-          if ((c + 1) % (4 / kParts) == 0) {
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.p_ready[i][c / (4 / kParts)]);
-          }
-        }
-      };
-      if (mixed)
-        probabilities(std::true_type{});
-      else
-        probabilities(std::false_type{});
-      float l0, l1;
-      f2_split(add2(sum[0], sum[1]), l0, l1);
-      l += l0 + l1;
-    }
-    // ------------------------------------------------------------ epilogue
-    if (w.q0 + i * kRows < w.nq) {
-      // (without keys of its own, a tile still waits for its Q, whose memory it writes)
-      if (ok && n > 0) ok = __all_sync(~0u, mbar_wait_bounded(w.n[i] > 0 ? &sm.o_full[i] : &sm.q_full, 0, kWait));
-      tc_fence_after();
-      // the finished row goes through this tile's Q memory: chunk x of a row at x ^ (row & 7)
-      uint4* mine = reinterpret_cast<uint4*>(sm.q[i]) + row * 16;
-      const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float o[32];
-        if (w.n[i] > 0) {
-          tmem_ld32(to + 32 * c, o);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = 0.f;
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint4 v;
-          uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float p0 = o[8 * x + 2 * y] * inv, p1 = o[8 * x + 2 * y + 1] * inv;
-            e[y] = l == 0.f && ok ? 0u : pack_p<DT>(p0, p1);
-          }
-          mine[(4 * c + x) ^ (row & 7)] = v;
-        }
+        };
+        if (mixed)
+          probabilities(std::true_type{});
+        else
+          probabilities(std::false_type{});
+        float l0, l1;
+        f2_split(add2(sum[0], sum[1]), l0, l1);
+        l += l0 + l1;
       }
-      if (ok && *(volatile int*)&sm.dirty && qi < w.nq) {
-        // values that were set to 0 and that this row does see
-        const uint16_t* qr = a.q + (int64_t)(w.q_base + qi) * a.q_st + head * a.q_sh;
-        for (int j = cut; j < w.n[i]; ++j) {
-          for (int key = kRows * j; key < min(kRows * (j + 1), lim); ++key) {
-            const uint16_t* vr = a.v + (int64_t)(w.k_base + key) * a.v_st + kv_head * a.v_sh;
+      // ---------------------------------------------------------- epilogue
+      if (first < w->nq) {
+        if (n > 0) {
+          if (ok) ok = __all_sync(~0u, mbar_wait_bounded(&sm.o_full[i], o_par, kWait));
+          o_par ^= 1;
+          tc_fence_after();
+        }
+        const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
+        uint16_t* out = a.out + (int64_t)(w->q_base + qi) * a.o_st + w->head * a.o_sh;
+        write_row<DT>(to, n > 0, inv, qi < w->nq ? out : nullptr);
+        tc_fence_before();
+        if (ok && *(volatile int*)&w->dirty && qi < w->nq) {
+          // values that were set to 0 and that this row does see
+          const int kv_head = w->head / (a.Hq / a.Hkv);
+          const uint16_t* qr = a.q + (int64_t)(w->q_base + qi) * a.q_st + w->head * a.q_sh;
+          for (int key = kRows * w->cut; key < min(kRows * n, lim); ++key) {
+            const uint16_t* vr = a.v + (int64_t)(w->k_base + key) * a.v_st + kv_head * a.v_sh;
             float p = -1.f;
             for (int d = 0; d < kD; ++d) {
               if (!not_finite<DT>(vr[d])) continue;
               if (p == -1.f) {
-                const uint16_t* kr = a.k + (int64_t)(w.k_base + key) * a.k_st + kv_head * a.k_sh;
+                const uint16_t* kr = a.k + (int64_t)(w->k_base + key) * a.k_st + kv_head * a.k_sh;
                 float dot = 0.f;
                 for (int x = 0; x < kD; ++x) dot = fmaf(to_f<DT>(qr[x]), to_f<DT>(kr[x]), dot);
                 p = ex2(fmaf(a.negate ? -dot : dot, a.scale_log2, kShift - m)) * inv;
               }
-              uint16_t* at = reinterpret_cast<uint16_t*>(mine + ((d >> 3) ^ (row & 7))) + (d & 7);
-              *at = from_f<DT>(to_f<DT>(*at) + p * to_f<DT>(vr[d]));
+              out[d] = from_f<DT>(to_f<DT>(out[d]) + p * to_f<DT>(vr[d]));
             }
           }
         }
+        if (a.lse && qi < w->nq)
+          a.lse[(int64_t)(w->q_base + qi) * a.Hq + w->head] = l == 0.f ? -INFINITY : m - kShift + log2f(l);
       }
-      if (a.lse && qi < w.nq)
-        a.lse[(int64_t)(w.q_base + qi) * a.Hq + head] = l == 0.f ? -INFINITY : m - kShift + log2f(l);
-      __syncwarp();
-      // two rows per instruction, 16 bytes per lane
-#pragma unroll 4
-      for (int r = 0; r < 32; r += 2) {
-        const int rr = (warp & 3) * 32 + r + (lane >> 4), x = lane & 15, at = w.q0 + i * kRows + rr;
-        if (at < w.nq)
-          *reinterpret_cast<uint4*>(a.out + (int64_t)(w.q_base + at) * a.o_st + head * a.o_sh + 8 * x) =
-              reinterpret_cast<const uint4*>(sm.q[i])[rr * 16 + (x ^ (rr & 7))];
-      }
+      if (!ok) break;
+      pieces.done(lane);
     }
   }
   tc_fence_before();

@@ -119,4 +119,26 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// -------------------------------------------------- taking over blocks ---
+// Ask for a block of this grid that has not been launched yet: 16 bytes at
+// `answer`, completing `bar`.  After a "no" it must not be asked again.
+__device__ __forceinline__ void next_block_ask(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// its blockIdx.x, or -1: there is none
+__device__ __forceinline__ int next_block_get(const void* answer) {
+  int x;
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b128 h;\n .reg .b32 y, z, w;\n ld.shared.b128 h, [%1];\n mov.b32 %0, -1;\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, h;\n}\n"
+      : "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return x;
+}
+
 }  // namespace innerq
