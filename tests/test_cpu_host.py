@@ -242,3 +242,69 @@ def test_struct_formats_match_c_layout(tmp_path):
             args[i] = 1.0 if kinds[i] == "f" else 1
             packed = fmt.pack(*args)
             assert any(packed[off:off + width]) and not any(packed[:off] + packed[off + width:]), (name, i)
+
+
+def test_paged_and_prompt_entry_points_reject_bad_arguments_without_a_gpu():
+    """Checks of the paged cache's and the prompt attention's entry points run
+    before any device work."""
+    from innerq_b200 import _lib
+    lib = _lib.load()
+
+    def paged(**kw):
+        f = dict(size=_lib.PAGED_FORMAT.size, dtype=0, D=128, Hkv=2, tiles=2, n_pages=4, n_slots=2, sink=32, recent=32, B=1,
+                 cols=4, pages=256, dk=256, dv=256, table=256, stride=4, slots=256, lens=256)
+        f.update(kw)
+        return _lib.PAGED_FORMAT.pack(*f.values())
+
+    def new(**kw):
+        f = dict(size=_lib.PAGED_NEW_FORMAT.size, Hq=4, T=1, rot=128, inter=0, max_pos=9, q=256, q1=512, q2=128, k=256, k1=256,
+                 k2=128, v=256, v1=256, v2=128, cu=0, cos=256, sin=256, cs=64, qo=256, qo1=512, qo2=128, ko=0, ko1=256, ko2=128)
+        f.update(kw)
+        return _lib.PAGED_NEW_FORMAT.pack(*f.values())
+
+    def prompt(**kw):
+        f = dict(size=_lib.PROMPT_FORMAT.size, dtype=0, D=128, B=1, Hq=4, Hkv=2, Tq=8, Tk=8, causal=1, scale=1.0, q=256, q1=512,
+                 q2=128, k=256, k1=256, k2=128, v=256, v1=256, v2=128, cu_q=256, cu_k=256, o=256, o1=512, o2=128, lse=0)
+        f.update(kw)
+        return _lib.PROMPT_FORMAT.pack(*f.values())
+
+    bad_cache = [(dict(size=8), -1, "struct_size"), (dict(dtype=2), -1, "dtype"), (dict(D=64), -2, "head_dim"),
+                 (dict(Hkv=0), -1, "size"), (dict(tiles=0), -1, "tiles"), (dict(tiles=65), -1, "tiles"),
+                 (dict(sink=16), -1, "multiples"), (dict(recent=-32), -1, "multiples"), (dict(slots=0), -1, "null"),
+                 (dict(pages=0), -1, "null"), (dict(dk=264), -1, "aligned"), (dict(B=-1), -1, "size")]
+    for kw, code, word in bad_cache:
+        for call in (lambda c: lib.innerq_paged_append(c, new(), None), lambda c: lib.innerq_paged_read(c, 256, 256, 1, 256, 256, None),
+                     lambda c: lib.innerq_paged_attn(c, 4, 256, 512, 128, 1.0, 256, 1 << 30, 256, 512, 128, None, None)):
+            assert call(paged(**kw)) == code and word in _lib.last_error(), (kw, _lib.last_error())
+        assert lib.innerq_paged_attn_workspace(paged(**kw), 4) == -1
+    for kw, word in [(dict(size=4), "struct_size"), (dict(T=-1), "size"), (dict(T=2), "cu_seqlens"), (dict(rot=24), "rotation"),
+                     (dict(rot=144), "rotation"), (dict(q=0), "null"), (dict(v=0), "null"), (dict(cos=0), "table"),
+                     (dict(max_pos=0), "table"), (dict(k1=257), "strides"), (dict(q=264), "aligned"), (dict(cs=63), "aligned")]:
+        assert lib.innerq_paged_append(paged(), new(**kw), None) == -1 and word in _lib.last_error(), (kw, _lib.last_error())
+    assert lib.innerq_paged_append(paged(B=0), new(T=0), None) == 0  # nothing to do
+    assert lib.innerq_paged_read(paged(), 0, 256, 1, 256, 256, None) == -1
+    assert lib.innerq_paged_read(paged(), 256, 256, -1, 256, 256, None) == -1
+    assert lib.innerq_paged_read(paged(), 256, 256, 0, 256, 256, None) == 0
+    attn = lambda c=paged(), hq=4, q=256, ws=256, n=1 << 30: lib.innerq_paged_attn(  # noqa: E731
+        c, hq, q, 512, 128, 1.0, ws, n, 256, 512, 128, None, None)
+    assert attn(hq=3) == -1 and "heads" in _lib.last_error()
+    assert attn(hq=18) == -2 and "GQA" in _lib.last_error()
+    assert attn(q=0) == -1 and attn(ws=8) == -1 and attn(n=16) == -1 and "workspace" in _lib.last_error()
+    assert attn(paged(cols=1 << 30, tiles=64)) == -1 and "too large" in _lib.last_error()
+    assert attn(paged(B=0)) == 0
+    for kw, code, word in [(dict(size=4), -1, "struct_size"), (dict(dtype=5), -1, "dtype"), (dict(D=64), -2, "head_dim"),
+                           (dict(Hq=3), -1, "heads"), (dict(Tq=-1), -1, "sizes"), (dict(q=0), -1, "null"), (dict(cu_k=0), -1, "null"),
+                           (dict(k=0), -1, "null"), (dict(q1=513), -1, "strides"), (dict(v=264), -1, "aligned")]:
+        assert lib.innerq_prompt_attn(prompt(**kw), None) == code and word in _lib.last_error(), (kw, _lib.last_error())
+    assert lib.innerq_prompt_attn(prompt(B=0), None) == 0 and lib.innerq_prompt_attn(prompt(Tq=0), None) == 0
+
+
+def test_paged_cache_and_prompt_attention_refuse_cpu_tensors():
+    from innerq_b200.paged import PagedCache
+    from innerq_b200.prompt import prompt_attention
+    with pytest.raises(RuntimeError, match="CUDA"):
+        PagedCache(torch.zeros((1, 1, 1, 4608), dtype=torch.uint8), torch.zeros((1, 1, 32, 128), dtype=torch.float16),
+                   torch.zeros((1, 1, 32, 128), dtype=torch.float16), 0, 0)
+    x = torch.zeros((1, 1, 128), dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        prompt_attention(x, x, x, torch.zeros(2, dtype=torch.int32))

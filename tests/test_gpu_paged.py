@@ -366,3 +366,92 @@ def test_decode_step_in_a_graph():
                 want, _ = s.oracle.attend(b, q[b], D ** -0.5)
                 close(out[b].double().cpu().numpy(), want, "fp16", np.abs(s.oracle.cv[b]).max())
     s.check_read()
+
+
+def test_refusals():
+    """Arguments of the wrong shape, type or device raise before any launch."""
+    from innerq_b200 import _lib
+    from innerq_b200.paged import PagedCache
+    from innerq_b200.prompt import prompt_attention
+    c = PagedCache.allocate(4, 2, 2, 64, 32, 32)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    x = lambda n, h: torch.zeros((n, h, D), dtype=torch.float16, device="cuda")  # noqa: E731
+    tab, sl, ln = i32(2, 3), i32(2), i32(2)
+    with pytest.raises(ValueError):
+        PagedCache(c.pages, c.dense_k, c.dense_v, 32, 64)  # another window than the slots have
+    with pytest.raises(ValueError):
+        PagedCache(c.pages, c.dense_k, c.dense_v, 16, 48)
+    with pytest.raises(ValueError):
+        PagedCache(c.pages[..., :4000], c.dense_k, c.dense_v, 32, 32)
+    with pytest.raises(NotImplementedError):
+        PagedCache(c.pages, c.dense_k[..., :64].contiguous(), c.dense_v[..., :64].contiguous(), 32, 32)
+    with pytest.raises(TypeError):
+        PagedCache(c.pages, c.dense_k.float(), c.dense_v.float(), 32, 32)
+    with pytest.raises(ValueError):
+        PagedCache.allocate(4, 2, 2, 48)
+    with pytest.raises(TypeError):
+        c.attend(x(2, 4), tab.long(), sl, ln)
+    with pytest.raises(TypeError):
+        c.attend(x(2, 4), tab, sl, ln.cpu())
+    with pytest.raises(ValueError):
+        c.attend(x(2, 4), tab, sl[:1], ln)
+    with pytest.raises(ValueError):
+        c.attend(x(3, 4), tab, sl, ln)
+    with pytest.raises(TypeError):
+        c.attend(x(2, 4).bfloat16(), tab, sl, ln)
+    with pytest.raises(_lib.InnerqError):
+        c.attend(x(2, 5), tab, sl, ln)  # not a multiple of the key heads
+    with pytest.raises(_lib.InnerqError):
+        c.attend(x(2, 18), tab, sl, ln)  # more than eight query heads to a key head
+    with pytest.raises(ValueError):
+        c.attend(x(2, 4), tab, sl, ln, out=x(2, 6))
+    with pytest.raises(ValueError):
+        c.attend(x(2, 4), tab, sl, ln, lse=torch.zeros((2, 5), device="cuda"))
+    with pytest.raises(ValueError):
+        c.append(None, x(3, 2), x(3, 2), tab, sl, ln)  # three tokens, two sequences, no cu_seqlens
+    with pytest.raises(ValueError):
+        c.append(None, x(2, 3), x(2, 3), tab, sl, ln)
+    with pytest.raises(ValueError):
+        c.append(x(1, 4), x(2, 2), x(2, 2), tab, sl, ln)
+    with pytest.raises(ValueError):
+        c.append(None, x(2, 2), x(2, 2), tab, sl, ln, cos=torch.zeros((4, 64), device="cuda"))
+    with pytest.raises(TypeError):
+        c.append(None, x(2, 2), x(2, 2), tab, sl, ln, cos=torch.zeros((4, 64), device="cuda").half(),
+                 sin=torch.zeros((4, 64), device="cuda").half())
+    with pytest.raises(_lib.InnerqError):
+        c.append(None, x(2, 2), x(2, 2), tab, sl, ln, cos=torch.zeros((4, 12), device="cuda"), sin=torch.zeros((4, 12), device="cuda"))
+    q, k = x(4, 4), x(4, 2)
+    with pytest.raises(ValueError):
+        prompt_attention(q, k, x(5, 2), i32(2))
+    with pytest.raises(TypeError):
+        prompt_attention(q, k.bfloat16(), k, i32(2))
+    with pytest.raises(ValueError):
+        prompt_attention(q, k, k, i32(2), i32(3))
+    with pytest.raises(TypeError):
+        prompt_attention(q, k, k, i32(2).long())
+    with pytest.raises(_lib.InnerqError):
+        prompt_attention(x(4, 3), k, k, i32(2))
+    with pytest.raises(TypeError):
+        prompt_attention(q.float(), k.float(), k.float(), i32(2))
+
+
+def test_nothing_to_do():
+    """No sequences, no tokens."""
+    from innerq_b200.paged import PagedCache
+    from innerq_b200.prompt import prompt_attention
+    c = PagedCache.allocate(1, 2, 1, 32, 0, 0)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    x = lambda n, h: torch.zeros((n, h, D), dtype=torch.float16, device="cuda")  # noqa: E731
+    assert c.attend(x(0, 4), i32(0, 1), i32(0), i32(0)).shape == (0, 4, D)
+    assert c.append(x(0, 4), x(0, 2), x(0, 2), i32(0, 1), i32(0), i32(0)).shape == (0, 4, D)
+    k, v = c.read(i32(0, 1), i32(0), i32(0), i32(0), i32(1), 0)
+    assert k.shape == v.shape == (0, 2, D)
+    assert prompt_attention(x(0, 4), x(0, 2), x(0, 2), i32(1)).shape == (0, 4, D)
+    # queries without any keys in the whole call
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    assert torch.equal(prompt_attention(x(3, 4) + 1, x(0, 2), x(0, 2), cu, i32(2)), x(3, 4))
+    # a sequence whose page table has no columns: only the 16-bit rows count
+    kv = torch.ones((1, 2, D), dtype=torch.float16, device="cuda")
+    c.append(None, kv, kv, i32(1, 0), i32(1), i32(1))
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    assert torch.equal(c.attend(x(1, 4), i32(1, 0), i32(1), one), x(1, 4) + 1)
