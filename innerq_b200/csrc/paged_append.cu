@@ -327,7 +327,7 @@ __device__ __forceinline__ void rotate_batch(const Angles& g, int d0, int d1, co
 template <int DT>
 __device__ __forceinline__ void rotate_rows(const Angles& g, int d0, int d1, const uint16_t* src, int64_t src_sh, uint16_t* dst,
                                             int64_t dst_sh, int heads, int h0, int step) {
-  constexpr int kBatch = 4;
+  constexpr int kBatch = 2;
   int left = heads > h0 ? (heads - h0 + step - 1) / step : 0;
   const int64_t ss = step * src_sh, ds = step * dst_sh;
   src += h0 * src_sh;
@@ -352,8 +352,10 @@ __device__ __forceinline__ void rotate_token(const NewDev& n, int Hkv, int tok, 
 }
 
 // the row that a token of the sink or the window gets in its slot
+// (wait: the first head's loads come before the grid's predecessor is waited for)
 template <int DT>
-__device__ __forceinline__ void keep_token(const PagedDev& c, const NewDev& n, int tok, int b, int pos, int row, int h0, int step) {
+__device__ __forceinline__ void keep_token(const PagedDev& c, const NewDev& n, int tok, int b, int pos, int row, int h0, int step,
+                                           bool wait) {
   const int u = threadIdx.x & 7;
   int d0, d1;
   unit_chunks(n, u, d0, d1);
@@ -365,6 +367,10 @@ __device__ __forceinline__ void keep_token(const PagedDev& c, const NewDev& n, i
     uint4 x = *reinterpret_cast<const uint4*>(p + d0), y = *reinterpret_cast<const uint4*>(p + d1);
     const uint4 v0 = *reinterpret_cast<const uint4*>(r + d0), v1 = *reinterpret_cast<const uint4*>(r + d1);
     rotate_unit<DT>(g, x, y);
+    if (wait && h == h0) {
+      griddep_wait();
+      griddep_launch_dependents();
+    }
     const int64_t at = c.dense_base(b, h);
     if (at < 0) return;
     uint16_t* k = c.dk + at + (int64_t)row * kD;
@@ -383,24 +389,30 @@ constexpr int kTokenHeads = kAppendThreads / 8 / kTokens;  // heads that its thr
 // packing; 2: prompts, the sink's and the window's rows (after the packing,
 // which may read what they overwrite)
 template <int DT, int ROLE>
-__global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(PagedDev c, NewDev n, int n_pack, int split) {
-  griddep_wait();
-  griddep_launch_dependents();
+__global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(PagedDev c, NewDev n, int n_pack, int split) {
   const int blk = blockIdx.x, parts = (c.Hkv + kPackHeads - 1) / kPackHeads;
   if (ROLE == 2) {
+    // Up to the wait this reads only what earlier kernels than its predecessor
+    // (role 1) wrote, and they are complete: role 1 lets this grid start after
+    // its own wait.
     const int groups = (c.dense_rows() + kTokens - 1) / kTokens, b = blk / groups;
-    const int row = blk % groups * kTokens + ((threadIdx.x >> 3) & (kTokens - 1));
+    const int row = blk % groups * kTokens + ((threadIdx.x >> 3) & (kTokens - 1)), h0 = threadIdx.x / (8 * kTokens);
     const int len0 = c.lens[b], cu0 = n.cu[b], after = len0 + min(n.cu[b + 1], n.T) - cu0;
-    if (len0 < 0 || cu0 < 0 || row >= c.dense_rows()) return;
     // the position whose row this is: of the window's the one at or after its first
     const int np = c.n_packed(after), j = row - c.w_sink;
     int place = (j - np) % c.ring();
     if (place < 0) place += c.ring();
     const int pos = j < 0 ? row : c.w_sink + np + place;
-    if (pos < len0 || pos >= after) return;
-    keep_token<DT>(c, n, cu0 + pos - len0, b, pos, row, threadIdx.x / (8 * kTokens), kTokenHeads);
+    if (len0 >= 0 && cu0 >= 0 && row < c.dense_rows() && pos >= len0 && pos < after && h0 < c.Hkv) {
+      keep_token<DT>(c, n, cu0 + pos - len0, b, pos, row, h0, kTokenHeads, true);
+    } else {
+      griddep_wait();
+      griddep_launch_dependents();
+    }
     return;
   }
+  griddep_wait();
+  griddep_launch_dependents();
   // packing (bound by instructions) and rotation (by memory) blocks alternate
   const int packs = (int)((int64_t)blk * n_pack / gridDim.x);
   if ((int)((int64_t)(blk + 1) * n_pack / gridDim.x) > packs) {
@@ -413,7 +425,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(PagedDev c, N
     if (len0 < 0) return;
     const int h0 = (threadIdx.x >> 3) + rest % split * rows;
     rotate_token<DT>(n, c.Hkv, tok, len0, h0, rows * split);
-    keep_token<DT>(c, n, tok, tok, len0, c.row_of(len0), h0, rows * split);
+    keep_token<DT>(c, n, tok, tok, len0, c.row_of(len0), h0, rows * split, false);
     return;
   }
   __shared__ int sb;
