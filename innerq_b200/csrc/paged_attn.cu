@@ -147,23 +147,23 @@ struct State {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = NAN;
   }
-  // the largest logits of a tile x[row pair][..] f (f >= 0) per column
+  // this lane's largest logits of a tile x[row pair][..] f (f >= 0) per column
   __device__ __forceinline__ void largest(const float x[2][4], float f0, float f1, float& t0, float& t1) const {
-    t0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2]));
-    t1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3]));
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, o));
-      t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, o));
-    }
-    t0 *= f0;
-    t1 *= f1;
+    t0 = fmaxf(fmaxf(x[0][0], x[0][2]), fmaxf(x[1][0], x[1][2])) * f0;
+    t1 = fmaxf(fmaxf(x[0][1], x[0][3]), fmaxf(x[1][1], x[1][3])) * f1;
   }
+  // No lane's logits lie more than the slack above the running maximum.  The
+  // maximum over the lanes is only taken where this fails.
   __device__ __forceinline__ bool fits(float t0, float t1) const {
     return !__any_sync(~0u, t0 > m[0] + kSlack || t1 > m[1] + kSlack);
   }
   // raise the running maxima and rescale
   __device__ __forceinline__ void raise(float t0, float t1) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, o));
+      t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, o));
+    }
     const float n0 = fmaxf(m[0], t0), n1 = fmaxf(m[1], t1), c0 = ex2(m[0] - n0), c1 = ex2(m[1] - n1);
     m[0] = n0;
     m[1] = n1;
