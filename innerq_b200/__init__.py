@@ -7,6 +7,12 @@ Drop-in modules mirroring the reference package ``innerq`` (mthcom/innerq):
 * ``innerq_b200.models`` — ``src/innerq/models`` (Llama / Mistral hooks plus the
   ``"innerq"`` attention function that reads the packed cache directly)
 
+Beyond the reference, for serving sequences of different lengths:
+
+* ``innerq_b200.paged``  — a paged 4-bit cache: append with rotation, read-back,
+  ragged decode attention
+* ``innerq_b200.prompt`` — causal attention over prompts packed one behind the other
+
 Compute runs in ``libinnerq_b200.so`` (hand-written CUDA for sm_100a, C ABI in
 ``include/innerq_b200.h``); there is no CPU fallback.
 """

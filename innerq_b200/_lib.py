@@ -144,7 +144,7 @@ KERNELS_PER_CALL = {
     "innerq_dequant_ref": 1, "innerq_decode_attn": 3, "innerq_decode_attn_partials": 2,
     "innerq_lse_merge": 1, "innerq_decode_attn_noalloc": 3, "innerq_append_step": 1,
     "innerq_lse_merge_ranks": 1, "innerq_paged_append": 1, "innerq_paged_read": 1,
-    "innerq_paged_attn": 1, "innerq_prompt_attn": 1,
+    "innerq_paged_attn": 2, "innerq_prompt_attn": 1,
 }
 launch_count = [0]
 
