@@ -138,6 +138,25 @@ def load() -> C.CDLL:
     return lib
 
 
+_host = None
+
+
+def host():
+    """The host module of the paged cache and of prompt attention
+    (csrc/host.cpp), bound to the library; raises loudly when it has not been
+    built."""
+    global _host
+    if _host is None:
+        load()
+        try:
+            from . import _host as m
+        except ImportError as e:
+            raise ImportError(f"innerq_b200/_host.so: {e}; build it with `python -m innerq_b200.build`") from e
+        m.bind(LIB_PATH)
+        _host = m
+    return _host
+
+
 # kernels each compute entry point launches (for launch accounting in bench.py)
 KERNELS_PER_CALL = {
     "innerq_norm_factor": 1, "innerq_quant_pack": 1, "innerq_unpack_ref": 1, "innerq_dequant": 1,

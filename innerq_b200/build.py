@@ -1,4 +1,5 @@
-"""Build libinnerq_b200.so in-tree with nvcc for sm_100a.
+"""Build libinnerq_b200.so in-tree with nvcc for sm_100a, and the host module
+_host.so (csrc/host.cpp, over torch's C++ tensors) with g++.
 
     python -m innerq_b200.build [--force] [-j N]
 
@@ -12,16 +13,19 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libinnerq_b200.so")
+HOST = os.path.join(PKG, "_host.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -55,12 +59,30 @@ def _compile(src: str, force: bool) -> str:
     return obj
 
 
+def _build_host(force: bool) -> None:
+    src = os.path.join(CSRC, "host.cpp")
+    newest = max(os.path.getmtime(p) for p in (src, os.path.join(ROOT, "include", "innerq_b200.h")))
+    if not force and os.path.exists(HOST) and os.path.getmtime(HOST) >= newest:
+        return
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-I", os.path.join(torch, "include"), "-I", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"], src, "-o", HOST,
+           "-L", os.path.join(torch, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src}:\n{r.stderr}")
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = True) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     jobs = jobs or max(1, min(len(srcs), os.cpu_count() or 1))
-    with cf.ThreadPoolExecutor(jobs) as ex:
+    with cf.ThreadPoolExecutor(jobs + 1) as ex:
+        host = ex.submit(_build_host, force)
         objs = list(ex.map(lambda s: _compile(s, force), srcs))
+        host.result()
     newest_obj = max(os.path.getmtime(o) for o in objs)
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < newest_obj:
         cmd = [nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", LIB, *objs,
