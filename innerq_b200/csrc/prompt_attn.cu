@@ -8,8 +8,9 @@
 // the inputs' type for the second product (its sum l is not); everything else
 // is fp32.
 //
-// A CTA owns 256 queries of one head as two tiles of 128, so that one tile's
-// softmax runs while the tensor core works for the other:
+// A piece of work is two query tiles of 128 rows, a row being one token's query
+// of one of the heads that share their keys; one tile's softmax runs while the
+// tensor core works for the other:
 //   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per query row (no
 //                   shuffles); rescaling and the epilogue too
 //   warp 8          issues every MMA: S_i = Q_i K^T from shared memory, then
@@ -42,8 +43,7 @@
 namespace innerq {
 namespace {
 
-constexpr int kRows = 128;               // queries of a tile, keys of a tile
-constexpr int kPair = 2 * kRows;         // queries of a CTA
+constexpr int kRows = 128;               // rows of a query tile, keys of a key tile
 constexpr int kHalfTile = kRows * 128;   // bytes of 64 channels of a tile
 constexpr int kTileBytes = 2 * kHalfTile;
 constexpr int kRing = 5;                 // K and V tiles in flight
@@ -72,10 +72,11 @@ struct PromptDev {
   float scale_log2;  // > 0; `negate` holds the sign
   int negate;
   int B, Hq, Hkv, Tq, Tk, causal, slots;
+  int pack, tokens, groups;  // query heads of a row's token, tokens of a tile, groups of heads
 };
 
-// One piece of work: 256 queries of one head of one sequence, and how many key
-// tiles each of its two query tiles needs (n0 < 0: there is no more work).
+// One piece of work: two query tiles of one sequence and group of heads, and how
+// many key tiles each needs (n0 < 0: there is no more work).
 struct Work {
   int head, q_base, nq, k_base, nk, q0, n0, n1;
   int cut;    // from this key tile on, some row must not see all of a tile
@@ -166,13 +167,13 @@ template <int DT> __device__ __forceinline__ bool not_finite(uint32_t h) {
 // The work of block `block` (the last queries of a sequence see the most keys:
 // heavy blocks first); one warp.  False: none, the grid is an upper bound.
 __device__ __forceinline__ bool decode(const PromptDev& a, int block, int lane, Work& w) {
-  const int slot = a.slots - 1 - block / a.Hq;
-  w.head = block % a.Hq;
-  // slots of sequence b start at cu_q[b] / 256 + b: room for its pairs of tiles
+  const int slot = a.slots - 1 - block / a.groups, pair = 2 * a.tokens;
+  w.head = block % a.groups * a.pack;
+  // slots of sequence b start at cu_q[b] / pair + b: room for its pairs of tiles
   int found = -1;
   for (int b = lane; b < a.B; b += 32) {
     const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
-    if (lo >= 0 && lo / kPair + b <= slot && slot < lo / kPair + b + (hi - lo + kPair - 1) / kPair) found = b;
+    if (lo >= 0 && lo / pair + b <= slot && slot < lo / pair + b + (hi - lo + pair - 1) / pair) found = b;
   }
   const int b = __reduce_max_sync(~0u, found);
   if (b < 0) return false;
@@ -180,17 +181,17 @@ __device__ __forceinline__ bool decode(const PromptDev& a, int block, int lane, 
   w.nq = min(a.cu_q[b + 1], a.Tq) - w.q_base;
   w.k_base = max(0, a.cu_k[b]);
   w.nk = max(0, min(a.cu_k[b + 1], a.Tk) - w.k_base);
-  w.q0 = (slot - (w.q_base / kPair + b)) * kPair;
+  w.q0 = (slot - (w.q_base / pair + b)) * pair;
   if (w.q0 >= w.nq) return false;
   int n[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int first = w.q0 + i * kRows, last = min(first + kRows, w.nq) - 1;
+    const int first = w.q0 + i * a.tokens, last = min(first + a.tokens, w.nq) - 1;
     n[i] = ((first < w.nq ? max(0, w.limit(last, a.causal)) : 0) + kRows - 1) / kRows;
   }
   w.n0 = n[0];
   w.n1 = n[1];
-  w.cut = max(0, w.limit(w.q0 + (n[0] > 0 ? 0 : kRows), a.causal)) / kRows;
+  w.cut = max(0, w.limit(w.q0 + (n[0] > 0 ? 0 : a.tokens), a.causal)) / kRows;
   w.dirty = 0;
   return true;
 }
@@ -296,9 +297,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         ++q_count;
         if (lane == 0) {
-          mbar_arrive_tx(&sm.q_full, tiles * kTileBytes);
+          mbar_arrive_tx(&sm.q_full, tiles * a.tokens * a.pack * 256);
           for (int i = 0; i < tiles; ++i)
-            for (int h = 0; h < 2; ++h) tma_load_3d(sm.q[i] + h * kHalfTile, &mq, 64 * h, head, q_row + i * kRows, &sm.q_full);
+            for (int h = 0; h < 2; ++h) tma_load_3d(sm.q[i] + h * kHalfTile, &mq, 64 * h, head, q_row + i * a.tokens, &sm.q_full);
         }
         for (int it = 0; ok && it < 2 * n; ++it) {
           if (filled == kRing)
@@ -496,15 +497,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;\n");
     // ------------------------------------------------------------- softmax
-    const int i = warp >> 2, row = tid & 127;
+    const int i = warp >> 2, row = tid & 127, tok = row / a.pack, sub = row % a.pack;  // row: token, then head
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 lanes per warp
     const uint32_t ts = tmem + i * 128 + lanes, to = tmem + 256 + i * 128 + lanes;
     const uint64_t scale = f2(a.scale_log2, a.scale_log2);
     Pieces pieces(sm);
     uint32_t s_par = 0, o_par = 0;
     while (Work* w = pieces.next()) {
-      const int first = w->q0 + i * kRows, n = i ? w->n1 : w->n0, qi = first + row;
-      const int lim = w->limit(qi, a.causal);
+      const int first = w->q0 + i * a.tokens, n = i ? w->n1 : w->n0, qi = first + tok;
+      const bool real = tok < a.tokens && qi < w->nq;
+      const int lim = real ? w->limit(qi, a.causal) : 0x7fffffff, head = w->head + sub;
       float m = kNoMax, l = 0.f;
       bool ok = true;
 #pragma unroll 1
@@ -597,13 +599,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
         }
         const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
-        uint16_t* out = a.out + (int64_t)(w->q_base + qi) * a.o_st + w->head * a.o_sh;
-        write_row<DT>(to, n > 0, inv, qi < w->nq ? out : nullptr);
+        uint16_t* out = a.out + (int64_t)(w->q_base + qi) * a.o_st + head * a.o_sh;
+        write_row<DT>(to, n > 0, inv, real ? out : nullptr);
         tc_fence_before();
-        if (ok && *(volatile int*)&w->dirty && qi < w->nq) {
+        if (ok && *(volatile int*)&w->dirty && real) {
           // values that were set to 0 and that this row does see
-          const int kv_head = w->head / (a.Hq / a.Hkv);
-          const uint16_t* qr = a.q + (int64_t)(w->q_base + qi) * a.q_st + w->head * a.q_sh;
+          const int kv_head = head / (a.Hq / a.Hkv);
+          const uint16_t* qr = a.q + (int64_t)(w->q_base + qi) * a.q_st + head * a.q_sh;
           for (int key = kRows * w->cut; key < min(kRows * n, lim); ++key) {
             const uint16_t* vr = a.v + (int64_t)(w->k_base + key) * a.v_st + kv_head * a.v_sh;
             float p = -1.f;
@@ -619,8 +621,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (a.lse && qi < w->nq)
-          a.lse[(int64_t)(w->q_base + qi) * a.Hq + w->head] = l == 0.f ? -INFINITY : m - kShift + log2f(l);
+        if (a.lse && real)
+          a.lse[(int64_t)(w->q_base + qi) * a.Hq + head] = l == 0.f ? -INFINITY : m - kShift + log2f(l);
       }
       if (!ok) break;
       pieces.done(lane);
@@ -649,14 +651,14 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-// boxes of 128 tokens x 64 channels of one head of [T][H][128]
-bool encode(CUtensorMap* m, const void* base, int dtype, int H, int T, int64_t sh, int64_t st) {
+// boxes of `tokens` tokens x `heads` heads x 64 channels of [T][H][128]
+bool encode(CUtensorMap* m, const void* base, int dtype, int H, int T, int64_t sh, int64_t st, int heads, int tokens) {
   const EncodeFn fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)kD, (cuuint64_t)H, (cuuint64_t)T};
   // a dimension of one element has no stride of its own
   const cuuint64_t strides[2] = {(cuuint64_t)(H > 1 ? sh : kD) * 2, (cuuint64_t)(T > 1 ? st : kD) * 2};
-  const cuuint32_t box[3] = {64, 1, kRows}, one[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, (cuuint32_t)heads, (cuuint32_t)tokens}, one[3] = {1, 1, 1};
   return fn(m, dtype == INNERQ_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
             const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -675,7 +677,7 @@ cudaError_t launch_prompt(const CUtensorMap& mq, const CUtensorMap& mk, const CU
     if (e != cudaSuccess) return e;
     if (dev < 64) ready[dev] = true;
   }
-  return launch_pdl(prompt_kernel<DT>, dim3((unsigned)a.slots * a.Hq), dim3(kThreads), smem, s, mq, mk, mv, a);
+  return launch_pdl(prompt_kernel<DT>, dim3((unsigned)a.slots * a.groups), dim3(kThreads), smem, s, mq, mk, mv, a);
 }
 
 }  // namespace
@@ -710,13 +712,19 @@ extern "C" int innerq_prompt_attn(const innerq_prompt_args* p, void* stream) {
   a.scale_log2 = std::max(1e-37f, (p->scale < 0 ? -p->scale : p->scale) * 1.4426950408889634f);
   a.negate = p->scale < 0;
   a.B = p->B; a.Hq = p->Hq; a.Hkv = p->Hkv; a.Tq = p->Tq; a.Tk = p->Tk; a.causal = p->causal;
-  a.slots = p->Tq / kPair + p->B;
-  if ((int64_t)a.slots * a.Hq > 0x7fffffff) return set_last_error(INNERQ_ERR_ARG, "too many blocks for one launch");
+  // The rows of a query tile are tokens times the query heads that share their
+  // keys, so short prompts fill tiles too.
+  const int ratio = p->Hq / p->Hkv;
+  a.pack = ratio <= 32 ? ratio : 1;
+  a.tokens = kRows / a.pack;
+  a.groups = p->Hq / a.pack;
+  a.slots = p->Tq / (2 * a.tokens) + p->B;
+  if ((int64_t)a.slots * a.groups > 0x7fffffff) return set_last_error(INNERQ_ERR_ARG, "too many blocks for one launch");
   CUtensorMap mq, mk, mv;
   const bool none = p->Tk == 0;  // no keys: the maps are never used
-  if (!encode(&mq, p->q, p->dtype, p->Hq, p->Tq, p->q_sh, p->q_st) ||
-      !encode(&mk, none ? p->q : p->k, p->dtype, none ? 1 : p->Hkv, none ? 1 : p->Tk, p->k_sh, p->k_st) ||
-      !encode(&mv, none ? p->q : p->v, p->dtype, none ? 1 : p->Hkv, none ? 1 : p->Tk, p->v_sh, p->v_st))
+  if (!encode(&mq, p->q, p->dtype, p->Hq, p->Tq, p->q_sh, p->q_st, a.pack, a.tokens) ||
+      !encode(&mk, none ? p->q : p->k, p->dtype, none ? 1 : p->Hkv, none ? 1 : p->Tk, p->k_sh, p->k_st, 1, kRows) ||
+      !encode(&mv, none ? p->q : p->v, p->dtype, none ? 1 : p->Hkv, none ? 1 : p->Tk, p->v_sh, p->v_st, 1, kRows))
     return set_last_error(INNERQ_ERR_ARG, "q, k and v: strides or sizes that a tensor map cannot describe");
   const cudaStream_t s = (cudaStream_t)stream;
   const cudaError_t e = p->dtype == INNERQ_DT_BF16 ? launch_prompt<BF16>(mq, mk, mv, a, s) : launch_prompt<F16>(mq, mk, mv, a, s);
