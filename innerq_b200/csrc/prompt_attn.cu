@@ -219,9 +219,36 @@ struct Pieces {
   }
 };
 
-// the finished row of this thread: O / l, or zeros where there is no O
+// Four lanes swap 16-byte pieces w[0..3] so that lane k ends with piece k of
+// the rows of all four: a 4 x 4 transpose in two exchanges.
+__device__ __forceinline__ void transpose4(uint4 w[4], int lane) {
+#pragma unroll
+  for (int bit = 1; bit <= 2; bit <<= 1) {
+    const bool up = lane & bit;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      uint32_t* lo = reinterpret_cast<uint32_t*>(&w[bit == 1 ? 2 * x : x]);
+      uint32_t* hi = reinterpret_cast<uint32_t*>(&w[bit == 1 ? 2 * x + 1 : x + 2]);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t got = __shfl_xor_sync(~0u, up ? lo[y] : hi[y], bit);
+        if (up)
+          lo[y] = got;
+        else
+          hi[y] = got;
+      }
+    }
+  }
+}
+
+// The finished rows of a warp, one per thread: O / l, or zeros where there is
+// no O.  Four lanes write 64 contiguous bytes of a row (a thread on its own
+// would spread every store over 32 rows: 2.5 us per piece of work).
 template <int DT>
-__device__ __forceinline__ void write_row(uint32_t to, bool any, float inv, uint16_t* out) {
+__device__ __forceinline__ void write_rows(uint32_t to, bool any, float inv, uint16_t* out, int lane) {
+  uint64_t row[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) row[x] = __shfl_sync(~0u, (unsigned long long)out, (lane & ~3) + x);
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     float o[32];
@@ -232,14 +259,17 @@ __device__ __forceinline__ void write_row(uint32_t to, bool any, float inv, uint
 #pragma unroll
       for (int x = 0; x < 32; ++x) o[x] = 0.f;
     }
+    uint4 w[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      uint4 v;
-      uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+      uint32_t* e = reinterpret_cast<uint32_t*>(&w[x]);
 #pragma unroll
       for (int y = 0; y < 4; ++y) e[y] = inv == 0.f ? 0u : pack_p<DT>(o[8 * x + 2 * y] * inv, o[8 * x + 2 * y + 1] * inv);
-      if (out) *reinterpret_cast<uint4*>(out + 32 * c + 8 * x) = v;
     }
+    transpose4(w, lane);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (row[x]) reinterpret_cast<uint4*>(row[x])[4 * c + (lane & 3)] = w[x];
   }
 }
 
@@ -600,10 +630,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
         uint16_t* out = a.out + (int64_t)(w->q_base + qi) * a.o_st + head * a.o_sh;
-        write_row<DT>(to, n > 0, inv, real ? out : nullptr);
+        write_rows<DT>(to, n > 0, inv, real ? out : nullptr, lane);
         tc_fence_before();
+        __syncwarp();
         if (ok && *(volatile int*)&w->dirty && real) {
-          // values that were set to 0 and that this row does see
+          // values that were set to 0 and that this row does see (the row was
+          // written by this warp's lanes: made visible by the warp barrier)
           const int kv_head = head / (a.Hq / a.Hkv);
           const uint16_t* qr = a.q + (int64_t)(w->q_base + qi) * a.q_st + head * a.q_sh;
           for (int key = kRows * w->cut; key < min(kRows * n, lim); ++key) {
