@@ -170,17 +170,19 @@ __device__ __forceinline__ bool decode(const PromptDev& a, int block, int lane, 
   const int slot = a.slots - 1 - block / a.groups, pair = 2 * a.tokens;
   w.head = block % a.groups * a.pack;
   // slots of sequence b start at cu_q[b] / pair + b: room for its pairs of tiles
-  int found = -1;
-  for (int b = lane; b < a.B; b += 32) {
-    const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
-    if (lo >= 0 && lo / pair + b <= slot && slot < lo / pair + b + (hi - lo + pair - 1) / pair) found = b;
+  int b = -1, lo = 0, hi = 0, k_lo = 0, k_hi = 0;
+  for (int i = lane; i < a.B; i += 32) {
+    const int x = a.cu_q[i], y = a.cu_q[i + 1], kx = a.cu_k[i], ky = a.cu_k[i + 1];
+    if (x >= 0 && x / pair + i <= slot && slot < x / pair + i + (y - x + pair - 1) / pair) b = i, lo = x, hi = y, k_lo = kx, k_hi = ky;
   }
-  const int b = __reduce_max_sync(~0u, found);
-  if (b < 0) return false;
-  w.q_base = a.cu_q[b];
-  w.nq = min(a.cu_q[b + 1], a.Tq) - w.q_base;
-  w.k_base = max(0, a.cu_k[b]);
-  w.nk = max(0, min(a.cu_k[b + 1], a.Tk) - w.k_base);
+  const uint32_t who = __ballot_sync(~0u, b >= 0);
+  if (!who) return false;
+  const int src = __ffs(who) - 1;
+  b = __shfl_sync(~0u, b, src);
+  w.q_base = __shfl_sync(~0u, lo, src);
+  w.nq = min(__shfl_sync(~0u, hi, src), a.Tq) - w.q_base;
+  w.k_base = max(0, __shfl_sync(~0u, k_lo, src));
+  w.nk = max(0, min(__shfl_sync(~0u, k_hi, src), a.Tk) - w.k_base);
   w.q0 = (slot - (w.q_base / pair + b)) * pair;
   if (w.q0 >= w.nq) return false;
   int n[2];
@@ -301,6 +303,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sm.o_full[i], 1);
     }
     mbar_fence_init();
+  }
+  if (tid == 9 * 32) {
+    tma_prefetch(&mq);
+    tma_prefetch(&mk);
+    tma_prefetch(&mv);
   }
   if (warp == 8) tmem_alloc(&sm.tmem, 512);
   tc_fence_before();
