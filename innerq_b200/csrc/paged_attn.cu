@@ -421,35 +421,21 @@ __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* v
   }
 }
 
-__device__ __forceinline__ int tiles_of(const PagedDev& c, int b, int cap) {
-  const int len = c.lens[b];
-  return len <= 0 ? 0 : min((int)(((int64_t)len + 31) >> 5), cap);
-}
+__device__ __forceinline__ int tiles_in(int len, int cap) { return len <= 0 ? 0 : min((int)(((int64_t)len + 31) >> 5), cap); }
+__device__ __forceinline__ int tiles_of(const PagedDev& c, int b, int cap) { return tiles_in(c.lens[b], cap); }
 
 // length of a unit of nt tiles in the list: a unit takes time beyond its tiles
 // (its query, its first loads, the join), so it is followed by kUnitCost
 // places that hold no tile
 __device__ __forceinline__ int places_of(int nt) { return nt ? nt + kUnitCost : 0; }
 
-// inclusive scan over the block
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(~0u, v, o);
     if (lane >= o) v += x;
   }
-  if (lane == 31) warp_sums[w] = v;
-  __syncthreads();
-  int add = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < w) add += warp_sums[i];
-    total += warp_sums[i];
-  }
-  __syncthreads();
-  return v + add;
+  return v;
 }
 
 template <int RH>
@@ -460,8 +446,6 @@ struct alignas(128) Smem {
   uint64_t bars[kWarps][kStages];
   int4 put[kWarps];
   int bad[kWarps];
-  int sums[kWarps];
-  int unit_b, unit_start, unit_tiles;
 };
 
 // tiles per CTA: equal ranges, whole rounds of the four warps
@@ -482,37 +466,40 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
   griddep_wait();
   griddep_launch_dependents();
 
-  // the list of tiles: where this CTA's range begins
+  // the list of tiles: where this CTA's range begins (every warp for itself)
+  auto length = [&](int b) { return b < c.B ? c.lens[b] : 0; };
+  auto places = [&](int len) { return places_of(tiles_in(len, a.cap)) * c.Hkv; };
   int total = 0;
-  for (int b0 = 0; b0 < c.B; b0 += 128) {
-    int sum;
-    block_scan(b0 + tid < c.B ? places_of(tiles_of(c, b0 + tid, a.cap)) * c.Hkv : 0, sm.sums, sum);
-    total += sum;
-  }
+  for (int b0 = 0; b0 < c.B; b0 += 32) total += __reduce_add_sync(~0u, places(length(b0 + lane)));
   const int per = range_of(total, gridDim.x);
   const int lo = blockIdx.x * per, hi = min(total, lo + per);
-  if (blockIdx.x == 0 || lo < total) {
-    for (int b0 = 0, at = 0; b0 < c.B; b0 += 128) {
-      int sum;
-      const int n = b0 + tid < c.B ? tiles_of(c, b0 + tid, a.cap) : 0;
-      const int places = places_of(n) * c.Hkv, end = at + block_scan(places, sm.sums, sum), start = end - places;
-      if (n > 0 && start <= lo && lo < end) {
-        sm.unit_b = b0 + tid;
-        sm.unit_start = start;
-        sm.unit_tiles = n;
-      }
-      if (blockIdx.x == 0 && b0 + tid < c.B) a.starts[b0 + tid] = start;
-      at += sum;
+  if (blockIdx.x == 0 && w == 0) {  // for merge_kernel
+    for (int b0 = 0, at = 0; b0 < c.B; b0 += 32) {
+      const int v = places(length(b0 + lane)), end = at + warp_scan(v, lane);
+      if (b0 + lane < c.B) a.starts[b0 + lane] = end - v;
+      at = __shfl_sync(~0u, end, 31);
     }
-    if (blockIdx.x == 0 && tid == 0) a.starts[c.B] = total;
+    if (lane == 0) a.starts[c.B] = total;
   }
   if (lo >= total) return;
-  __syncthreads();
-  int b = sm.unit_b, nt = sm.unit_tiles;
-  int h = (lo - sm.unit_start) / places_of(nt);
-  int u0 = sm.unit_start + h * places_of(nt);
+  int b = 0, nt = 0, u0 = 0, packed = 0;
+  for (int b0 = 0, at = 0;; b0 += 32) {
+    const int len = length(b0 + lane), v = places(len), sum = __reduce_add_sync(~0u, v);
+    if (lo < at + sum) {
+      const int end = at + warp_scan(v, lane);
+      const int src = __ffs(__ballot_sync(~0u, lo < end)) - 1;
+      b = b0 + src;
+      u0 = __shfl_sync(~0u, end - v, src);
+      const int l = __shfl_sync(~0u, len, src);
+      nt = tiles_in(l, a.cap);
+      packed = c.n_packed(l) >> 5;
+      break;
+    }
+    at += sum;
+  }
+  int h = (lo - u0) / places_of(nt);
+  u0 += h * places_of(nt);
   const int sink_tiles = c.w_sink >> 5;
-  int packed = c.n_packed(c.lens[b]) >> 5;
   // the unit after (b, h); false when it begins outside the range
   auto advance = [&]() {
     u0 += places_of(nt);
