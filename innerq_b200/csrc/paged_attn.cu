@@ -1,5 +1,5 @@
 // Decode attention over the paged 4-bit cache: one query token per sequence, a
-// length per sequence, flash-decoding over 32-token tiles.
+// length per sequence, one pass over 32-token tiles that may be split anywhere.
 //
 // Mathematics.  A 4-bit code u (0..15, offset 8) placed in the mantissa of a
 // 16-bit word IS the fp16 subnormal u 2^-24 (16 u 2^-24 four bits higher), so
@@ -10,10 +10,11 @@
 // 8 query heads) with fp32 accumulators that start at the offset term; group
 // scales are applied in fp32.  The query is scaled per head by a power of two
 // into [2^14, 2^15), exact in fp16 for both dtypes; the slots whose codes sit
-// four bits higher take q / 16 and p / 16.  A probability is 2^15 p rounded to
-// fp16 (11 bits down to 2^-29 of the tile's largest), the one rounding of the
-// 4-bit path, and the sum that divides the result is taken over the rounded
-// values by an MMA against ones.  16-bit tokens (sink, window) use the same
+// four bits higher take q / 16 and p / 16.  A probability is 2^8 p, relative to a
+// running maximum that may lag by 2^7, rounded to fp16 (11 bits down to 2^-22):
+// the one rounding of the 4-bit path, and what an fp16 operand takes; with fp16
+// inputs it adds as much error again as rounding the output does.  The sum that
+// divides the result is taken over the rounded values by an MMA against ones.  16-bit tokens (sink, window) use the same
 // MMAs on their own type; bf16 probabilities are split into two parts there.
 //
 // Work.  The tiles of all (sequence, head) units form one list that is cut

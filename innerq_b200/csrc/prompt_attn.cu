@@ -1,7 +1,7 @@
 // Attention of whole prompts packed one behind the other, on the tensor cores
 // (tcgen05).
 //
-// Mathematics.  Flash attention: over key tiles of 128, S = Q K^T, running row
+// Mathematics.  One pass over key tiles of 128: S = Q K^T, running row
 // maximum m and sum l, P = 2^(S scale log2 e - m), O += P V.  m may lag behind
 // the true maximum by 2^8 before O is rescaled, so rescaling is rare; P carries
 // 2^7 so that fp16 keeps 11 bits down to 2^-21 of the largest.  P is rounded to
@@ -52,9 +52,10 @@ constexpr float kShift = 7.f;            // P carries 2^7
 constexpr float kSlack = 8.f;            // lag of the running maximum
 constexpr float kNoMax = -1e30f;
 constexpr uint32_t kWait = 1u << 14;
-// P is handed over in two parts, so that P V starts before P is complete: 454
-// against 466 us in one part, 457 in four (8192 tokens)
-constexpr int kParts = 2;
+// P is handed over in two parts, so that P V starts before P is complete; the
+// first has this many of its four quarters: 508 us with 1, 501 with 2, 497 with
+// 3, some 515 in one part (8192 tokens, sustained)
+constexpr int kParts = 2, kFirstPart = 3;
 // one pair of exponentials of this many goes to the FMA pipe: 472 us of 477
 // without (8192 tokens), 2.25 ms of 2.38 (chunks over 8111 tokens); every
 // second pair is slower again (497 us)
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto values = [&](int i, int st, int part, uint32_t acc) {
         const uint32_t db = v_lo + st * (kTileBytes >> 4);
 #pragma unroll
-        for (int k = part * (8 / kParts); k < (part + 1) * (8 / kParts); ++k)
+        for (int k = part ? 2 * kFirstPart : 0; k < (part ? 8 : 2 * kFirstPart); ++k)
           mma_ts<hi>(leader, tm + 256 + i * 128, tm + i * 128 + 8 * k, db + k * (2048 >> 4), id_o, k > 0 ? 1u : acc);
       };
       // ring slots of K_j / V_j in turn, with the parities of their fillings
@@ -612,11 +613,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               p[x] = pack_p<DT>(p0, p1);
             }
             tmem_st16(ts + 16 * c, p);
-            if ((c + 1) % (4 / kParts) == 0) {
+            if (c == kFirstPart - 1 || c == 3) {
               tmem_wait_st();
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive(&sm.p_ready[i][c / (4 / kParts)]);
+              if (lane == 0) mbar_arrive(&sm.p_ready[i][c == 3]);
             }
           }
         };
