@@ -26,10 +26,13 @@
 // of the next piece of work run under the epilogue of the last; warp 11 asks.
 // What bounds it: per key tile of a pair the four products take 2048 cycles of
 // the tensor core at least, the exponentials about as many of the special
-// function units, and a tile's chain (scores, softmax, P V) some 3200; the two
-// tiles overlap it to 63% tensor occupancy.  One prompt of 8192 tokens, 32
-// heads, bf16: 444 us (1239 TFLOP/s), 505 us back to back at the board's power
-// limit (1.57 GHz); 16 prompts of 1 to 300 tokens: 23 us.
+// function units, and a tile's chain (scores, softmax, P V) some 3200, 2000 of
+// them softmax; two tiles overlap it to 59% tensor occupancy (special functions
+// 45%, issue slots 47%), and without any product the rest alone takes 0.82 of
+// the time.  One prompt of 8192 tokens, 32 heads, bf16: 435 us (1260 TFLOP/s),
+// 497 us back to back at the board's power limit (1.57 GHz); 16 prompts of 1 to
+// 300 tokens: 17 us.  Two warps per 32 rows, each with half of the columns, are
+// slower (485 us: the halves have to meet for every maximum).
 // Tensor memory: S0 | S1 | O0 | O1, 128 columns each.  In-order execution of
 // the MMAs makes "S_i(j + 1) is complete" mean that O_i is at rest too.
 #include <algorithm>
@@ -57,8 +60,8 @@ constexpr uint32_t kWait = 1u << 14;
 // 3, some 515 in one part (8192 tokens, sustained)
 constexpr int kParts = 2, kFirstPart = 3;
 // one pair of exponentials of this many goes to the FMA pipe: 472 us of 477
-// without (8192 tokens), 2.25 ms of 2.38 (chunks over 8111 tokens); every
-// second pair is slower again (497 us)
+// without (8192 tokens, an earlier state of the kernel), 2.25 ms of 2.38
+// (chunks over 8111 tokens); every second pair is slower again (497 us)
 constexpr int kPolyOf = 4;
 
 struct PromptDev {
