@@ -47,7 +47,7 @@ constexpr int kStages = 3;
 constexpr int kCtasPerSm = 3;
 // what a unit costs beyond its tiles, in tiles: 96 sequences of 1 to 20000
 // tokens take 277 us with 0, 123 with 4, 77 with 12, 82 with 24
-constexpr int kUnitCost = 12;
+constexpr int kUnitCost = 16;
 constexpr int kHeadPitch = 148;  // floats per head of the combine buffer: conflict-free
 constexpr float kPScale = 8.f;   // probabilities carry 2^8 relative to the running maximum,
 constexpr float kSlack = 7.f;    // which may lag behind the true one by 2^7 before it is raised
@@ -593,29 +593,47 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
     if (idx < packed_end) {
       Query q;
       load_query<DT>(a, b, h, lane, q);
+      // The logits of a tile are computed next to the values of the one before
+      // it: two independent streams of instructions.
+      float x[2][4];
+      auto logits = [&](int st, float y[2][4]) { packed_logits<DT>(sm.ring[w][st], lane, q, y); };
+      auto settle = [&]() {
+        float t0, t1;
+        s.largest(x, q.f[0], q.f[1], t0, t1);
+        if (!s.fits(t0, t1)) s.raise(t0, t1);
+      };
       failed = failed || !mbar_wait_bounded(&sm.bars[w][st_get], parity, kWaitLimit);
+      if (!failed) {
+        logits(st_get, x);
+        settle();
+      }
 #pragma unroll 1
       while (!failed) {
-        float x[2][4], t0, t1;
-        packed_logits<DT>(sm.ring[w][st_get], lane, q, x);
-        s.largest(x, q.f[0], q.f[1], t0, t1);
-        if (!s.fits(t0, t1)) {  // seldom after the first tile, which is then read again
-          s.raise(t0, t1);
-          continue;
-        }
-        packed_values<DT>(sm.ring[w][st_get], lane, q, x, s);
+        const int st = st_get;
         if (++st_get == kStages) {
           st_get = 0;
           parity ^= 1;
         }
+        idx += kWarps;
+        if (idx >= packed_end) {
+          packed_values<DT>(sm.ring[w][st], lane, q, x, s);
+          __syncwarp();
+          if (lane == 0) --in_flight;
+          break;
+        }
+        failed = !mbar_wait_bounded(&sm.bars[w][st_get], parity, kWaitLimit);
+        if (failed) break;
+        float y[2][4];
+        packed_values<DT>(sm.ring[w][st], lane, q, x, s);
+        logits(st_get, y);
         __syncwarp();
         if (lane == 0) {
           --in_flight;
           issue();
         }
-        idx += kWarps;
-        if (idx >= packed_end) break;
-        failed = !mbar_wait_bounded(&sm.bars[w][st_get], parity, kWaitLimit);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[0][i] = y[0][i], x[1][i] = y[1][i];
+        settle();
       }
       if (failed) s.poison();
     }
