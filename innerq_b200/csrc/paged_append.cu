@@ -15,8 +15,9 @@
 // What bounds it: rotation moves bytes (q in and out), packing is instructions
 // (some 600 per 32 tokens, head and warp: seven exact cuts per group and 7
 // packed compares and adds per pair of values), so their blocks alternate in
-// one launch.  A prompt of 16384 tokens with 40 / 8 heads in bf16, 420 MB: 95 us
-// (4.4 TB/s); one block per token and one per (tile, head) took 140 us.
+// one launch.  A prompt of 16384 tokens with 40 / 8 heads in bf16, 420 MB: 92 us
+// (4.6 TB/s); one block per token and one per (tile, head) took 140 us.  Eight
+// tokens per rotation block: 110 us with the read-back, four 114, sixteen 117.
 // Sharing a group's cuts over its threads took packing from 63 to 50 us,
 // keeping a token's angles over its heads and exact batches of heads took
 // rotation from 95 to 65 us.
@@ -391,7 +392,7 @@ __device__ __forceinline__ void keep_token(const PagedDev& c, const NewDev& n, i
   }
 }
 
-constexpr int kTokens = 4;                                // tokens of a block of prompts: one per quarter warp
+constexpr int kTokens = 8;                                // tokens of a block of prompts, eight threads each at a time
 constexpr int kTokenHeads = kAppendThreads / 8 / kTokens;  // heads that its threads take at once
 
 // role 0: a decode step, one token per sequence; 1: prompts, rotation and

@@ -27,10 +27,11 @@
 // What bounds it: 540 warp instructions per tile of 32 tokens (half of them
 // bit operations that expand codes, 34 MMAs) against 4608 bytes, at 12 warps
 // per SM; issue slots are 55-60% busy and DRAM at 80% of a copy's rate.  32
-// sequences of 32768 tokens, 8 key heads, 1.22 GB: 232 us (5.3 TB/s), 236 to
-// 250 us when run back to back, where the board's power limit lowers the
-// clocks; one sequence of 4096 tokens: 10 us, of which the list takes 1.2, the
-// first copy 0.7, a tile 2, the join 1 and the merge 2.  Three CTAs of 168 registers with rings of
+// sequences of 32768 tokens, 8 key heads, 1.22 GB: 216 us (5.6 TB/s), 245 us
+// when run back to back, where the board's power limit lowers the clocks; one
+// sequence of 4096 tokens: 10 us, of which the list takes 1.2, the first copy
+// 0.7, a tile 2, the join 1 and the merge 2.  Computing a tile's logits next to
+// the values of the tile before it took 224 us to 216.  Three CTAs of 168 registers with rings of
 // three beat four of 128 with rings of two (spills): 232 against 228-245 us,
 // and 73 against 84 us on 96 sequences of 1 to 20000 tokens.
 #include <algorithm>
@@ -46,7 +47,8 @@ constexpr int kWarps = 4;
 constexpr int kStages = 3;
 constexpr int kCtasPerSm = 3;
 // what a unit costs beyond its tiles, in tiles: 96 sequences of 1 to 20000
-// tokens take 277 us with 0, 123 with 4, 77 with 12, 82 with 24
+// tokens take 73.6 us with 12, 69.5 with 16, 71.2 with 24 (an earlier state of
+// the kernel 277 with 0, 123 with 4)
 constexpr int kUnitCost = 16;
 constexpr int kHeadPitch = 148;  // floats per head of the combine buffer: conflict-free
 constexpr float kPScale = 8.f;   // probabilities carry 2^8 relative to the running maximum,

@@ -81,7 +81,7 @@ def test_lengths(n, causal, dtype):
     check(q, k, v, n, n, causal, dtype)
 
 
-@pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 3), (6, 2), (5, 1), (8, 8), (16, 2), (40, 8), (7, 1), (20, 1)])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 3), (6, 2), (5, 1), (8, 8), (16, 2), (40, 8), (7, 1), (20, 1), (32, 1), (33, 1), (64, 1)])
 def test_heads(hq, hkv):
     n = [200, 77]
     q, k, v = data(n, n, hq, hkv, "fp16", seed=hq)
@@ -96,6 +96,17 @@ def test_keys_longer_or_shorter_than_queries(nq, nk, causal):
     that see nothing: zeros."""
     q, k, v = data(nq, nk, 4, 2, "bf16", seed=sum(nq) + sum(nk))
     check(q, k, v, nq, nk, causal, "bf16")
+
+
+def test_many_sequences():
+    """More sequences than a warp, some empty; more pieces of work than CTAs."""
+    r = np.random.RandomState(11)
+    nq = np.where(r.rand(700) < 0.2, 0, r.randint(1, 40, 700)).tolist()
+    q, k, v = data(nq, nq, 4, 2, "fp16", seed=12)
+    check(q, k, v, nq, nq, True, "fp16")
+    nk = [n + int(x) for n, x in zip(nq, r.randint(0, 200, 700))]
+    q, k, v = data(nq, nk, 2, 2, "bf16", seed=13)
+    check(q, k, v, nq, nk, True, "bf16")
 
 
 def test_long():
