@@ -24,7 +24,7 @@
 // tile) and no synchronisation until a unit ends.  A unit inside one range is
 // written at once, the others leave fp32 partials that merge_kernel joins.
 //
-// What bounds it: 540 warp instructions per tile of 32 tokens (half of them
+// What bounds it: 507 warp instructions per tile of 32 tokens (half of them
 // bit operations that expand codes, 34 MMAs) against 4608 bytes, at 12 warps
 // per SM; issue slots are 55-60% busy and DRAM at 80% of a copy's rate.  32
 // sequences of 32768 tokens, 8 key heads, 1.22 GB: 216 us (5.6 TB/s), 245 us
