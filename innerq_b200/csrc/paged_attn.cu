@@ -13,9 +13,17 @@
 // four bits higher take q / 16 and p / 16.  A probability is 2^8 p, relative to a
 // running maximum that may lag by 2^7, rounded to fp16 (11 bits down to 2^-22):
 // the one rounding of the 4-bit path, and what an fp16 operand takes; with fp16
-// inputs it adds as much error again as rounding the output does.  The sum that
-// divides the result is taken over the rounded values by an MMA against ones.  16-bit tokens (sink, window) use the same
-// MMAs on their own type; bf16 probabilities are split into two parts there.
+// inputs it adds as much error again as rounding the output does (a second part
+// for what it leaves takes 216 us to 249 on the case below).  The sum that
+// divides the result is taken over the rounded values by MMAs, against a code of
+// 11: an MMA aligns its products by the operands' nominal exponents, so products
+// with a subnormal are cut off at 2^-16 to 2^-17 of the tile's largest
+// probability, always towards zero.  Over tens of thousands of tokens that adds
+// up along the values' scales (3e-4 of the output, measured), unless 8 sum p
+// loses as much: a random code loses about 0.7 of what an odd one does, and
+// 8 / 11 of the sum against 11 is taken off.  16-bit tokens (sink, window) use
+// the same MMAs on their own type, with ones, and bf16 probabilities are split
+// into two parts there.
 //
 // Work.  The tiles of all (sequence, head) units form one list that is cut
 // into equal ranges, one per resident CTA, so ragged lengths balance without
@@ -54,6 +62,7 @@ constexpr int kHeadPitch = 148;  // floats per head of the combine buffer: confl
 constexpr float kPScale = 8.f;   // probabilities carry 2^8 relative to the running maximum,
 constexpr float kSlack = 7.f;    // which may lag behind the true one by 2^7 before it is raised
 constexpr float kOutScale = 16777216.f;  // what the codes' 2^-24 left in the accumulators
+constexpr uint32_t kSumCode = 11;  // the code against which probabilities are summed
 constexpr float kNoMax = -1e30f; // running maximum before the first logit
 
 struct AttnDev {
@@ -302,14 +311,15 @@ __device__ __forceinline__ void packed_values(const uint8_t* blk, int lane, cons
   }
   float ps[4];
   {
-    const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u};  // 1 and 16
-    mma_from<F16>(ps, ones, pb[0], pb[1], zero);
-    mma_acc<F16>(ps, ones, pb[2], pb[3]);
+    constexpr uint32_t c = kSumCode * 0x10001u;
+    const uint32_t code[4] = {c, c, c << 4, c << 4};
+    mma_from<F16>(ps, code, pb[0], pb[1], zero);
+    mma_acc<F16>(ps, code, pb[2], pb[3]);
   }
-  s.l[0] += ps[0];
-  s.l[1] += ps[1];
+  s.l[0] = fmaf(ps[0], kOutScale / kSumCode, s.l[0]);
+  s.l[1] = fmaf(ps[1], kOutScale / kSumCode, s.l[1]);
   float off[4];
-  quad(off, ps[0] * (-8.f / 16777216.f), ps[1] * (-8.f / 16777216.f));
+  quad(off, ps[0] * (-8.f / kSumCode), ps[1] * (-8.f / kSumCode));
   const uint4 v0 = reinterpret_cast<const uint4*>(blk + kVScale)[2 * gid];
   const uint4 v1 = reinterpret_cast<const uint4*>(blk + kVScale)[2 * gid + 1];
 #pragma unroll

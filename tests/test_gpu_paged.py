@@ -455,3 +455,26 @@ def test_nothing_to_do():
     c.append(None, kv, kv, i32(1, 0), i32(1), i32(1))
     one = torch.ones(1, dtype=torch.int32, device="cuda")
     assert torch.equal(c.attend(x(1, 4), i32(1, 0), i32(1), one), x(1, 4) + 1)
+
+
+@pytest.mark.parametrize("dtype,hq", [("fp16", 8), ("fp16", 5), ("bf16", 8)])
+def test_long_contexts_have_no_error_of_one_sign(dtype, hq):
+    """What a tile's sums lose must not add up over a long context.  Errors of
+    one sign show along the values' sizes: there the rounding of the output and
+    of the probabilities (each at most 2^-11 / sqrt 3 rms for fp16; the
+    output's is 2^-8 / sqrt 3 for bf16) leaves about 1 / sqrt 128 of itself per
+    row.  The limit is four such deviations of the rows' mean, and 1e-4 for
+    what the sums may lose."""
+    s = Server(2, 2, dtype, 32, 96, 128, 33000, seed=21)
+    s.step([33000, 21003])
+    rows = []
+    at = torch.arange(2).cuda()
+    q = torch.randn((2, 2 * hq, D), device="cuda", generator=s.g).to(s.dt)
+    out = s.cache.attend(q, s.table[at], s.slots[at], s.dev(s.lens)).double().cpu().numpy()
+    for b in range(2):
+        want, _ = s.oracle.attend(b, q[b].float().cpu().numpy(), D ** -0.5)
+        for h in range(2 * hq):
+            size = np.abs(s.oracle.cv[b][:, h // hq]).mean(0)
+            rows.append((out[b, h] - want[h]) @ size / np.linalg.norm(size) / np.linalg.norm(want[h]))
+    deviation = math.hypot(ULP[dtype], 2.0 ** -11) / math.sqrt(3 * D)
+    assert abs(np.mean(rows)) < 4 * deviation / math.sqrt(len(rows)) + 1e-4, (np.mean(rows), np.max(np.abs(rows)))
