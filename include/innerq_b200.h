@@ -300,7 +300,8 @@ int innerq_decode_attn_noalloc(const innerq_attn_args* args, void* out, int64_t 
  * pages.  A group that holds a value that is not finite has a NaN scale.
  *   pages   [n_pages][Hkv][page_tiles][4608] bytes (innerq_b200/csrc/paged.cuh)
  *   dense_k, dense_v  [n_slots][Hkv][w_sink + w_recent + 32][D] dtype
- *   table   [B] rows (table_stride apart) of max_pages page numbers
+ *   table   [B] rows (table_stride apart) of max_pages page numbers; NULL only
+ *           with B == 0 or max_pages == 0
  *   slots, seq_lens   [B]
  * The lengths, slots and page numbers are read on the device, so a launch can
  * be recorded in a CUDA graph and replayed.  What they name wrongly is never

@@ -594,7 +594,9 @@ int paged_dev(const innerq_paged* c, PagedDev& d) {
     return set_last_error(INNERQ_ERR_ARG, "sink %d and recent window %d must be multiples of 32 up to 4096", c->w_sink, c->w_recent);
   if (c->B > 0 && (!c->slots || !c->seq_lens || !c->dense_k || !c->dense_v))
     return set_last_error(INNERQ_ERR_ARG, "null pointer");
-  if (c->B > 0 && c->n_pages > 0 && c->max_pages > 0 && (!c->pages || !c->table)) return set_last_error(INNERQ_ERR_ARG, "null pages or page table");
+  // the table is read before a page number is compared with n_pages
+  if (c->B > 0 && c->max_pages > 0 && (!c->table || (c->n_pages > 0 && !c->pages)))
+    return set_last_error(INNERQ_ERR_ARG, "null pages or page table");
   if (!aligned16(c->pages) || !aligned16(c->dense_k) || !aligned16(c->dense_v))
     return set_last_error(INNERQ_ERR_ARG, "pages and slots must be 16-byte aligned");
   d.pages = (uint8_t*)c->pages;

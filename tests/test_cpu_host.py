@@ -308,3 +308,22 @@ def test_paged_cache_and_prompt_attention_refuse_cpu_tensors():
     x = torch.zeros((1, 1, 128), dtype=torch.float16)
     with pytest.raises(RuntimeError, match="CUDA"):
         prompt_attention(x, x, x, torch.zeros(2, dtype=torch.int32))
+
+
+def test_paged_entry_points_refuse_a_null_page_table_of_a_cache_without_pages():
+    """The kernels read a page number before they compare it with the number of
+    pages, so a table with columns is needed even where there are no pages."""
+    from innerq_b200 import _lib
+    lib = _lib.load()
+    f = dict(size=_lib.PAGED_FORMAT.size, dtype=0, D=128, Hkv=2, tiles=2, n_pages=0, n_slots=2, sink=32, recent=32, B=1, cols=4,
+             pages=0, dk=256, dv=256, table=0, stride=4, slots=256, lens=256)
+    cache = _lib.PAGED_FORMAT.pack(*f.values())
+    new = _lib.PAGED_NEW_FORMAT.pack(_lib.PAGED_NEW_FORMAT.size, 4, 1, 128, 0, 9, 256, 512, 128, 256, 256, 128, 256, 256, 128, 0,
+                                     256, 256, 64, 256, 512, 128, 0, 256, 128)
+    for call in (lambda: lib.innerq_paged_append(cache, new, None), lambda: lib.innerq_paged_read(cache, 256, 256, 1, 256, 256, None),
+                 lambda: lib.innerq_paged_attn(cache, 4, 256, 512, 128, 1.0, 256, 1 << 30, 256, 512, 128, None, None)):
+        assert call() == -1 and "page table" in _lib.last_error()
+    assert lib.innerq_paged_attn_workspace(cache, 4) == -1
+    # without columns there is no table
+    f.update(cols=0)
+    assert lib.innerq_paged_attn_workspace(_lib.PAGED_FORMAT.pack(*f.values()), 4) > 0
