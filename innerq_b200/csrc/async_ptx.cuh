@@ -40,6 +40,11 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     if (mbar_try_wait(bar, parity)) return true;
   return false;
 }
+// The same for a converged warp, decided by all lanes together: a lane whose
+// tries ran out takes the others with it, so that collectives may follow.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, uint32_t limit) {
+  return __all_sync(~0u, mbar_wait_bounded(bar, parity, limit));
+}
 __device__ __forceinline__ void fence_proxy_async() {
   asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
 }

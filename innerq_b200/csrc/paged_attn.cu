@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
         s.largest(x, q.f[0], q.f[1], t0, t1);
         if (!s.fits(t0, t1)) s.raise(t0, t1);
       };
-      failed = failed || !mbar_wait_bounded(&sm.bars[w][st_get], parity, kWaitLimit);
+      failed = failed || !mbar_wait_warp(&sm.bars[w][st_get], parity, kWaitLimit);
       if (!failed) {
         logits(st_get, x);
         settle();
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
           if (lane == 0) --in_flight;
           break;
         }
-        failed = !mbar_wait_bounded(&sm.bars[w][st_get], parity, kWaitLimit);
+        failed = !mbar_wait_warp(&sm.bars[w][st_get], parity, kWaitLimit);
         if (failed) break;
         float y[2][4];
         packed_values<DT>(sm.ring[w][st], lane, q, x, s);

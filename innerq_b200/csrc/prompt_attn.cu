@@ -211,7 +211,7 @@ struct Pieces {
   __device__ __forceinline__ Pieces(Smem& s) : sm(s) {}
   // the next piece; null: no more (or, with ok false, a wait that ran out)
   __device__ __forceinline__ Work* next() {
-    ok = __all_sync(~0u, mbar_wait_bounded(&sm.work_full[slot], parity, kWait));
+    ok = mbar_wait_warp(&sm.work_full[slot], parity, kWait);
     Work* w = &sm.work[slot];
     return ok && w->n0 >= 0 ? w : nullptr;
   }
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         pieces.done(lane);
         if (n == 0) continue;
         const int kv_head = head / (a.Hq / a.Hkv);
-        if (q_count > 0) ok = __all_sync(~0u, mbar_wait_bounded(&sm.q_empty, (q_count - 1) & 1, kWait));
+        if (q_count > 0) ok = mbar_wait_warp(&sm.q_empty, (q_count - 1) & 1, kWait);
         if (!ok) break;
         ++q_count;
         if (lane == 0) {
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int it = 0; ok && it < 2 * n; ++it) {
           if (filled == kRing)
-            ok = __all_sync(~0u, mbar_wait_bounded(&sm.empty[st], parity, kWait));
+            ok = mbar_wait_warp(&sm.empty[st], parity, kWait);
           else
             ++filled;
           if (ok && lane == 0) {
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             next_block_ask(&sm.answer, &sm.asked);
           }
           __syncwarp();
-          asking = __all_sync(~0u, mbar_wait_bounded(&sm.asked, asked_par, kWait));
+          asking = mbar_wait_warp(&sm.asked, asked_par, kWait);
           asked_par ^= 1;
           const int x = asking ? next_block_get(&sm.answer) : -1;
           fence_proxy_async();
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           any = asking && decode(a, x, lane, w);
         }
         if (!any) w.n0 = -1;
-        if (!__all_sync(~0u, mbar_wait_bounded(&sm.work_empty[put], put_par, kWait))) return;
+        if (!mbar_wait_warp(&sm.work_empty[put], put_par, kWait)) return;
         if (lane == 0) {
           sm.work[put] = w;
           mbar_arrive(&sm.work_full[put]);
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = max(w->n0, w->n1), cut = w->cut;
         if (warp == 11) publish(-1);
         for (int it = 0; ok && it < 2 * n; ++it) {
-          ok = __all_sync(~0u, mbar_wait_bounded(&sm.full[st], par, kWait));
+          ok = mbar_wait_warp(&sm.full[st], par, kWait);
           if (!ok) break;
           if ((it & 1) && (it >> 1) >= cut) {
             uint4* p = reinterpret_cast<uint4*>(sm.ring[st]) + (warp - 10) * (kTileBytes / 32);
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {
-        ok = __all_sync(~0u, mbar_wait_bounded(&sm.s_full[i], s_par, kWait));
+        ok = mbar_wait_warp(&sm.s_full[i], s_par, kWait);
         if (!ok) break;
         s_par ^= 1;
         tc_fence_after();
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------------------------------------------------- epilogue
       if (first < w->nq) {
         if (n > 0) {
-          if (ok) ok = __all_sync(~0u, mbar_wait_bounded(&sm.o_full[i], o_par, kWait));
+          if (ok) ok = mbar_wait_warp(&sm.o_full[i], o_par, kWait);
           o_par ^= 1;
           tc_fence_after();
         }

@@ -327,3 +327,15 @@ def test_paged_entry_points_refuse_a_null_page_table_of_a_cache_without_pages():
     # without columns there is no table
     f.update(cols=0)
     assert lib.innerq_paged_attn_workspace(_lib.PAGED_FORMAT.pack(*f.values()), 4) > 0
+
+
+def test_waits_before_warp_collectives_are_decided_by_the_whole_warp():
+    """In the paged attention a wait that runs out must end the loop for all
+    lanes of a warp or for none: shuffles, votes and matrix instructions follow.
+    Every use of the bounded wait there is the voting form, or lane 0's drain of
+    its own copies."""
+    src = open(os.path.join(os.path.dirname(HEADER), "..", "innerq_b200", "csrc", "paged_attn.cu")).read()
+    single = [m.start() for m in re.finditer(r"mbar_wait_bounded\(", src)]
+    drain = src.index("if (failed && lane == 0)")
+    assert len(re.findall(r"mbar_wait_warp\(", src)) == 2
+    assert len(single) == 1 and single[0] > drain
