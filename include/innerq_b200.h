@@ -354,7 +354,10 @@ typedef struct {
  * length BEFORE the call, the position of sequence b's first new token), write
  * k and v to the sink / window, and quantize and pack the tiles that leave the
  * window.  The pages a sequence needs for its new length must be in its row of
- * the table.  One launch for one token per sequence, else two.
+ * the table.  A token that belongs to no sequence (one of a sequence of negative
+ * length, such as the padding row of a recorded decode batch, or one past
+ * cu_seqlens[B]) changes nothing, and its rows of q_out and k_out are NaN.  One
+ * launch for one token per sequence, else two.
  */
 int innerq_paged_append(const innerq_paged* cache, const innerq_paged_new* tokens, void* stream);
 

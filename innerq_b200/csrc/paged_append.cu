@@ -361,6 +361,22 @@ __device__ __forceinline__ void rotate_token(const NewDev& n, int Hkv, int tok, 
     rotate_rows<DT>(g, d0, d1, n.k + (int64_t)tok * n.k_st, n.k_sh, n.k_out + (int64_t)tok * n.ko_st, n.ko_sh, Hkv, h0, step);
 }
 
+// the rows of a token that belongs to no sequence
+template <int DT>
+__device__ __forceinline__ void nan_token(const NewDev& n, int Hkv, int tok, int h0, int step) {
+  constexpr uint32_t nan2 = nan16<DT>() * 0x00010001u;
+  const uint4 nan4 = make_uint4(nan2, nan2, nan2, nan2);
+  const int d = 16 * (threadIdx.x & 7);
+  auto fill = [&](uint16_t* row, int64_t sh, int heads) {
+    for (int h = h0; h < heads; h += step) {
+      *reinterpret_cast<uint4*>(row + h * sh + d) = nan4;
+      *reinterpret_cast<uint4*>(row + h * sh + d + 8) = nan4;
+    }
+  };
+  fill(n.q_out + (int64_t)tok * n.qo_st, n.qo_sh, n.Hq);
+  if (n.k_out) fill(n.k_out + (int64_t)tok * n.ko_st, n.ko_sh, Hkv);
+}
+
 // the row that a token of the sink or the window gets in its slot
 // (wait: the first head's loads come before the grid's predecessor is waited for)
 template <int DT>
@@ -432,8 +448,11 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(PagedDev c, N
   const int rest = blk - packs;
   if (ROLE == 0) {  // `split` blocks share a token's heads
     const int rows = kAppendThreads / 8, tok = rest / split, len0 = c.lens[tok];
-    if (len0 < 0) return;
     const int h0 = (threadIdx.x >> 3) + rest % split * rows;
+    if (len0 < 0) {
+      nan_token<DT>(n, c.Hkv, tok, h0, rows * split);
+      return;
+    }
     rotate_token<DT>(n, c.Hkv, tok, len0, h0, rows * split);
     keep_token<DT>(c, n, tok, tok, len0, c.row_of(len0), h0, rows * split, false);
     return;
@@ -443,10 +462,12 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(PagedDev c, N
   find_seq(n.cu, c.B, tok0, &sb);
   int b = max(sb, 0);
   while (b < c.B && tok >= n.cu[b + 1]) ++b;
-  if (b >= c.B || tok >= n.T) return;
-  const int len0 = c.lens[b], cu0 = n.cu[b];
-  if (len0 < 0 || tok < cu0) return;
-  rotate_token<DT>(n, c.Hkv, tok, len0 + tok - cu0, threadIdx.x / (8 * kTokens), kTokenHeads);
+  if (tok >= n.T) return;
+  const int len0 = b < c.B ? c.lens[b] : -1, cu0 = b < c.B ? n.cu[b] : 0, h0 = threadIdx.x / (8 * kTokens);
+  if (len0 < 0 || tok < cu0)
+    nan_token<DT>(n, c.Hkv, tok, h0, kTokenHeads);
+  else
+    rotate_token<DT>(n, c.Hkv, tok, len0 + tok - cu0, h0, kTokenHeads);
 }
 
 // (u - 8) s of the codes in bits 0-3 and 16-19 of w: exact in the dtype before
@@ -574,7 +595,7 @@ cudaError_t launch_append(const PagedDev& c, const NewDev& n, cudaStream_t s) {
   }
   const int n_rotate = (n.T + kTokens - 1) / kTokens, rows = c.w_sink + c.w_recent + 32;
   cudaError_t e = launch_pdl(append_kernel<DT, 1>, dim3(n_pack + n_rotate), block, 0, s, c, n, n_pack, 1);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || c.B == 0) return e;
   return launch_pdl(append_kernel<DT, 2>, dim3(c.B * ((rows + kTokens - 1) / kTokens)), block, 0, s, c, n, 0, 1);
 }
 
@@ -626,7 +647,7 @@ extern "C" int innerq_paged_append(const innerq_paged* cache, const innerq_paged
     return set_last_error(INNERQ_ERR_ARG, "%d tokens for %d sequences need cu_seqlens", a->T, c.B);
   if (a->rot_dim < 0 || a->rot_dim > kD || a->rot_dim % 16)
     return set_last_error(INNERQ_ERR_ARG, "rotation over %d channels (a multiple of 16 up to 128)", a->rot_dim);
-  if (c.B == 0 || a->T == 0) return INNERQ_OK;
+  if (a->T == 0) return INNERQ_OK;
   if (!a->k || !a->v || (a->Hq > 0 && (!a->q || !a->q_out))) return set_last_error(INNERQ_ERR_ARG, "null pointer");
   if (a->rot_dim && (!a->cos || !a->sin || a->max_pos <= 0)) return set_last_error(INNERQ_ERR_ARG, "no rotation table");
   const int64_t st[] = {a->q_st, a->q_sh, a->k_st, a->k_sh, a->v_st, a->v_sh, a->qo_st, a->qo_sh, a->ko_st, a->ko_sh};

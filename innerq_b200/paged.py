@@ -96,8 +96,9 @@ class PagedCache:
         token per sequence, T == B.  cos, sin: fp32 [positions, rot / 2]; the
         token at position t is rotated by row t over its first rot channels,
         in pairs (i, i + rot / 2), or (2i, 2i + 1) with interleaved=True; a
-        position without a row gives NaN.  Without cos and sin nothing is
-        rotated.  Returns the rotated q (None without q), with return_k the
+        position without a row gives NaN, and so does a token of no sequence
+        (of a negative length, or past cu_seqlens[-1]), which changes nothing.
+        Without cos and sin nothing is rotated.  Returns the rotated q (None without q), with return_k the
         pair (q, rotated k): the 16-bit keys that attention over the prompt
         reads."""
         _lib.launch_count[0] += 1 if cu_seqlens is None else 2

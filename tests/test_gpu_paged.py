@@ -478,3 +478,41 @@ def test_long_contexts_have_no_error_of_one_sign(dtype, hq):
             rows.append((out[b, h] - want[h]) @ size / np.linalg.norm(size) / np.linalg.norm(want[h]))
     deviation = math.hypot(ULP[dtype], 2.0 ** -11) / math.sqrt(3 * D)
     assert abs(np.mean(rows)) < 4 * deviation / math.sqrt(len(rows)) + 1e-4, (np.mean(rows), np.max(np.abs(rows)))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("rot", [0, 64, 128])
+@pytest.mark.parametrize("one", [True, False])
+def test_tokens_of_no_sequence_are_nan_and_write_nothing(one, rot, dtype):
+    """A negative length (a padding row of a batch) and tokens past the last
+    sequence: NaN in every channel of the rotated queries and keys, nothing
+    written, the other tokens as without them."""
+    from innerq_b200.paged import PagedCache
+    g = torch.Generator(device="cuda").manual_seed(22)
+    n = 3 if one else 40
+    x = torch.randn((n, 5 + 2 + 2, D), device="cuda", generator=g).to(DT[dtype])
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    cos, sin = (torch.from_numpy(t).cuda() for t in table(64, rot)) if rot else (None, None)
+    tab = i32(0, 1, 2)[:, None]
+    results = []
+    for lens, cu in ((i32(4, -1, 2), [0, 9, 20, 31]), (i32(4, 0, 2), [0, 9, 20, 40])):
+        c = PagedCache.allocate(3, 2, 3, 32, 32, 32, DT[dtype])
+        c.pages.fill_(1), c.dense_k.fill_(1), c.dense_v.fill_(1)
+        old = [torch.full((n, h, D), 7.0, dtype=DT[dtype], device="cuda") for h in (5, 2, 5, 2)]
+        del old  # what the allocator hands out next
+        q, k = c.append(x[:, :5], x[:, 5:7], x[:, 7:], tab, i32(0, 1, 2), lens, None if one else i32(*cu), cos=cos, sin=sin,
+                        return_k=True)
+        results.append((q, k, c))
+    (q, k, c), (q1, k1, c1) = results
+    lost = torch.zeros(n, dtype=torch.bool, device="cuda")
+    lost[1:2] = one
+    if not one:
+        lost[9:20] = lost[31:] = True
+    for got, whole in ((q, q1), (k, k1)):
+        assert torch.isnan(got[lost]).all()
+        assert torch.equal(got[~lost], whole[~lost])
+    assert (c.dense_k[1] == 1).all() and (c.dense_v[1] == 1).all() and (c.pages == 1).all()
+    assert torch.equal(c.dense_k[0], c1.dense_k[0])
+    if not one:  # no sequences at all
+        q, k = c.append(x[:, :5], x[:, 5:7], x[:, 7:], tab[:0], i32(), i32(), i32(0), cos=cos, sin=sin, return_k=True)
+        assert torch.isnan(q).all() and torch.isnan(k).all()
