@@ -576,7 +576,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int x = 0; x < 4; ++x) t4[x] = max3(c ? t4[x] : s[2 * x], s[c + 2 * x], s[c + 2 * x + 1]);
         }
-        const float t = max3(max3(t4[0], t4[1], t4[2]), t4[3], t4[3]) * a.scale_log2;
+        // a row without a query (another sequence's, or bits that nothing wrote)
+        // has no say in what the warp does with the others
+        const float t = real ? max3(max3(t4[0], t4[1], t4[2]), t4[3], t4[3]) * a.scale_log2 : -INFINITY;
         // finite logits throughout: some exponentials may take the FMA pipe
         const bool mixed = !whole ? false : __all_sync(~0u, t < INFINITY);
         if (__any_sync(~0u, t > m + kSlack)) {

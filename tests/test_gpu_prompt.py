@@ -188,3 +188,32 @@ def test_same_inputs_same_bits():
     q, k, v = data(n, n, 4, 2, "bf16", seed=9)
     a = prompt_attention(q, k, v, cu(n))
     assert torch.equal(a, prompt_attention(q, k, v, cu(n)))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("ratio", [2, 3, 5, 6, 7, 32, 33])
+def test_bits_do_not_depend_on_what_ran_before(ratio, dtype):
+    """Ratios that leave rows of a query tile without a query: whatever an
+    earlier call left in shared memory, the same inputs give the same bits."""
+    from innerq_b200.prompt import prompt_attention
+    n = [300, 77, 129]
+    q, k, v = data(n, n, ratio, 1, dtype, seed=ratio)
+    outs = []
+    for fill in (0.0, 1.0, 300.0, float("nan"), float("inf")):
+        other = torch.full((4000, 8, D), fill, dtype=DT[dtype], device="cuda")
+        prompt_attention(other, other[:, :4].contiguous(), other[:, :4].contiguous(), cu([4000]))
+        outs.append(prompt_attention(q, k, v, cu(n)))
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (5, 1)])
+def test_bits_do_not_depend_on_the_neighbours(hq, hkv, dtype):
+    """A sequence alone and beside others: the same bits, whatever they hold."""
+    from innerq_b200.prompt import prompt_attention
+    q, k, v = data([200], [200], hq, hkv, dtype, seed=20)
+    alone = prompt_attention(q, k, v, cu([200]))
+    for fill in (1.0, -60.0, 60000.0, float("nan"), float("inf")):
+        x = [torch.cat([t, torch.full((300, t.shape[1], D), fill, dtype=t.dtype, device="cuda")]) for t in (q, k, v)]
+        assert torch.equal(prompt_attention(*x, cu([200, 300]))[:200], alone), fill
