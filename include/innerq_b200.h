@@ -389,6 +389,7 @@ int innerq_paged_attn(const innerq_paged* cache, int Hq, const void* q, int64_t 
  * cu_q[b] .. cu_q[b + 1] and cu_k[b] .. cu_k[b + 1].  Causal: query i of a
  * sequence of nq queries and nk keys sees keys j <= i + nk - nq, so a chunk of
  * a prompt sees the tokens before it.  A query that sees no key gets zeros and
+ * lse -inf, one that sees only keys whose logits are -inf gets NaN (0 / 0) and
  * lse -inf.  What is masked (later tokens, other sequences) never reaches a
  * result, whatever bits it holds.  Hq any multiple of Hkv.  The lengths are
  * read on the device.

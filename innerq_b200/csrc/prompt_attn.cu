@@ -123,6 +123,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ uint64_t add2_ftz(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // the larger of three; NaN if one is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -130,15 +135,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// 2^y of two finite values on the FMA pipe, which the special-function unit's
-// 2^x leaves idle: y = n + f with n the nearest integer, a polynomial of
-// degree 4 for 2^f on [-1/2, 1/2] (minimax of the relative error, 2.6e-6, from
-// the Remez exchange), and n added to the exponent.  Values below -125 count
-// as -125.
+// 2^y of two values (finite, or -inf) on the FMA pipe, which the
+// special-function unit's 2^x leaves idle: y = n + f with n the nearest
+// integer, a polynomial of degree 4 for 2^f on [-1/2, 1/2] (minimax of the
+// relative error, 2.6e-6, from the Remez exchange), and n added to the exponent.
+// Values below -127 + 2^-16 count as that: the exponent field is 0 there and the
+// result, some 80 units of the smallest subnormal, is 0 in either type and in a
+// sum that takes subnormals for 0 (add2_ftz), so -inf has no weight.
 __device__ __forceinline__ void exp2_poly(uint64_t y, float& a, float& b) {
   float y0, y1;
   f2_split(y, y0, y1);
-  y = f2(fmaxf(y0, -125.f), fmaxf(y1, -125.f));
+  const float least = -127.f + 1.f / 65536.f;
+  y = f2(fmaxf(y0, least), fmaxf(y1, least));
   const float big = 12582912.f;  // 1.5 2^23: a sum with it is rounded to an integer
   const uint64_t t = add2(y, f2(big, big)), n = add2(t, f2(-big, -big));
   const uint64_t f = fma2(n, f2(-1.f, -1.f), y);
@@ -579,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // a row without a query (another sequence's, or bits that nothing wrote)
         // has no say in what the warp does with the others
         const float t = real ? max3(max3(t4[0], t4[1], t4[2]), t4[3], t4[3]) * a.scale_log2 : -INFINITY;
-        // finite logits throughout: some exponentials may take the FMA pipe
+        // no logit is NaN or +inf: some exponentials may take the FMA pipe
         const bool mixed = !whole ? false : __all_sync(~0u, t < INFINITY);
         if (__any_sync(~0u, t > m + kSlack)) {
           const float mn = fmaxf(m, t), corr = ex2(m - mn);
@@ -614,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 p0 = ex2(p0);
                 p1 = ex2(p1);
               }
-              sum[x & 1] = add2(sum[x & 1], f2(p0, p1));
+              sum[x & 1] = add2_ftz(sum[x & 1], f2(p0, p1));
               p[x] = pack_p<DT>(p0, p1);
             }
             tmem_st16(ts + 16 * c, p);
@@ -641,7 +649,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           o_par ^= 1;
           tc_fence_after();
         }
-        const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
+        // a row that sees no key is 0; one that does, but whose logits are all
+        // -inf, is 0 / 0
+        const float inv = !ok ? NAN : l != 0.f ? 1.f / l : lim > 0 ? NAN : 0.f;
         uint16_t* out = a.out + (int64_t)(w->q_base + qi) * a.o_st + head * a.o_sh;
         write_rows<DT>(to, n > 0, inv, real ? out : nullptr, lane);
         tc_fence_before();

@@ -217,3 +217,42 @@ def test_bits_do_not_depend_on_the_neighbours(hq, hkv, dtype):
     for fill in (1.0, -60.0, 60000.0, float("nan"), float("inf")):
         x = [torch.cat([t, torch.full((300, t.shape[1], D), fill, dtype=t.dtype, device="cuda")]) for t in (q, k, v)]
         assert torch.equal(prompt_attention(*x, cu([200, 300]))[:200], alone), fill
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("nk", [1, 100, 128, 129, 256, 300])
+def test_rows_whose_logits_are_all_minus_infinity(nk, causal, dtype):
+    """Keys with an infinite channel: softmax is 0 / 0, NaN, for every row that
+    sees a key, at every length; a row that sees none gets zeros.  The
+    log-sum-exp is -inf for both."""
+    from innerq_b200.prompt import prompt_attention
+    nq = [nk, nk + 10]
+    q, k, v = data(nq, [nk, nk], 2, 1, dtype, seed=nk)
+    q = q.abs() + 1
+    k[..., 5] = float("-inf")
+    lse = torch.zeros(q.shape[:2], device="cuda")
+    out = prompt_attention(q, k, v, cu(nq), cu([nk, nk]), causal=causal, lse=lse)
+    blind = torch.zeros(len(q), dtype=torch.bool, device="cuda")
+    blind[nk:nk + 10] = causal  # ten queries more than keys
+    assert torch.isnan(out[~blind]).all()
+    assert (out[blind] == 0).all()
+    assert torch.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("n", [128, 300, 513])
+def test_keys_of_minus_infinity_have_no_weight(n, dtype):
+    """Some keys with an infinite channel, whole key tiles among them: the
+    others' softmax, whatever finite values those keys have."""
+    q, k, v = data([n], [n], 2, 1, dtype, seed=n)
+    q = q.abs()
+    q[..., 5] = 1.0
+    gone = torch.arange(n, device="cuda") % 3 == 1
+    gone[128:256] = True
+    k[gone, 0, 5] = float("-inf")
+    for causal in (False, True):
+        out = check(q, k, v, [n], [n], causal, dtype)
+        other = v.clone()
+        other[gone] = 60000.0
+        assert torch.equal(check(q, k, other, [n], [n], causal, dtype), out)
