@@ -269,7 +269,6 @@ __device__ __forceinline__ void load_query(const AttnDev& a, int b, int h, int l
 template <int DT>
 __device__ __forceinline__ void packed_logits(const uint8_t* blk, int lane, const Query& q, float x[2][4]) {
   const int gid = lane >> 2;
-  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int mm = 0; mm < 2; ++mm) {
     const uint4 w0 = reinterpret_cast<const uint4*>(blk)[64 * mm + lane];
@@ -344,11 +343,23 @@ __device__ __forceinline__ void packed_values(const uint8_t* blk, int lane, cons
   }
 }
 
+template <int DT> __device__ __forceinline__ bool not_finite(uint32_t h) {
+  constexpr uint32_t e = DT == F16 ? 0x7c00u : 0x7f80u;
+  return (h & e) == e;
+}
+template <int DT> __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+  return w & ((not_finite<DT>(w) ? 0u : 0xffffu) | (not_finite<DT>(w >> 16) ? 0u : 0xffff0000u));
+}
+
 // one 16-bit tile (sink or window) straight from global memory: kr / vr point
-// at its first row, `valid` of its 32 rows hold tokens
-template <int DT>
+// at its first row, `valid` of its 32 rows hold tokens.  An infinite value counts
+// with any probability above 0, of which an fp16 operand may be 0 and a second
+// part 0 or negative: `seen` becomes NaN where a sum is not finite, and the
+// unit's tiles are then taken again with ONE_BY_ONE, which adds the values that
+// are not finite in fp32.
+template <int DT, bool ONE_BY_ONE>
 __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* vr, int valid, const AttnDev& a, int b, int h,
-                                        int lane, State& s) {
+                                        int lane, float& seen, State& s) {
   const int gid = lane >> 2, tq = lane & 3;
   uint4 qw[4];
 #pragma unroll
@@ -414,6 +425,10 @@ __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* v
       uint32_t w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = m ? v[i].y : v[i].x;
+      if constexpr (ONE_BY_ONE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = finite_halves<DT>(w[i]);
+      }
       uint32_t f[2][4];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -429,10 +444,55 @@ __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* v
         mma_acc<DT>(d, f[0], pe[0], pe[1]);
         mma_acc<DT>(d, f[1], pe[2], pe[3]);
       }
+      if constexpr (ONE_BY_ONE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p0 = ex2(x[i >> 1][2 * (i & 1)] - s.m[0] + kPScale), p1 = ex2(x[i >> 1][2 * (i & 1) + 1] - s.m[1] + kPScale);
+#pragma unroll 1
+          for (int j = 0; j < 8; ++j) {  // token 8 i + j: its probabilities are with lanes 4 j ..
+            const float y0 = __shfl_sync(~0u, p0, 4 * j + tq), y1 = __shfl_sync(~0u, p1, 4 * j + tq);
+            if (8 * i + j >= valid) continue;
+            const uint32_t y = reinterpret_cast<const uint32_t*>(vr + (8 * i + j) * kD)[8 * gid + 2 * part + m];
+            if (not_finite<DT>(y)) d[0] = fmaf(y0, lo_f<DT>(y), d[0]), d[1] = fmaf(y1, lo_f<DT>(y), d[1]);
+            if (not_finite<DT>(y >> 16)) d[2] = fmaf(y0, hi_f<DT>(y), d[2]), d[3] = fmaf(y1, hi_f<DT>(y), d[3]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) seen = fmaf(d[i], 0.f, seen);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) s.acc[2 * part + m][i] = fmaf(d[i], 1.f / 16777216.f, s.acc[2 * part + m][i]);
     }
   }
+}
+
+// a warp's 16-bit tiles of a unit that begins at place u0: every fourth place from
+// idx to end but the packed ones.  True: some sum is not finite.
+template <int DT, bool ONE_BY_ONE>
+__device__ __forceinline__ bool dense_tiles(const PagedDev& c, const AttnDev& a, int b, int h, int u0, int idx, int packed_lo,
+                                            int packed_end, int end, int lane, State& s) {
+  float seen = 0.f;
+  s.reset();
+#pragma unroll 1
+  for (int p = idx;; p += kWarps) {
+    if (p >= packed_lo && p < packed_end) p = packed_end + ((p - packed_end) & (kWarps - 1));
+    if (p >= end) break;
+    const int64_t base = c.dense_base(b, h);
+    if (base < 0) {
+      s.poison();
+      continue;
+    }
+    const int t = 32 * (p - u0);
+    const int64_t at = base + (int64_t)c.row_of(t) * kD;
+    dense_tile<DT, ONE_BY_ONE>(c.dk + at, c.dv + at, c.lens[b] - t, a, b, h, lane, seen, s);
+  }
+  return __any_sync(~0u, seen != 0.f);
+}
+template <int DT>
+__device__ __noinline__ void dense_tiles_one_by_one(const PagedDev& c, const AttnDev& a, int b, int h, int u0, int idx, int packed_lo,
+                                                    int packed_end, int end, int lane, State* s) {
+  dense_tiles<DT, true>(c, a, b, h, u0, idx, packed_lo, packed_end, end, lane, *s);
 }
 
 __device__ __forceinline__ int tiles_in(int len, int cap) { return len <= 0 ? 0 : min((int)(((int64_t)len + 31) >> 5), cap); }
@@ -468,7 +528,7 @@ __device__ __forceinline__ int range_of(int total, int grid) {
 }
 
 template <int DT, int RH>
-__global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnDev a) {
+__global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(const __grid_constant__ PagedDev c, const __grid_constant__ AttnDev a) {
   extern __shared__ __align__(128) uint8_t raw[];
   Smem<RH>& sm = *reinterpret_cast<Smem<RH>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
@@ -585,21 +645,12 @@ __global__ void __launch_bounds__(128, kCtasPerSm) attn_kernel(PagedDev c, AttnD
   State s;
   while (true) {
     const int end = min(hi, u0 + nt);
-    s.reset();
     // the 16-bit tiles (sink and window) first, while the copies are under way
     const int packed_lo = u0 + sink_tiles, packed_end = min(end, packed_lo + packed);
-#pragma unroll 1
-    for (int p = idx;; p += kWarps) {
-      if (p >= packed_lo && p < packed_end) p = packed_end + ((p - packed_end) & (kWarps - 1));
-      if (p >= end) break;
-      const int64_t base = c.dense_base(b, h);
-      if (base < 0) {
-        s.poison();
-        continue;
-      }
-      const int t = 32 * (p - u0);
-      const int64_t at = base + (int64_t)c.row_of(t) * kD;
-      dense_tile<DT>(c.dk + at, c.dv + at, c.lens[b] - t, a, b, h, lane, s);
+    if (dense_tiles<DT, false>(c, a, b, h, u0, idx, packed_lo, packed_end, end, lane, s)) {
+      State again;
+      dense_tiles_one_by_one<DT>(c, a, b, h, u0, idx, packed_lo, packed_end, end, lane, &again);
+      s = again;
     }
     if (idx < packed_lo) idx = packed_lo + ((idx - packed_lo) & (kWarps - 1));
     if (idx < packed_end) {

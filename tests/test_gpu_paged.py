@@ -516,3 +516,39 @@ def test_tokens_of_no_sequence_are_nan_and_write_nothing(one, rot, dtype):
     if not one:  # no sequences at all
         q, k = c.append(x[:, :5], x[:, 5:7], x[:, 7:], tab[:0], i32(), i32(), i32(0), cos=cos, sin=sin, return_k=True)
         assert torch.isnan(q).all() and torch.isnan(k).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("length", [20, 90, 700, 9000])
+def test_infinite_values_of_the_16_bit_tokens(length, dtype):
+    """An infinity in the sink or the window, times any probability above 0, is
+    an infinity: of its sign, in its channel, in every query's output.  Two of
+    both signs, or a NaN, are NaN.  The other channels do not change by a bit.
+    One of the infinities sits at a token whose probability is below what fp16
+    holds."""
+    from innerq_b200.paged import PagedCache
+    g = torch.Generator(device="cuda").manual_seed(length)
+    x = torch.randn((length, 2, D), device="cuda", generator=g).to(DT[dtype])
+    q = torch.randn((1, 8, D), device="cuda", generator=g).to(DT[dtype])
+    q[..., 0] = 8.0
+    x[:, 0, 0] = 0
+    x[7, 0, 0] = -40.0  # logit 8 * -40 / sqrt 128 = -28: 2^-41
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    tab = torch.arange(-(-length // 64), dtype=torch.int32, device="cuda")[None]
+    last = length - 1
+    inf, nan = float("inf"), float("nan")
+    outs = []
+    for bad in (False, True):
+        v = x[:, 1:].clone()
+        for t, d, y in ((3, 10, inf), (4, 11, -inf), (last, 12, inf), (last - 2, 13, -inf), (3, 14, inf), (last, 14, -inf),
+                        (last - 5, 15, nan), (7, 16, inf), (7, 17, -inf)):
+            v[t, 0, d] = y if bad else 0.0
+        c = PagedCache.allocate(tab.shape[1], 1, 1, 64, 32, 32, DT[dtype])
+        c.append(None, x[:, :1], v, tab, i32(0), i32(0), i32(0, length))
+        outs.append(c.attend(q, tab, i32(0), i32(length))[0].double().cpu())
+    clean, got = outs
+    want = {10: inf, 11: -inf, 12: inf, 13: -inf, 14: nan, 15: nan, 16: inf, 17: -inf}
+    for d, w in want.items():
+        assert torch.equal(got[:, d], torch.full((8,), w, dtype=torch.float64)) or (w != w and torch.isnan(got[:, d]).all()), (d, got[:, d])
+    keep = [d for d in range(D) if d not in want]
+    assert torch.equal(got[:, keep], clean[:, keep])
