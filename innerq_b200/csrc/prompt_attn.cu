@@ -257,9 +257,11 @@ __device__ __forceinline__ void transpose4(uint4 w[4], int lane) {
 
 // The finished rows of a warp, one per thread: O / l, or zeros where there is
 // no O.  Four lanes write 64 contiguous bytes of a row (a thread on its own
-// would spread every store over 32 rows: 2.5 us per piece of work).
+// would spread every store over 32 rows: 2.5 us per piece of work).  True: this
+// thread's row holds something that is not finite (fp16; not looked for in bf16).
 template <int DT>
-__device__ __forceinline__ void write_rows(uint32_t to, bool any, float inv, uint16_t* out, int lane) {
+__device__ __forceinline__ bool write_rows(uint32_t to, bool any, float inv, uint16_t* out, int lane) {
+  __half2 seen = __half2half2(__half(0.f));
   uint64_t row[4];
 #pragma unroll
   for (int x = 0; x < 4; ++x) row[x] = __shfl_sync(~0u, (unsigned long long)out, (lane & ~3) + x);
@@ -279,12 +281,17 @@ __device__ __forceinline__ void write_rows(uint32_t to, bool any, float inv, uin
       uint32_t* e = reinterpret_cast<uint32_t*>(&w[x]);
 #pragma unroll
       for (int y = 0; y < 4; ++y) e[y] = inv == 0.f ? 0u : pack_p<DT>(o[8 * x + 2 * y] * inv, o[8 * x + 2 * y + 1] * inv);
+      if constexpr (DT == F16) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) seen = __hfma2(as_pair<F16>(e[y]), __half2half2(__half(0.f)), seen);
+      }
     }
     transpose4(w, lane);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
       if (row[x]) reinterpret_cast<uint4*>(row[x])[4 * c + (lane & 3)] = w[x];
   }
+  return DT == F16 && !__hbeq2(seen, seen);
 }
 
 template <int DT>
@@ -653,25 +660,79 @@ __global__ void __launch_bounds__(kThreads, 1)
         // -inf, is 0 / 0
         const float inv = !ok ? NAN : l != 0.f ? 1.f / l : lim > 0 ? NAN : 0.f;
         uint16_t* out = a.out + (int64_t)(w->q_base + qi) * a.o_st + head * a.o_sh;
-        write_rows<DT>(to, n > 0, inv, real ? out : nullptr, lane);
+        const bool odd = write_rows<DT>(to, n > 0, inv, real ? out : nullptr, lane);
         tc_fence_before();
         __syncwarp();
-        if (ok && *(volatile int*)&w->dirty && real) {
-          // values that were set to 0 and that this row does see (the row was
-          // written by this warp's lanes: made visible by the warp barrier)
-          const int kv_head = head / (a.Hq / a.Hkv);
+        // Values that are not finite, one by one (the row was written by this
+        // warp's lanes: made visible by the warp barrier).
+        const bool dirty = *(volatile int*)&w->dirty, fine = ok && real && inv == inv;
+        const int keys = fine ? min(kRows * n, lim) : 0;
+        if (__any_sync(~0u, fine && (dirty || (DT == F16 && odd)))) {
+          const int kv_head = w->head / (a.Hq / a.Hkv);
           const uint16_t* qr = a.q + (int64_t)(w->q_base + qi) * a.q_st + head * a.q_sh;
-          for (int key = kRows * w->cut; key < min(kRows * n, lim); ++key) {
-            const uint16_t* vr = a.v + (int64_t)(w->k_base + key) * a.v_st + kv_head * a.v_sh;
+          auto value_row = [&](int key) { return a.v + (int64_t)(w->k_base + key) * a.v_st + kv_head * a.v_sh; };
+          auto weight = [&](int key) {
+            const uint16_t* kr = a.k + (int64_t)(w->k_base + key) * a.k_st + kv_head * a.k_sh;
+            float dot = 0.f;
+            for (int x = 0; x < kD; ++x) dot = fmaf(to_f<DT>(qr[x]), to_f<DT>(kr[x]), dot);
+            return ex2(fmaf(a.negate ? -dot : dot, a.scale_log2, kShift - m)) * inv;
+          };
+          if (DT == F16 && __any_sync(~0u, fine && odd)) {
+            // An infinity times a probability that is 0 in fp16, but not 0, left
+            // NaN.  Such channels (lost) start again from 0 and take all values
+            // that are not finite until they are NaN for good; the lanes look for
+            // keys with such values, 32 at a time.
+            uint32_t lost[kD / 32];
+#pragma unroll
+            for (int x = 0; x < kD / 32; ++x) {
+              lost[x] = 0;
+              for (int y = 0; fine && odd && y < 32; ++y)
+                if (to_f<DT>(out[32 * x + y]) != to_f<DT>(out[32 * x + y])) {
+                  lost[x] |= 1u << y;
+                  out[32 * x + y] = 0;
+                }
+            }
+            const int most = __reduce_max_sync(~0u, keys);
+            for (int key0 = 0; key0 < most && __any_sync(~0u, lost[0] | lost[1] | lost[2] | lost[3]); key0 += 32) {
+              bool found = false;
+              if (key0 + lane < most) {
+                const uint4* row4 = reinterpret_cast<const uint4*>(value_row(key0 + lane));
+                for (int x = 0; x < kD / 8; ++x) {
+                  const uint4 v = row4[x];
+                  const uint32_t* e = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+                  for (int y = 0; y < 4; ++y) found |= not_finite<DT>(e[y]) | not_finite<DT>(e[y] >> 16);
+                }
+              }
+              for (uint32_t hits = __ballot_sync(~0u, found); hits; hits &= hits - 1) {
+                const int key = key0 + __ffs(hits) - 1;
+                if (key >= keys || !(lost[0] | lost[1] | lost[2] | lost[3])) continue;
+                const uint16_t* vr = value_row(key);
+                float p = -1.f;
+#pragma unroll
+                for (int x = 0; x < kD / 32; ++x)
+                  for (uint32_t left = lost[x]; left; left &= left - 1) {
+                    const int d = 32 * x + __ffs(left) - 1;
+                    const float v = to_f<DT>(vr[d]);
+                    // (once more the same infinity: a sum of 100000 keys would
+                    // take their weights otherwise)
+                    if (!not_finite<DT>(vr[d]) || v == to_f<DT>(out[d])) continue;
+                    if (p == -1.f) p = weight(key);
+                    const float sum = fmaf(p, v, to_f<DT>(out[d]));
+                    out[d] = from_f<DT>(sum);
+                    if (sum != sum) lost[x] &= ~(left & (0u - left));
+                  }
+              }
+              __syncwarp();
+            }
+          }
+          // values that were set to 0 and that this row does see
+          for (int key = kRows * w->cut; dirty && key < keys; ++key) {
+            const uint16_t* vr = value_row(key);
             float p = -1.f;
             for (int d = 0; d < kD; ++d) {
               if (!not_finite<DT>(vr[d])) continue;
-              if (p == -1.f) {
-                const uint16_t* kr = a.k + (int64_t)(w->k_base + key) * a.k_st + kv_head * a.k_sh;
-                float dot = 0.f;
-                for (int x = 0; x < kD; ++x) dot = fmaf(to_f<DT>(qr[x]), to_f<DT>(kr[x]), dot);
-                p = ex2(fmaf(a.negate ? -dot : dot, a.scale_log2, kShift - m)) * inv;
-              }
+              if (p == -1.f) p = weight(key);
               out[d] = from_f<DT>(to_f<DT>(out[d]) + p * to_f<DT>(vr[d]));
             }
           }

@@ -256,3 +256,30 @@ def test_keys_of_minus_infinity_have_no_weight(n, dtype):
         other = v.clone()
         other[gone] = 60000.0
         assert torch.equal(check(q, k, other, [n], [n], causal, dtype), out)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n", [40, 128, 300, 1000])
+def test_infinite_values_with_small_probabilities(n, causal, dtype):
+    """An infinity times any probability above 0 is an infinity, also where the
+    probability is below what fp16 holds (2^-41 here), in a key tile that all
+    queries see whole as in one that they do not; of both signs it is NaN.  The
+    other channels do not change by a bit."""
+    from innerq_b200.prompt import prompt_attention
+    q, k, v = data([n], [n], 5, 1, dtype, seed=n)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[[7, n - 3], 0, 0] = -40.0  # logit 8 * -40 / sqrt 128 = -28
+    outs = []
+    for inf in (0.0, float("inf")):
+        v[[7, 7, n - 3, 7, n - 3], 0, [16, 17, 18, 19, 19]] = torch.tensor([inf, -inf, inf, inf, -inf]).to(v)
+        outs.append(prompt_attention(q, k, v, cu([n]), causal=causal).double())
+    clean, got = outs
+    sees = lambda t: torch.arange(n, device="cuda")[:, None].expand(n, 5) >= (t if causal else 0)  # noqa: E731
+    inf = float("inf")
+    for d, t, sign in ((16, 7, inf), (17, 7, -inf), (18, n - 3, inf)):
+        assert torch.equal(got[..., d], torch.where(sees(t), sign, clean[..., d])), d
+    assert torch.equal(torch.nan_to_num(got[..., 19], nan=7.0, posinf=8.0),
+                       torch.where(sees(n - 3), 7.0, torch.where(sees(7), 8.0, clean[..., 19])))
+    keep = [d for d in range(D) if d not in (16, 17, 18, 19)]
+    assert torch.equal(got[..., keep], clean[..., keep])
