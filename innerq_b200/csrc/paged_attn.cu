@@ -2,28 +2,36 @@
 // length per sequence, one pass over 32-token tiles that may be split anywhere.
 //
 // Mathematics.  A 4-bit code u (0..15, offset 8) placed in the mantissa of a
-// 16-bit word IS the fp16 subnormal u 2^-24 (16 u 2^-24 four bits higher), so
-// one AND expands two codes into an fp16 tensor-core operand, exactly:
+// 16-bit word IS the fp16 subnormal u 2^-24 (u 2^-20 four bits higher), so one
+// AND expands two codes into an fp16 tensor-core operand, exactly:
 //   q.k_t = sum_g s_tg (sum_{d in g} q_d u_td - 8 sum_{d in g} q_d)
 //   out_d = sum_tiles s_gd (sum_t p_t u_td - 8 sum_t p_t) / sum_t p_t
 // The inner sums are mma.m16n8k16 (codes as A: 16 tokens, or 16 channels, by
 // 8 query heads) with fp32 accumulators that start at the offset term; group
 // scales are applied in fp32.  The query is scaled per head by a power of two
-// into [2^14, 2^15), exact in fp16 for both dtypes; the slots whose codes sit
-// four bits higher take q / 16 and p / 16.  A probability is 2^8 p, relative to a
-// running maximum that may lag by 2^7, rounded to fp16 (11 bits down to 2^-22):
-// the one rounding of the 4-bit path, and what an fp16 operand takes; with fp16
-// inputs it adds as much error again as rounding the output does (a second part
-// for what it leaves takes 216 us to 249 on the case below).  The sum that
-// divides the result is taken over the rounded values by MMAs, against a code of
-// 11: an MMA aligns its products by the operands' nominal exponents, so products
-// with a subnormal are cut off at 2^-16 to 2^-17 of the tile's largest
-// probability, always towards zero.  Over tens of thousands of tokens that adds
-// up along the values' scales (3e-4 of the output, measured), unless 8 sum p
-// loses as much: a random code loses about 0.7 of what an odd one does, and
-// 8 / 11 of the sum against 11 is taken off.  16-bit tokens (sink, window) use
-// the same MMAs on their own type, with ones, and bf16 probabilities are split
-// into two parts there.
+// into [2^14, 2^15) (channels below 2^-24 of the largest lose bits as fp16);
+// the slots whose codes sit four bits higher take q / 16.  A probability is
+// 2^8 p, relative to a running maximum that may lag by 2^7, rounded to fp16
+// (11 bits down to 2^-22), as an fp16 operand takes it; with fp16 inputs that
+// adds as much error again as rounding the output does (a second part for what
+// it leaves took an earlier state of the kernel from 216 us to 249 on the case
+// below).  The sum that divides the result is taken over the rounded values.
+//   An MMA aligns its products by the operands' nominal exponents, 2^-14 for a
+// subnormal, and cuts what lies some 26 bits below the largest off, towards
+// zero.  Over tens of thousands of tokens that adds up along the values' scales
+// unless it stays far below the probabilities' own last bits.  The values' codes
+// therefore sit four bits up throughout: the cut is at 2^-20 of the tile's
+// largest probability then, and the offset 8 sum p, an MMA against the code 8,
+// loses what a zero value does.  At 33000 and 131000 tokens the part of the error
+// that has a sign is at most 2e-5 of the output (the output's own rounding to
+// fp16: 2e-4) for values normal, uniform, of one sign, constant and with one
+// outlier per group; ordinary numbers u - 8 as operands do no better and take
+// 256 us where this takes 227.  With the low codes where they lie (217 us) the
+// cut is at 2^-16, the outliers' error was up to 4.5 times the rounding, and no
+// constant in place of the 8 helps all of them.  Logits keep the cheaper form:
+// their cut-off parts have the query's signs and sum to some 1e-5 of a logit.
+//   16-bit tokens (sink, window) use the same MMAs on their own type, with ones,
+// and bf16 probabilities are split into two parts there.
 //
 // Work.  The tiles of all (sequence, head) units form one list that is cut
 // into equal ranges, one per resident CTA, so ragged lengths balance without
@@ -61,8 +69,7 @@ constexpr int kUnitCost = 16;
 constexpr int kHeadPitch = 148;  // floats per head of the combine buffer: conflict-free
 constexpr float kPScale = 8.f;   // probabilities carry 2^8 relative to the running maximum,
 constexpr float kSlack = 7.f;    // which may lag behind the true one by 2^7 before it is raised
-constexpr float kOutScale = 16777216.f;  // what the codes' 2^-24 left in the accumulators
-constexpr uint32_t kSumCode = 11;  // the code against which probabilities are summed
+constexpr float kOutScale = 1048576.f;  // what the values' 2^-20 left in the accumulators
 constexpr float kNoMax = -1e30f; // running maximum before the first logit
 
 struct AttnDev {
@@ -150,10 +157,22 @@ __device__ __forceinline__ void code_frags(uint32_t w0, uint32_t w1, uint32_t a[
   b[3] = w1 & 0x00f000f0u;
 }
 
+// The same slots with every code four bits up, u 2^-20.
+__device__ __forceinline__ void value_frags(uint32_t w0, uint32_t w1, uint32_t a[4], uint32_t b[4]) {
+  a[0] = (w0 << 4) & 0x00f000f0u;
+  a[1] = (w1 << 4) & 0x00f000f0u;
+  a[2] = w0 & 0x00f000f0u;
+  a[3] = w1 & 0x00f000f0u;
+  b[0] = (w0 >> 4) & 0x00f000f0u;
+  b[1] = (w1 >> 4) & 0x00f000f0u;
+  b[2] = (w0 >> 8) & 0x00f000f0u;
+  b[3] = (w1 >> 8) & 0x00f000f0u;
+}
+
 // What one warp has accumulated of a unit.  A lane holds the query heads
 // 2 tq + {0, 1} and, of each, the channels 16 gid + 2 mt + {0, 1}:
-// acc[mt][2 i + c] is channel 16 gid + 2 mt + i of head 2 tq + c, in units of
-// 2^-16 (codes carry 2^-24, probabilities 2^8); l carries 2^8.
+// acc[mt][2 i + c] is channel 16 gid + 2 mt + i of head 2 tq + c; acc and l carry
+// 2^8.
 struct State {
   float acc[8][4], m[2], l[2];
   __device__ __forceinline__ void reset() {
@@ -304,21 +323,17 @@ __device__ __forceinline__ void packed_values(const uint8_t* blk, int lane, cons
   const float b0 = kPScale - s.m[0], b1 = kPScale - s.m[1];
   uint32_t pb[4];
 #pragma unroll
-  for (int mm = 0; mm < 2; ++mm) {
-    pb[2 * mm] = transpose8x8(half2_of(ex2(fmaf(x[mm][0], q.f[0], b0)), ex2(fmaf(x[mm][1], q.f[1], b1))));
-    pb[2 * mm + 1] = transpose8x8(half2_of(ex2(fmaf(x[mm][2], q.f[0], b0 - 4.f)), ex2(fmaf(x[mm][3], q.f[1], b1 - 4.f))));
-  }
+  for (int i = 0; i < 4; ++i)
+    pb[i] = transpose8x8(half2_of(ex2(fmaf(x[i >> 1][2 * (i & 1)], q.f[0], b0)), ex2(fmaf(x[i >> 1][2 * (i & 1) + 1], q.f[1], b1))));
   float ps[4];
-  {
-    constexpr uint32_t c = kSumCode * 0x10001u;
-    const uint32_t code[4] = {c, c, c << 4, c << 4};
-    mma_from<F16>(ps, code, pb[0], pb[1], zero);
-    mma_acc<F16>(ps, code, pb[2], pb[3]);
-  }
-  s.l[0] = fmaf(ps[0], kOutScale / kSumCode, s.l[0]);
-  s.l[1] = fmaf(ps[1], kOutScale / kSumCode, s.l[1]);
+  // 8 sum p, the offset; an eighth of it divides the result
+  const uint32_t eights[4] = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};
+  mma_from<F16>(ps, eights, pb[0], pb[1], zero);
+  mma_acc<F16>(ps, eights, pb[2], pb[3]);
+  s.l[0] = fmaf(ps[0], kOutScale / 8.f, s.l[0]);
+  s.l[1] = fmaf(ps[1], kOutScale / 8.f, s.l[1]);
   float off[4];
-  quad(off, ps[0] * (-8.f / kSumCode), ps[1] * (-8.f / kSumCode));
+  quad(off, -ps[0], -ps[1]);
   const uint4 v0 = reinterpret_cast<const uint4*>(blk + kVScale)[2 * gid];
   const uint4 v1 = reinterpret_cast<const uint4*>(blk + kVScale)[2 * gid + 1];
 #pragma unroll
@@ -329,7 +344,7 @@ __device__ __forceinline__ void packed_values(const uint8_t* blk, int lane, cons
     for (int m = 0; m < 2; ++m) {
       const int mt = 2 * pc + m;
       uint32_t a[4], b[4];
-      code_frags(pw[2 * m], pw[2 * m + 1], a, b);
+      value_frags(pw[2 * m], pw[2 * m + 1], a, b);
       float d[4];
       mma_from<F16>(d, a, pb[0], pb[1], off);
       mma_acc<F16>(d, b, pb[2], pb[3]);
@@ -462,7 +477,7 @@ __device__ __forceinline__ void dense_tile(const uint16_t* kr, const uint16_t* v
         for (int i = 0; i < 4; ++i) seen = fmaf(d[i], 0.f, seen);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s.acc[2 * part + m][i] = fmaf(d[i], 1.f / 16777216.f, s.acc[2 * part + m][i]);
+      for (int i = 0; i < 4; ++i) s.acc[2 * part + m][i] = fmaf(d[i], 1.f / kOutScale, s.acc[2 * part + m][i]);
     }
   }
 }

@@ -552,3 +552,81 @@ def test_infinite_values_of_the_16_bit_tokens(length, dtype):
         assert torch.equal(got[:, d], torch.full((8,), w, dtype=torch.float64)) or (w != w and torch.isnan(got[:, d]).all()), (d, got[:, d])
     keep = [d for d in range(D) if d not in want]
     assert torch.equal(got[:, keep], clean[:, keep])
+
+
+def held(c, pages, length):
+    """What a cache holds of the sequence of slot 0, [length, H, D] in 64 bits."""
+    t, d = torch.arange(32, device="cuda")[:, None], torch.arange(D, device="cuda")[None]
+    H, dt, sink = c.n_kv_heads, c.dtype, c.w_sink
+    n = c.packed_tokens(length)
+    blocks = c.pages[pages.long()].transpose(0, 1).reshape(H, -1, 4608)[:, :n // 32]
+    scale = lambda lo: blocks[..., lo:lo + 256].contiguous().view(dt).double()  # noqa: E731
+
+    def code(base, word, nibble):
+        return (blocks.long()[..., base + word * 4 + nibble // 2] >> (4 * (nibble % 2))) % 16 - 8
+    g, l, m = d // 32, d // 8 % 4, d % 8
+    k = code(0, ((t // 8 * 8 + t % 8) * 4 + l) * 4 + g, m) * scale(2048)[..., (t % 8 * 4 + t // 8) * 4 + g]
+    word = (((d // 4 % 4 * 8 + d // 16) * 4 + t % 8 // 2) * 2 + d // 2 % 2) * 2 + d % 2
+    v = code(2304, word, t // 8 + 4 * (t % 2)) * scale(4352)[..., None, :]
+    at = torch.cat([torch.arange(min(sink, length)), torch.arange(sink + n, length)]).cuda()
+    row = torch.where(at < sink, at, sink + (at - sink) % (c.w_recent + 32))
+    out = []
+    for packed, dense in ((k, c.dense_k), (v, c.dense_v)):
+        x = torch.empty((length, H, D), dtype=torch.float64, device="cuda")
+        x[sink:sink + n] = packed.reshape(H, n, D).transpose(0, 1)
+        x[at] = dense[0][:, row].transpose(0, 1).double()
+        out.append(x)
+    return out
+
+
+@pytest.mark.parametrize("kind", ["normal", "one sign", "outliers", "constant"])
+@pytest.mark.parametrize("dtype,length,hq", [("fp16", 33000, 8), ("fp16", 120001, 8), ("bf16", 33000, 4)])
+def test_sums_over_long_contexts_do_not_depend_on_how_codes_are_spread(dtype, length, hq, kind):
+    """Values whose codes are spread, of one sign, nearly all zero (one large
+    value per group) or all alike, against 64 bits over what the cache holds.
+    Rounding of the output (2^-11 / sqrt 3 of a value in fp16, 2^-8 / sqrt 3 in
+    bf16, at most) and of the probabilities to 11 bits (a random walk, 2^-11 /
+    sqrt 3 of sqrt(sum p^2 v^2) at most) are all that may be left: the errors'
+    mean along the values' sizes within four of its deviations, and a row's
+    error within 1.25 of them together, the 128 channels' own scatter (four
+    deviations of a root of a mean of 128 squares) included.  5e-5 for the sums
+    in 32 bits."""
+    from innerq_b200.paged import PagedCache
+    dt, H = DT[dtype], 2
+    g = torch.Generator(device="cuda").manual_seed(24)
+    z = torch.randn((length, H, D), device="cuda", generator=g)
+    if kind == "one sign":
+        z = z.abs()
+    elif kind == "constant":
+        z = torch.full_like(z, 0.75)
+    elif kind == "outliers":
+        at = torch.randint(0, 32, (length // 32 + 1, 1, H, D), device="cuda", generator=g)
+        big = (torch.arange(32, device="cuda")[None, :, None, None] == at).flatten(0, 1)[:length]
+        z = torch.where(big, 20.0 * torch.sign(z), 0.5 * z)
+    k = torch.randn((length, H, D), device="cuda", generator=g).to(dt)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    tab = torch.arange(length // 128 + 1, dtype=torch.int32, device="cuda")[None]
+    c = PagedCache.allocate(tab.shape[1], H, 1, 128, 32, 96, dt)
+    c.append(None, k, z.to(dt), tab, i32(0), i32(0), i32(0, length))
+    q = torch.randn((1, H * hq, D), device="cuda", generator=g).to(dt)
+    lse = torch.empty((1, H * hq), device="cuda")
+    out = c.attend(q, tab, i32(0), i32(length), lse=lse)[0].double()
+    kk, vv = held(c, tab[0], length)
+    along, size_of_rounding = [], []
+    for h in range(H):
+        s = q[0, h * hq:h * hq + hq].double() @ kk[:, h].T * D ** -0.5
+        p = torch.softmax(s, -1)
+        want = p @ vv[:, h]
+        err = out[h * hq:h * hq + hq] - want
+        assert float((lse[0, h * hq:h * hq + hq].double() - torch.logsumexp(s, -1) / math.log(2)).abs().max()) < 1e-4
+        walk = (p.square() @ vv[:, h].square()).sqrt()
+        expect = ((ULP[dtype] * want).square() + (2.0 ** -11 * walk).square()).sum(-1).div(3 * D).sqrt()  # rms of a channel
+        size = want.norm(dim=1) / D ** 0.5
+        assert bool((err.norm(dim=1) / D ** 0.5 <= 1.25 * expect + 5e-5 * size).all()), (err.norm(dim=1) / D ** 0.5 / expect)
+        if kind in ("normal", "outliers"):  # elsewhere the output's own rounding has a sign
+            scale = vv[:, h].abs().mean(0)
+            along += ((err @ scale) / scale.norm() / D ** 0.5 / size).tolist()
+            size_of_rounding += (expect / size / D ** 0.5).tolist()
+    if along:
+        n = len(along)
+        assert abs(sum(along) / n) <= 4 * sum(size_of_rounding) / n / n ** 0.5 + 5e-5, (sum(along) / n, sum(size_of_rounding) / n)
