@@ -101,8 +101,10 @@ class PagedCache:
         Without cos and sin nothing is rotated.  Returns the rotated q (None without q), with return_k the
         pair (q, rotated k): the 16-bit keys that attention over the prompt
         reads."""
-        _lib.launch_count[0] += 1 if cu_seqlens is None else 2
-        return _host.append(self._c, q, k, v, page_table, slots, seq_lens, cu_seqlens, cos, sin, interleaved, return_k)
+        out = _host.append(self._c, q, k, v, page_table, slots, seq_lens, cu_seqlens, cos, sin, interleaved, return_k)
+        if k.shape[0]:
+            _lib.launch_count[0] += 1 if cu_seqlens is None or not seq_lens.shape[0] else 2
+        return out
 
     def attend(self, q: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor, seq_lens: torch.Tensor,
                scale: float | None = None, out: torch.Tensor | None = None,
@@ -111,8 +113,10 @@ class PagedCache:
         over its seq_lens[b] cached tokens (this step's included) -> out
         [B, Hq, 128].  A sequence without tokens gets zeros.  lse (optional,
         fp32 [B, Hq]): log2-sum-exp2 of the scaled logits."""
-        _lib.launch_count[0] += 2
-        return _host.attend(self._c, q, page_table, slots, seq_lens, scale, out, lse)
+        out = _host.attend(self._c, q, page_table, slots, seq_lens, scale, out, lse)
+        if q.shape[0]:
+            _lib.launch_count[0] += 2
+        return out
 
     def read(self, page_table: torch.Tensor, slots: torch.Tensor, seq_lens: torch.Tensor, starts: torch.Tensor,
              cu_seqlens: torch.Tensor, n_tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -121,5 +125,7 @@ class PagedCache:
         [n_tokens, Hkv, 128] is token starts[b] + i of sequence b.  n_tokens is
         cu_seqlens[-1], known to the caller; positions outside a sequence read
         as NaN.  Feeds prompt_attention with the tokens before a chunk."""
-        _lib.launch_count[0] += 1
-        return _host.read(self._c, page_table, slots, seq_lens, starts, cu_seqlens, n_tokens)
+        out = _host.read(self._c, page_table, slots, seq_lens, starts, cu_seqlens, n_tokens)
+        if n_tokens and seq_lens.shape[0]:
+            _lib.launch_count[0] += 1
+        return out

@@ -35,5 +35,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     defaults to 128 ** -0.5.  Returns out [Tq, Hq, 128]; lse (optional, fp32
     [Tq, Hq]) receives the log2-sum-exp2 of the scaled logits.  Rows past
     cu_seqlens[-1] are not written."""
-    _lib.launch_count[0] += 1
-    return _host.prompt(q, k, v, cu_seqlens, cu_seqlens_k, scale, causal, out, lse)
+    out = _host.prompt(q, k, v, cu_seqlens, cu_seqlens_k, scale, causal, out, lse)
+    if q.shape[0] and cu_seqlens.shape[0] > 1:
+        _lib.launch_count[0] += 1
+    return out

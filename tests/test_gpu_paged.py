@@ -630,3 +630,38 @@ def test_sums_over_long_contexts_do_not_depend_on_how_codes_are_spread(dtype, le
     if along:
         n = len(along)
         assert abs(sum(along) / n) <= 4 * sum(size_of_rounding) / n / n ** 0.5 + 5e-5, (sum(along) / n, sum(size_of_rounding) / n)
+
+
+def test_launches_are_counted_where_kernels_are_launched():
+    """Calls that are refused or have nothing to do count no launches."""
+    from innerq_b200 import _lib
+    from innerq_b200.paged import PagedCache
+    from innerq_b200.prompt import prompt_attention
+    c = PagedCache.allocate(4, 2, 2, 64, 32, 32)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    x = lambda n, h: torch.zeros((n, h, D), dtype=torch.float16, device="cuda")  # noqa: E731
+    tab, sl, ln = i32(2, 3), i32(2), i32(2)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+
+    def count(call, error=None):
+        n = _lib.launch_count[0]
+        if error:
+            with pytest.raises(error):
+                call()
+        else:
+            call()
+        return _lib.launch_count[0] - n
+    assert count(lambda: c.attend(x(3, 4), tab, sl, ln), ValueError) == 0
+    assert count(lambda: c.attend(x(2, 5), tab, sl, ln), _lib.InnerqError) == 0
+    assert count(lambda: c.append(None, x(3, 2), x(3, 2), tab, sl, ln), ValueError) == 0
+    assert count(lambda: c.read(tab, sl, ln, ln, ln, 2), ValueError) == 0
+    assert count(lambda: prompt_attention(x(4, 3), x(4, 2), x(4, 2), cu), _lib.InnerqError) == 0
+    assert count(lambda: c.attend(x(0, 4), tab[:0], sl[:0], ln[:0])) == 0
+    assert count(lambda: c.append(None, x(0, 2), x(0, 2), tab, sl, ln, i32(3))) == 0
+    assert count(lambda: c.read(tab, sl, ln, ln, i32(3), 0)) == 0
+    assert count(lambda: prompt_attention(x(0, 4), x(0, 2), x(0, 2), cu)) == 0
+    assert count(lambda: c.append(None, x(2, 2), x(2, 2), tab, sl, ln)) == 1
+    assert count(lambda: c.append(None, x(2, 2), x(2, 2), tab, sl, ln, cu)) == 2
+    assert count(lambda: c.attend(x(2, 4), tab, sl, ln)) == 2
+    assert count(lambda: c.read(tab, sl, ln, ln, cu, 2)) == 1
+    assert count(lambda: prompt_attention(x(2, 4), x(2, 2), x(2, 2), cu)) == 1
