@@ -7,8 +7,10 @@
 // Every function raises TypeError / ValueError / NotImplementedError for bad
 // arguments before any launch, and innerq_b200._lib.InnerqError for a status
 // of the C ABI.  Inputs whose rows are not contiguous and 16-byte aligned are
-// copied first.  Work goes to the current stream of the tensors' device.
+// copied first; an output of prompt attention with such rows is written through
+// a copy.  Work goes to the current stream of the tensors' device.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
@@ -119,12 +121,13 @@ Tensor index(const Tensor& t, const char* what, int64_t n, at::Device device) {
   return t.stride(0) == 1 ? t : t.contiguous();
 }
 
-// a given output: like the query, contiguous rows
+// a given output: like the query, contiguous rows that do not overlap
 Tensor output(PyObject* o, const Tensor& q) {
   if (o == Py_None) return at::empty(q.sizes(), q.options());
   const Tensor& t = tensor(o, "out");
   if (t.sizes() != q.sizes() || t.scalar_type() != q.scalar_type() || t.device() != q.device() || t.stride(2) != 1)
     throw Raise{PyExc_ValueError, "out must be like the query, with contiguous rows"};
+  if (at::has_internal_overlap(t) == at::MemOverlap::Yes) throw Raise{PyExc_ValueError, "rows of out overlap"};
   return t;
 }
 float* lse_of(PyObject* o, const Tensor& q) {
@@ -352,7 +355,10 @@ PyObject* prompt(PyObject* const* a) {
   p.scale = scale_of(a[5]);
   p.causal = truth(a[6]);
   const c10::cuda::CUDAGuard guard(device);
-  Tensor out = output(a[7], q);
+  const Tensor given = output(a[7], q);
+  // rows that the kernel cannot write in 16-byte pieces: through a copy
+  const bool fits = given.stride(0) % 8 == 0 && given.stride(1) % 8 == 0 && (uintptr_t)given.data_ptr() % 16 == 0;
+  const Tensor out = fits ? given : given.clone(at::MemoryFormat::Contiguous);
   p.lse = lse_of(a[8], q);
   p.D = q.size(2);
   p.B = cu.size(0) - 1;
@@ -375,7 +381,8 @@ PyObject* prompt(PyObject* const* a) {
   p.o_st = out.stride(0);
   p.o_sh = out.stride(1);
   check(f_prompt(&p, stream_of(device)), "innerq_prompt_attn");
-  return THPVariable_Wrap(std::move(out));
+  if (!fits) given.copy_(out);
+  return THPVariable_Wrap(given);
 }
 
 // ------------------------------------------------------------------ module ---

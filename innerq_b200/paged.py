@@ -111,7 +111,8 @@ class PagedCache:
                lse: torch.Tensor | None = None) -> torch.Tensor:
         """Decode attention: q [B, Hq, 128], one query token per sequence,
         over its seq_lens[b] cached tokens (this step's included) -> out
-        [B, Hq, 128].  A sequence without tokens gets zeros.  lse (optional,
+        [B, Hq, 128] (given: contiguous rows, any strides, apart from q).  A
+        sequence without tokens gets zeros.  lse (optional,
         fp32 [B, Hq]): log2-sum-exp2 of the scaled logits."""
         out = _host.attend(self._c, q, page_table, slots, seq_lens, scale, out, lse)
         if q.shape[0]:

@@ -32,7 +32,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     cu_seqlens[b] .. cu_seqlens[b + 1] and the keys cu_seqlens_k[b] ..
     cu_seqlens_k[b + 1] (default: the same).  causal: query i of nq sees the
     keys j <= i + nk - nq.  A query that sees no key gets zeros.  scale
-    defaults to 128 ** -0.5.  Returns out [Tq, Hq, 128]; lse (optional, fp32
+    defaults to 128 ** -0.5.  Returns out [Tq, Hq, 128] (given: contiguous
+    rows, any token and head stride, apart from the inputs); lse (optional, fp32
     [Tq, Hq]) receives the log2-sum-exp2 of the scaled logits.  Rows past
     cu_seqlens[-1] are not written."""
     out = _host.prompt(q, k, v, cu_seqlens, cu_seqlens_k, scale, causal, out, lse)

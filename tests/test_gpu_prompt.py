@@ -283,3 +283,30 @@ def test_infinite_values_with_small_probabilities(n, causal, dtype):
                        torch.where(sees(n - 3), 7.0, torch.where(sees(7), 8.0, clean[..., 19])))
     keep = [d for d in range(D) if d not in (16, 17, 18, 19)]
     assert torch.equal(got[..., keep], clean[..., keep])
+
+
+@pytest.mark.parametrize("lo,hi", [(64, 192), (5, 133), (1, 129)])
+def test_a_given_output_may_have_any_strides(lo, hi):
+    """Rows that begin anywhere, as in the cache's attend; what lies between
+    them and the rows past the last sequence are left alone."""
+    from innerq_b200.prompt import prompt_attention
+    n = [130, 31]
+    q, k, v = data([170], [170], 4, 2, "fp16", seed=25)
+    want = prompt_attention(q, k, v, cu(n))[:161]
+    wide = torch.full((170, 4, 257), 3.0, dtype=torch.float16, device="cuda")
+    out = wide[..., lo:hi]
+    assert prompt_attention(q, k, v, cu(n), out=out) is not None
+    assert torch.equal(out[:161], want)
+    assert (wide[161:] == 3).all() and (wide[..., :lo] == 3).all() and (wide[..., hi:] == 3).all()
+
+
+def test_an_output_whose_rows_overlap_is_refused():
+    from innerq_b200.paged import PagedCache
+    from innerq_b200.prompt import prompt_attention
+    q, k, v = data([3], [3], 4, 2, "fp16")
+    with pytest.raises(ValueError):
+        prompt_attention(q, k, v, cu([3]), out=torch.zeros((3, 1, D), dtype=torch.float16, device="cuda").expand(3, 4, D))
+    c = PagedCache.allocate(1, 2, 3, 32, 0, 32)
+    i32 = torch.zeros(3, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        c.attend(q, i32[:, None], i32, i32, out=torch.zeros((1, 4, D), dtype=torch.float16, device="cuda").expand(3, 4, D))
