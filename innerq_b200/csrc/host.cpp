@@ -32,6 +32,9 @@ struct Raise {
   std::string text;
 };
 
+// a Python error that is set already
+struct Pending {};
+
 // entry points of the library, resolved by bind()
 decltype(&innerq_paged_append) f_append = nullptr;
 decltype(&innerq_paged_read) f_read = nullptr;
@@ -88,7 +91,11 @@ int64_t integer(PyObject* o, const char* what) {
   }
   return v;
 }
-bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Pending{};
+  return v == 1;
+}
 
 float scale_of(PyObject* o) {
   if (o == Py_None) return 1.f / std::sqrt((float)kD);
@@ -413,6 +420,7 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
     PyErr_SetString(r.type, r.text.c_str());
   } catch (const Failed& f) {
     return raise(f);
+  } catch (const Pending&) {
   } catch (const c10::OutOfMemoryError& e) {
     PyObject* torch = PyImport_ImportModule("torch");
     PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;

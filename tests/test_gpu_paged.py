@@ -665,3 +665,22 @@ def test_launches_are_counted_where_kernels_are_launched():
     assert count(lambda: c.attend(x(2, 4), tab, sl, ln)) == 2
     assert count(lambda: c.read(tab, sl, ln, ln, cu, 2)) == 1
     assert count(lambda: prompt_attention(x(2, 4), x(2, 2), x(2, 2), cu)) == 1
+
+
+def test_switches_without_a_truth_value_raise():
+    """What has no truth value raises its own error, before any launch."""
+    from innerq_b200.paged import PagedCache
+    from innerq_b200.prompt import prompt_attention
+    c = PagedCache.allocate(1, 1, 1, 32, 0, 32)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    x = torch.zeros((1, 1, D), dtype=torch.float16, device="cuda")
+    cs = torch.ones((4, 64), device="cuda")
+    many = torch.ones(2)
+    c.dense_k.fill_(5)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        c.append(x, x, x, i32(0)[None], i32(0), i32(0), cos=cs, sin=cs, interleaved=many)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        c.append(x, x, x, i32(0)[None], i32(0), i32(0), return_k=many)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        prompt_attention(x, x, x, i32(0, 1), causal=many)
+    assert (c.dense_k == 5).all()
