@@ -65,10 +65,17 @@ class Server:
         self.model, self.chunk = model, chunk
         self.caches = [PagedCache.allocate(n_pages, model.kv_heads, n_slots, page_size, w_sink, w_recent, model.dtype)
                        for _ in model.layers]  # one table serves every layer
+        self.n_pages = n_pages
         self.free_pages, self.free_slots = list(range(n_pages)), list(range(n_slots))
         self.waiting, self.running = [], []
 
     def submit(self, prompt, new_tokens):
+        """Queue a request; one that could never be served raises."""
+        total = len(prompt) + new_tokens
+        if not len(prompt) or new_tokens < 1:
+            raise ValueError(f"a request needs tokens before and after: {len(prompt)} and {new_tokens}")
+        if self.caches[0].pages_for(total) > self.n_pages or total - 1 > len(self.model.cos):
+            raise ValueError(f"{total} tokens do not fit {self.n_pages} pages or {len(self.model.cos)} positions")
         r = Request(prompt, new_tokens)
         self.waiting.append(r)
         return r

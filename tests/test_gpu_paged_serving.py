@@ -67,3 +67,19 @@ def test_prompts_in_chunks_match_whole_prompts():
     for o in out[1:]:
         # the same products in another order: a few steps of fp16 of the largest logit
         assert float((o - out[0]).abs().max()) <= 2.0 ** -8 * float(out[0].abs().max())
+
+
+def test_requests_that_can_never_be_served_are_refused():
+    """A request without tokens, or that needs more pages or positions than
+    there are, would wait for ever and everything behind it too."""
+    from examples.paged_serving import Decoder, Server
+    model = Decoder(layers=1, heads=2, kv_heads=1, hidden=64, vocab=50, max_pos=300, dtype=torch.float16, seed=5)
+    s = Server(model, n_pages=4, n_slots=2, page_size=32, w_sink=32, w_recent=32, chunk=64)
+    for prompt, new in (([], 4), ([1], 0), ([1] * 150, 100), ([1] * 290, 12)):
+        with pytest.raises(ValueError):
+            s.submit(prompt, new)
+    assert not s.waiting
+    r = s.submit([1] * 150, 45)  # 195 tokens, 128 of them packed: all four pages
+    for _ in range(60):
+        s.step()
+    assert len(r.tokens) == 195 and not s.running and len(s.free_pages) == 4
