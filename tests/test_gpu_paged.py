@@ -554,8 +554,8 @@ def test_infinite_values_of_the_16_bit_tokens(length, dtype):
     assert torch.equal(got[:, keep], clean[:, keep])
 
 
-def held(c, pages, length):
-    """What a cache holds of the sequence of slot 0, [length, H, D] in 64 bits."""
+def held(c, pages, length, slot=0):
+    """What a cache holds of a sequence, [length, H, D] in 64 bits."""
     t, d = torch.arange(32, device="cuda")[:, None], torch.arange(D, device="cuda")[None]
     H, dt, sink = c.n_kv_heads, c.dtype, c.w_sink
     n = c.packed_tokens(length)
@@ -568,13 +568,14 @@ def held(c, pages, length):
     k = code(0, ((t // 8 * 8 + t % 8) * 4 + l) * 4 + g, m) * scale(2048)[..., (t % 8 * 4 + t // 8) * 4 + g]
     word = (((d // 4 % 4 * 8 + d // 16) * 4 + t % 8 // 2) * 2 + d // 2 % 2) * 2 + d % 2
     v = code(2304, word, t // 8 + 4 * (t % 2)) * scale(4352)[..., None, :]
-    at = torch.cat([torch.arange(min(sink, length)), torch.arange(sink + n, length)]).cuda()
+    at = torch.cat([torch.arange(min(sink, length)), torch.arange(min(sink + n, length), length)]).cuda()
     row = torch.where(at < sink, at, sink + (at - sink) % (c.w_recent + 32))
     out = []
     for packed, dense in ((k, c.dense_k), (v, c.dense_v)):
         x = torch.empty((length, H, D), dtype=torch.float64, device="cuda")
-        x[sink:sink + n] = packed.reshape(H, n, D).transpose(0, 1)
-        x[at] = dense[0][:, row].transpose(0, 1).double()
+        if n:
+            x[sink:sink + n] = packed.reshape(H, n, D).transpose(0, 1)
+        x[at] = dense[slot][:, row].transpose(0, 1).double()
         out.append(x)
     return out
 
@@ -684,3 +685,50 @@ def test_switches_without_a_truth_value_raise():
     with pytest.raises(RuntimeError, match="ambiguous"):
         prompt_attention(x, x, x, i32(0, 1), causal=many)
     assert (c.dense_k == 5).all()
+
+
+@pytest.mark.parametrize("dtype,page,sink,recent,longest", [("fp16", 64, 32, 96, 20000), ("bf16", 128, 0, 32, 60000),
+                                                           ("fp16", 32, 0, 0, 3000)])
+def test_every_tile_of_a_ragged_batch_counts_once(dtype, page, sink, recent, longest):
+    """Bounds that shrink with the context, so that a tile missed, taken twice
+    or weighted wrongly where the work is cut shows: it changes lse by 32 / n
+    and the output by far more than its own size allows.  An element's error is
+    at most the output's rounding and 2^-11 of sum p |v| and of the output (the
+    probabilities' rounding, above and below the line).  Where at least 100
+    tokens share the weight, the rounding of the probabilities is a random walk
+    of steps of at most 2^-11 / sqrt 3 of p v, and a row's root mean square stays
+    within 1.25 of both together.  The log-sum-exp is off by at most 2^-11 log2 e
+    (the sum of the rounded probabilities), and by a walk of a tenth of that,
+    below 1e-4, where 100 tokens share the weight."""
+    from innerq_b200.paged import PagedCache
+    dt, H, R = DT[dtype], 2, 3
+    g = torch.Generator(device="cuda").manual_seed(26)
+    r = np.random.RandomState(26)
+    lens = np.concatenate([[1, 31, 33, longest], np.exp(r.uniform(0, np.log(longest), 20)).astype(int)])
+    r.shuffle(lens)
+    B, cols = len(lens), longest // page + 1
+    tab = torch.from_numpy(r.permutation(B * cols).reshape(B, cols).astype(np.int32)).cuda()
+    slots = torch.from_numpy(r.permutation(B).astype(np.int32)).cuda()
+    c = PagedCache.allocate(B * cols, H, B, page, sink, recent, dt)
+    T = int(lens.sum())
+    i32 = lambda x: torch.from_numpy(np.asarray(x, np.int32)).cuda()  # noqa: E731
+    k, v = (torch.randn((T, H, D), device="cuda", generator=g).to(dt) for _ in range(2))
+    c.append(None, k, v, tab, slots, i32(np.zeros(B)), i32(np.concatenate([[0], np.cumsum(lens)])))
+    q = (torch.randn((B, H * R, D), device="cuda", generator=g) * torch.tensor([0.0, 0.3, 1.0] * H, device="cuda")[:, None]).to(dt)
+    lse = torch.empty((B, H * R), device="cuda")
+    out = c.attend(q, tab, slots, i32(lens), lse=lse).double()
+    for b, n in enumerate(lens):
+        kk, vv = held(c, tab[b], int(n), int(slots[b]))
+        for h in range(H):
+            rows = slice(h * R, h * R + R)
+            s = q[b, rows].double() @ kk[:, h].T * D ** -0.5
+            p = torch.softmax(s, -1)
+            want = p @ vv[:, h]
+            err = (out[b, rows] - want).abs()
+            many = p.square().sum(-1) < 0.01
+            off = (lse[b, rows].double() - torch.logsumexp(s, -1) / math.log(2)).abs()
+            assert bool((off < torch.where(many, 1e-4, 2.0 ** -11 * math.log2(math.e) + 1e-5)).all()), (b, n, off)
+            assert bool((err <= ULP[dtype] * want.abs() + 2.0 ** -11 * (p @ vv[:, h].abs() + want.abs()) + 1e-6).all()), (b, n)
+            walk = (p.square() @ vv[:, h].square()).sqrt()
+            expect = ((ULP[dtype] * want).square() + (2.0 ** -11 * walk).square()).mean(-1).div(3).sqrt()
+            assert bool((err.square().mean(-1).sqrt() <= 1.25 * expect + 1e-6)[many].all()), (b, n)

@@ -310,3 +310,40 @@ def test_an_output_whose_rows_overlap_is_refused():
     i32 = torch.zeros(3, dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError):
         c.attend(q, i32[:, None], i32, i32, out=torch.zeros((1, 4, D), dtype=torch.float16, device="cuda").expand(3, 4, D))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("nq,nk,hq,hkv", [([900, 40], [900, 40], 4, 2), ([1030], [1030], 5, 1), ([2500, 1, 1301], [2500, 1, 1301], 2, 1),
+                                          ([300, 77], [4000, 1205], 4, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_every_key_counts_once(nq, nk, hq, hkv, causal, dtype):
+    """Bounds that shrink with the context: an element's error is at most the
+    output's rounding and that of the probabilities, in sum p |v|.  Where at
+    least 100 keys share the weight the latter is a random walk, of steps of at
+    most the type's half step / sqrt 3 of p v, and a row's root mean square
+    stays within 1.35 of both together (128 channels scatter by a sixteenth; the
+    largest of some ten thousand rows by five of those): a single key missed or taken twice is several times
+    that.  The log-sum-exp is within 1e-4."""
+    from innerq_b200.prompt import prompt_attention
+    q, k, v = data(nq, nk, hq, hkv, dtype, seed=27)
+    q *= 0.5
+    lse = torch.empty(q.shape[:2], device="cuda")
+    out = prompt_attention(q, k, v, cu(nq), cu(nk), causal=causal, lse=lse).double()
+    R, o, x = hq // hkv, 0, 0
+    for a, b in zip(nq, nk):
+        i, j = torch.arange(a, device="cuda")[:, None], torch.arange(b, device="cuda")
+        for h in range(hq):
+            vv = v[x:x + b, h // R].double()
+            s = q[o:o + a, h].double() @ k[x:x + b, h // R].double().T * D ** -0.5
+            if causal:
+                s = s.masked_fill(j > i + b - a, float("-inf"))
+            p = torch.softmax(s, -1)
+            want = p @ vv
+            err = (out[o:o + a, h] - want).abs()
+            assert float((lse[o:o + a, h].double() - torch.logsumexp(s, -1) / np.log(2.0)).abs().max()) < 1e-4
+            assert bool((err <= ULP[dtype] * (want.abs() * 1.01 + p @ vv.abs()) + 1e-6).all())
+            walk = (p.square() @ vv.square()).sqrt()
+            expect = ((ULP[dtype] * want).square() + (ULP[dtype] * walk).square()).mean(-1).div(3).sqrt()
+            many = p.square().sum(-1) < 0.01
+            assert bool((err.square().mean(-1).sqrt() <= 1.35 * expect + 1e-6)[many].all())
+        o, x = o + a, x + b
