@@ -1,7 +1,8 @@
 """ctypes binding of libinnerq_b200.so (the C ABI in include/innerq_b200.h).
 
-This is the same binding a Python caller of the C ABI would write; the
-package's host code calls the library only through it.  Importing works
+This is the same binding a Python caller of the C ABI would write.  The
+package's host code calls the library through it, the paged cache and prompt
+attention through ``csrc/host.cpp`` (``host()`` below).  Importing works
 without a GPU (the CPU test-suite checks the exports); calling a compute entry
 point needs CUDA tensors.  There is no fallback: a missing library raises.
 """
@@ -80,8 +81,8 @@ class AttnArgs(C.Structure):
 
 
 # innerq_paged, innerq_paged_new and innerq_prompt_args, field by field in the
-# header's order, as struct formats: packing them in one call instead of
-# assigning ctypes fields keeps host time per launch low.
+# header's order, as struct formats, for callers of the C ABI through ctypes
+# (the package's own calls fill the structs in csrc/host.cpp).
 PAGED_FORMAT = struct.Struct("@11i4x3PPqPP")
 PAGED_NEW_FORMAT = struct.Struct("@6i" + "Pqq" * 3 + "3Pq" + "Pqq" * 2)
 PROMPT_FORMAT = struct.Struct("@9if" + "Pqq" * 3 + "2P" + "Pqq" + "P")
@@ -157,13 +158,13 @@ def host():
     return _host
 
 
-# kernels each compute entry point launches (for launch accounting in bench.py)
+# kernels each compute entry point launches (for launch accounting in bench.py;
+# innerq_b200.paged and innerq_b200.prompt count their own)
 KERNELS_PER_CALL = {
     "innerq_norm_factor": 1, "innerq_quant_pack": 1, "innerq_unpack_ref": 1, "innerq_dequant": 1,
     "innerq_dequant_ref": 1, "innerq_decode_attn": 3, "innerq_decode_attn_partials": 2,
     "innerq_lse_merge": 1, "innerq_decode_attn_noalloc": 3, "innerq_append_step": 1,
-    "innerq_lse_merge_ranks": 1, "innerq_paged_append": 1, "innerq_paged_read": 1,
-    "innerq_paged_attn": 2, "innerq_prompt_attn": 1,
+    "innerq_lse_merge_ranks": 1,
 }
 launch_count = [0]
 

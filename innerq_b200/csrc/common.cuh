@@ -228,6 +228,11 @@ template <> struct Pair<BF16> {
   using T = __nv_bfloat162;
   static constexpr uint32_t kOne = 0x3f803f80u, kBase = 0x43004300u;  // 1.0, 128.0
 };
+// the low 16 bits of h, as a number of the dtype, are an infinity or a NaN
+template <int DT> __device__ __forceinline__ bool not_finite(uint32_t h) {
+  constexpr uint32_t e = DT == F16 ? 0x7c00u : 0x7f80u;
+  return (h & e) == e;
+}
 template <int DT> __device__ __forceinline__ typename Pair<DT>::T as_pair(uint32_t w) {
   return *reinterpret_cast<const typename Pair<DT>::T*>(&w);
 }

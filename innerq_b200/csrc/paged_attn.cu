@@ -358,10 +358,6 @@ __device__ __forceinline__ void packed_values(const uint8_t* blk, int lane, cons
   }
 }
 
-template <int DT> __device__ __forceinline__ bool not_finite(uint32_t h) {
-  constexpr uint32_t e = DT == F16 ? 0x7c00u : 0x7f80u;
-  return (h & e) == e;
-}
 template <int DT> __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   return w & ((not_finite<DT>(w) ? 0u : 0xffffu) | (not_finite<DT>(w >> 16) ? 0u : 0xffff0000u));
 }

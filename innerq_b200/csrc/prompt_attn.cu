@@ -171,11 +171,6 @@ template <int DT> __device__ __forceinline__ uint32_t pack_p(float a, float b) {
   return r;
 }
 
-template <int DT> __device__ __forceinline__ bool not_finite(uint32_t h) {
-  constexpr uint32_t e = DT == F16 ? 0x7c00u : 0x7f80u;
-  return (h & e) == e;
-}
-
 // The work of block `block` (the last queries of a sequence see the most keys:
 // heavy blocks first); one warp.  False: none, the grid is an upper bound.
 __device__ __forceinline__ bool decode(const PromptDev& a, int block, int lane, Work& w) {
