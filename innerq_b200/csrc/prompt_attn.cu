@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // a row that sees no key is 0; one that does, but whose logits are all
         // -inf, is 0 / 0
-        const float inv = !ok ? NAN : l != 0.f ? 1.f / l : lim > 0 ? NAN : 0.f;
+        const float inv = !ok ? NAN : lim <= 0 ? 0.f : l != 0.f ? 1.f / l : NAN;
         uint16_t* out = a.out + (int64_t)(w->q_base + qi) * a.o_st + head * a.o_sh;
         const bool odd = write_rows<DT>(to, n > 0, inv, real ? out : nullptr, lane);
         tc_fence_before();
@@ -733,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (a.lse && real)
-          a.lse[(int64_t)(w->q_base + qi) * a.Hq + head] = l == 0.f ? -INFINITY : m - kShift + log2f(l);
+          a.lse[(int64_t)(w->q_base + qi) * a.Hq + head] = l == 0.f || lim <= 0 ? -INFINITY : m - kShift + log2f(l);
       }
       if (!ok) break;
       pieces.done(lane);
@@ -820,7 +820,8 @@ extern "C" int innerq_prompt_attn(const innerq_prompt_args* p, void* stream) {
   a.out = (uint16_t*)p->out;
   a.lse = p->lse;
   // a scale of 0 weighs all keys alike; masked logits are -inf, and -inf * 0 is NaN
-  a.scale_log2 = std::max(1e-37f, (p->scale < 0 ? -p->scale : p->scale) * 1.4426950408889634f);
+  a.scale_log2 = (p->scale < 0 ? -p->scale : p->scale) * 1.4426950408889634f;
+  if (a.scale_log2 < 1e-37f) a.scale_log2 = 1e-37f;  // (NaN stays)
   a.negate = p->scale < 0;
   a.B = p->B; a.Hq = p->Hq; a.Hkv = p->Hkv; a.Tq = p->Tq; a.Tk = p->Tk; a.causal = p->causal;
   // The rows of a query tile are tokens times the query heads that share their

@@ -347,3 +347,15 @@ def test_every_key_counts_once(nq, nk, hq, hkv, causal, dtype):
             many = p.square().sum(-1) < 0.01
             assert bool((err.square().mean(-1).sqrt() <= 1.35 * expect + 1e-6)[many].all())
         o, x = o + a, x + b
+
+
+@pytest.mark.parametrize("n,nk", [(40, 30), (300, 290)])
+def test_a_scale_that_is_not_a_number(n, nk):
+    """NaN for every query that sees a key, as in the cache's attend, zeros for
+    the others."""
+    from innerq_b200.prompt import prompt_attention
+    q, k, v = data([n], [nk], 4, 2, "fp16", seed=28)
+    lse = torch.zeros(q.shape[:2], device="cuda")
+    out = prompt_attention(q, k, v, cu([n]), cu([nk]), scale=float("nan"), lse=lse)
+    assert torch.isnan(out[10:]).all() and torch.isnan(lse[10:]).all()
+    assert (out[:10] == 0).all() and torch.isneginf(lse[:10]).all()
