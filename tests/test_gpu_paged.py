@@ -732,3 +732,25 @@ def test_every_tile_of_a_ragged_batch_counts_once(dtype, page, sink, recent, lon
             walk = (p.square() @ vv[:, h].square()).sqrt()
             expect = ((ULP[dtype] * want).square() + (2.0 ** -11 * walk).square()).mean(-1).div(3).sqrt()
             assert bool((err.square().mean(-1).sqrt() <= 1.25 * expect + 1e-6)[many].all()), (b, n)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_same_inputs_same_bits(dtype):
+    """Append, read-back and attention repeat themselves bit for bit, whatever
+    ran between."""
+    s = Server(7, 2, dtype, 32, 96, 64, 9000, seed=29)
+    s.step([8500, 1, 77, 3000, 129, 640, 33], 10)
+    q = torch.randn((7, 10, D), device="cuda", generator=s.g).to(s.dt)
+    lens = s.dev(s.lens)
+    first = s.cache.attend(q, s.table, s.slots, lens)
+    other = Server(3, 1, dtype, 0, 32, 32, 4000, seed=30)
+    for fill in (1e4, float("nan"), 0.0):
+        def values(k, v):
+            k[:], v[:] = fill, fill
+        other.lens[:] = 0
+        other.oracle = Oracle(0, 32, other.dt)
+        other.rot = 0
+        other.step([3000, 50, 1], kv=values)
+        other.cache.attend(torch.full((3, 8, D), fill, dtype=other.dt, device="cuda"), other.table, other.slots, other.dev(other.lens))
+        assert torch.equal(s.cache.attend(q, s.table, s.slots, lens), first)
+    s.check_read()
