@@ -13,11 +13,15 @@
 // is a single launch, and prompts take a second one for the rows.
 //
 // What bounds it: rotation moves bytes (q in and out), packing is instructions
-// (some 600 per 32 tokens, head and warp: seven exact cuts per group and 7
-// packed compares and adds per pair of values), so their blocks alternate in
-// one launch.  A prompt of 16384 tokens with 40 / 8 heads in bf16, 420 MB: 92 us
-// (4.6 TB/s); one block per token and one per (tile, head) took 140 us.  Eight
-// tokens per rotation block: 110 us with the read-back, four 114, sixteen 117.
+// (seven exact cuts per group, 7 packed compares and adds per pair of values),
+// so their blocks alternate in one launch.  A prompt of 16384 tokens with 40 / 8
+// heads in bf16, 464 MB: 95 us (4.9 TB/s; DRAM moves 420 MB of it).  Neither side
+// is full there: 52% of the issue slots, 30 warps per SM of which most wait for
+// loads (7.1 per instruction issued).  13 prompts of 11796 tokens, 290 MB: 58 us
+// (5.0 TB/s).  A decode step: 2.6 us for one sequence, 9.0 us for 128 (5.9 MB,
+// four of them completing a tile: latency of the packing blocks).  With the
+// read-back: one block per token and one per (tile, head) took 140 us; eight
+// tokens per rotation block 110 us, four 114, sixteen 117.
 // Sharing a group's cuts over its threads took packing from 63 to 50 us,
 // keeping a token's angles over its heads and exact batches of heads took
 // rotation from 95 to 65 us.
@@ -481,6 +485,10 @@ template <int DT> __device__ __forceinline__ uint32_t value2(uint32_t w, uint32_
 
 // Read-back: one block per head and tile of 32 positions.  Sink, packed part and
 // window begin and end at multiples of 32, so a tile is of one kind.
+// The windows of 128 sequences (16 bits, 8 heads, 127 MB): 24 us (5.3 TB/s);
+// 16384 packed tokens of one (86 MB): 17.7 us (4.9 TB/s).  Loads bound it (9.6 and
+// 5.8 warps wait for them per instruction issued) and, for packed tokens, 56% of
+// the issue slots.
 template <int DT>
 __global__ void __launch_bounds__(128, 8)
     read_kernel(PagedDev c, const int32_t* starts, const int32_t* cu, int n_tokens, uint16_t* ko, uint16_t* vo) {

@@ -29,7 +29,10 @@
 // 256 us where this takes 227.  With the low codes where they lie (217 us) the
 // cut is at 2^-16, the outliers' error was up to 4.5 times the rounding, and no
 // constant in place of the 8 helps all of them.  Logits keep the cheaper form:
-// their cut-off parts have the query's signs and sum to some 1e-5 of a logit.
+// only products with channels below a 64th of the query's largest are cut, and
+// what is lost has the query's signs.  Log-sum-exps are within 5e-5, and within
+// 3e-4 where a query's channels differ by factors of a thousand over keys with
+// outlier channels; the output's error is the same for all of these.
 //   16-bit tokens (sink, window) use the same MMAs on their own type, with ones,
 // and bf16 probabilities are split into two parts there.
 //
@@ -40,16 +43,17 @@
 // tile) and no synchronisation until a unit ends.  A unit inside one range is
 // written at once, the others leave fp32 partials that merge_kernel joins.
 //
-// What bounds it: 507 warp instructions per tile of 32 tokens (half of them
+// What bounds it: 566 warp instructions per tile of 32 tokens (half of them
 // bit operations that expand codes, 34 MMAs) against 4608 bytes, at 12 warps
-// per SM; issue slots are 55-60% busy and DRAM at 80% of a copy's rate.  32
-// sequences of 32768 tokens, 8 key heads, 1.22 GB: 216 us (5.6 TB/s), 245 us
-// when run back to back, where the board's power limit lowers the clocks; one
-// sequence of 4096 tokens: 10 us, of which the list takes 1.2, the first copy
-// 0.7, a tile 2, the join 1 and the merge 2.  Computing a tile's logits next to
-// the values of the tile before it took 224 us to 216.  Three CTAs of 168 registers with rings of
-// three beat four of 128 with rings of two (spills): 232 against 228-245 us,
-// and 73 against 84 us on 96 sequences of 1 to 20000 tokens.
+// per SM; issue slots are 59% busy and DRAM at 80% of a copy's rate.  32
+// sequences of 32768 tokens, 8 key heads, 1.22 GB: 227 us (5.4 TB/s), 251 to
+// 258 us when run back to back, where the board's power limit lowers the
+// clocks; one sequence of 4096 tokens: 10.6 us, of which (on an earlier state)
+// the list takes 1.2, the first copy 0.7, a tile 2, the join 1 and the merge 2.
+// Earlier states: a tile's logits next to the values of the tile before it took
+// 224 us to 216; three CTAs of 168 registers with rings of three against four of
+// 128 with rings of two (spills) 232 against 228-245 us, and 73 against 84 us on
+// 96 sequences of 1 to 20000 tokens.
 #include <algorithm>
 
 #include "async_ptx.cuh"
@@ -63,8 +67,8 @@ constexpr int kWarps = 4;
 constexpr int kStages = 3;
 constexpr int kCtasPerSm = 3;
 // what a unit costs beyond its tiles, in tiles: 96 sequences of 1 to 20000
-// tokens take 73.6 us with 12, 69.5 with 16, 71.2 with 24 (an earlier state of
-// the kernel 277 with 0, 123 with 4)
+// tokens take 75.7 us with 12, 71.9 with 16, 74.0 with 24 (an earlier state of
+// the kernel 277 with 0, 123 with 4); 32 of 32768 do not care (255 us)
 constexpr int kUnitCost = 16;
 constexpr int kHeadPitch = 148;  // floats per head of the combine buffer: conflict-free
 constexpr float kPScale = 8.f;   // probabilities carry 2^8 relative to the running maximum,

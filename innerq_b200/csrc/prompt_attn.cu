@@ -20,18 +20,19 @@
 //   warps 10, 11    look over the V tiles that some row must not see whole: a
 //                   masked probability is 0, but 0 * NaN is NaN, so values
 //                   that are not finite are set to 0 there and added again, in
-//                   the epilogue, to the rows that do see them
+//                   the epilogue, to the rows that do see them (as are, in
+//                   fp16, those that met a probability below what fp16 holds)
 // A CTA stays and takes over blocks that have not started (the grid is one block
 // per pair of query tiles and head, heavy ones first), so the loads and scores
 // of the next piece of work run under the epilogue of the last; warp 11 asks.
 // What bounds it: per key tile of a pair the four products take 2048 cycles of
 // the tensor core at least, the exponentials about as many of the special
 // function units, and a tile's chain (scores, softmax, P V) some 3200, 2000 of
-// them softmax; two tiles overlap it to 59% tensor occupancy (special functions
+// them softmax; two tiles overlap it to 58% tensor occupancy (special functions
 // 45%, issue slots 47%), and without any product the rest alone takes 0.82 of
-// the time.  One prompt of 8192 tokens, 32 heads, bf16: 435 us (1260 TFLOP/s),
-// 497 us back to back at the board's power limit (1.57 GHz); 16 prompts of 1 to
-// 300 tokens: 17 us.  Two warps per 32 rows, each with half of the columns, are
+// the time.  One prompt of 8192 tokens, 32 heads, bf16: 442 us (1245 TFLOP/s),
+// 503 to 514 us back to back at the board's power limit; 16 prompts of 1 to 300
+// tokens: 17 us.  Two warps per 32 rows, each with half of the columns, are
 // slower (485 us: the halves have to meet for every maximum).
 // Tensor memory: S0 | S1 | O0 | O1, 128 columns each.  In-order execution of
 // the MMAs makes "S_i(j + 1) is complete" mean that O_i is at rest too.
